@@ -357,8 +357,7 @@ def _evict(st):
     if own:
         from sycl_minimax_h3_b200 import ops
 
-        ops.kv_evict(_cache(st), st["spare"], case["budget"], sinks=case["sinks"], recent=case["recent"],
-                     max_len=max(case["lo"], case["hi"]))
+        ops.kv_evict(_cache(st), st["spare"], case["budget"], sinks=case["sinks"], recent=case["recent"])
     else:
         _plain_evict(st)
     r = st["region"]
