@@ -207,6 +207,74 @@ int h3s_selftest_wait_timeout(void* ctx, uint64_t wait_ns);
 int h3s_attention_sage_static(void* stream, const void* q, const void* k, const void* v, int64_t S, int64_t H, int64_t D,
                               int64_t stride, void* out, int out_dt, int* err);
 
+/* ---- the text model token by token: an 8-bit key/value cache and 4-bit linear layers ------------------------------ */
+
+/* No counterpart in the reference, whose text encoder reads a whole prompt at once (h3s_attention_causal). These serve
+ * a text model with grouped heads over sequences that grow. None of them allocates or waits for anything, so a CUDA
+ * graph can hold them; the lengths, tables and counts that they go by live on the device and may change between
+ * replays. Scratch is the caller's (work).
+ *
+ * The cache of `seqs` sequences: pages of 64 tokens with one float scale per page and head, in a pool that the sequences
+ * share through `table`; the tokens of a sequence that do not fill a page yet are in its tail, in the rows' own type dt.
+ * Token (slot) s of sequence b, head h: s < 64 * (lens[b] / 64): page table[b, s / 64], value code * scale, in float;
+ * else tail row s % 64. Which pages are free is the caller's to keep. A page id outside the pool, or lens / starts out
+ * of range, is found by the kernels: that page counts as unseen (attention) or that sequence is left alone (the others),
+ * and the next h3s_wait returns -1. All arrays are contiguous; k, v, tail_k and tail_v start on 16 bytes. */
+typedef struct h3s_kv_cache {
+    int8_t *k, *v;             /* [pages, heads, 64, dim] codes */
+    float *k_scale, *v_scale;  /* [pages, heads] */
+    void *tail_k, *tail_v;     /* [seqs, heads, 64, dim] in dt */
+    float* weight;             /* [pages, heads, 64] the attention weight each token has received, or NULL */
+    float* tail_weight;        /* [seqs, heads, 64]; NULL with weight */
+    int32_t* table;            /* [seqs, width] page ids, of which a sequence uses the first lens / 64 */
+    int32_t* lens;             /* [seqs] tokens, those of the current call included */
+    int64_t pages, seqs, width, heads, dim;   /* dim 64 or 128; width < 2^25 */
+    int32_t dt;
+} h3s_kv_cache;
+
+/* Writes the last n = starts[b+1] - starts[b] of sequence b's lens[b] tokens, for every b: rows starts[b] ... of k and v
+ * (T rows of heads x dim, row r at element r * stride, type dt; starts int32 [seqs + 1], rows behind starts[seqs] are not
+ * read). A block of 64 slots that is full now goes to page table[b, slot / 64]: scale = a / 127 with a the largest finite
+ * magnitude of its 64 x dim values of a head, code = 127 x / a rounded to the nearest, half way to even (the exact ratio;
+ * an infinity takes +-127, a NaN 0). The rest goes to the tail, so that the result does not depend on how the tokens
+ * were spread over calls. A page that is written takes over its tokens' weights; a new token's is 0. max_new: what the
+ * largest n is about (0: T), for the division of the work; no n is wrong. */
+int h3s_kv_append(void* ctx, const h3s_kv_cache* kv, const void* k, const void* v, int64_t T, int64_t stride,
+                  const int32_t* starts, int64_t max_new);
+
+/* Causal attention with grouped heads over the cache: query row starts[b] + i (i < n; T rows of Hq x dim at stride qs,
+ * type dt) is token lens[b] - n + i of sequence b and sees the slots up to its own; query head h reads key/value head
+ * h / (Hq / heads), scores q.k / sqrt(dim). out [T, Hq * dim] in dt, rounded once from float; a row that sees nothing
+ * (lens[b] < n) is 0, rows behind starts[seqs] are left as they were. accumulate: weight[slot] += the sum of the slot's
+ * softmax weights over the rows and heads that read it (kv->weight needed). max_new, max_len: what the largest n and
+ * length are about (0: T, 64 * width), for the division of the work; none is wrong. work: work_bytes of device memory,
+ * at least h3s_attention_cached_work(...) of the same arguments, on 16 bytes, this call's own until it has run. */
+int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64_t T, int64_t Hq, int64_t qs,
+                         const int32_t* starts, int64_t max_new, int64_t max_len, void* out, int accumulate, void* work,
+                         uint64_t work_bytes);
+uint64_t h3s_attention_cached_work(void* ctx, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int64_t max_new,
+                                   int64_t max_len, int accumulate);
+
+/* Cuts every sequence longer than `budget` (a multiple of 64) to it. Each head keeps its own tokens: the first `sinks`,
+ * the last `recent`, and of the others those with the largest weight (of equal ones the earlier; a NaN counts least), in
+ * their order. They are quantised again, as h3s_kv_append does, into the pages spare [seqs, budget / 64], weights with
+ * them; then the first budget / 64 entries of the sequence's table and of its row of spare change places, and lens[b] =
+ * budget: the old pages are the next eviction's spare ones. Sequences up to the budget keep everything, spare included.
+ * A spare page belongs to no sequence and is named once. work: 4 * seqs * heads * budget bytes. */
+int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budget, int64_t sinks, int64_t recent,
+                 void* work, uint64_t work_bytes);
+
+/* A linear layer with 4-bit weights for a few rows of x, out = x . W^T + bias:
+ *   W[n, k] = scale[k / group, n] * (code[n, k] - zero[k / group, n])      code 0..15, zero NULL: 8
+ * x [M, K] in x_dt; scale and zero [ceil(K / group), N] in s_dt; bias float [N] or NULL; out [M, N] in out_dt, rounded
+ * once from float. group 32, 64, 128 or 0 (one scale per output). tiles: the codes as h3s_int4_pack lays them out, 16 *
+ * ceil(N / 16) * 64 * ceil(K / 64) / 2 bytes on 16 bytes. Any M is right; from some hundred rows on a matrix product on
+ * unpacked weights is faster. M, K or N <= 0: nothing to do, returns 0. */
+int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, const void* tiles, int64_t N,
+                    const void* scale, const void* zero, int s_dt, int group, const float* bias, void* out, int out_dt);
+/* codes uint8 [N, K / 2] (K even), input 2 i in the low four bits of byte i -> tiles, once per layer. */
+int h3s_int4_pack(void* ctx, const uint8_t* codes, int64_t N, int64_t K, void* tiles);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,7 +11,7 @@ def build(verbose: bool = False) -> None:
     cmd = ["make", "-C", os.path.join(HERE, "csrc")]
     if not verbose:
         cmd.insert(1, "-s")
-    subprocess.run(cmd, check=True)
+    subprocess.run(cmd + ["-j4"], check=True)
 
 
 if __name__ == "__main__":

@@ -32,6 +32,8 @@
 #include "causal.cuh"
 #include "int8lin.cuh"
 #include "ulysses.cuh"
+#include "kvcache.cuh"
+#include "int4lin.cuh"
 
 namespace {
 
@@ -61,7 +63,7 @@ struct Ctx {
     cudaStream_t cs = nullptr;                   // uploads (h3s_upload), made on first use
     std::mutex cs_mu;
     std::string name;
-    int* err = nullptr;                          // device error word of this context's kernels
+    int* err = nullptr;                          // device error words of this context's kernels: waits, indexes
     bool profile = false, poison = false;
     bool sage_want = true;
     int64_t sage_min_s = 8192;
@@ -142,15 +144,26 @@ bool init(Ctx& c) {
     if ((e = cudaStreamCreateWithPriority(&c.aux, cudaStreamNonBlocking, prio_high)) != cudaSuccess ||
         (e = cudaEventCreateWithFlags(&c.ev_fork, cudaEventDisableTiming)) != cudaSuccess ||
         (e = cudaEventCreateWithFlags(&c.ev_join, cudaEventDisableTiming)) != cudaSuccess ||
-        (e = cudaMalloc(&c.err, sizeof(int))) != cudaSuccess || (e = cudaMemset(c.err, 0, sizeof(int))) != cudaSuccess) {
+        (e = cudaMalloc(&c.err, 2 * sizeof(int))) != cudaSuccess ||
+        (e = cudaMemsetAsync(c.err, 0, 2 * sizeof(int), c.aux)) != cudaSuccess ||
+        (e = cudaStreamSynchronize(c.aux)) != cudaSuccess) {
         cuda_fail("context", e);
         return false;
     }
     return true;
 }
 
+// A context may be made while one of the caller's streams is being captured into a graph: nothing that it allocates is
+// queued on that stream, so this thread's calls need not be refused for the capture's sake.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 Ctx* make_ctx(int device, cudaStream_t st, bool own) {
     DeviceGuard g(device);
+    RelaxedCapture relaxed;
     auto* c = new Ctx;
     c->device = device;
     if (own) {
@@ -502,6 +515,45 @@ uint8_t* static_scratch(int dev) {
     return g_static_ptr[dev];
 }
 
+// ---- the 8-bit key/value cache (kvcache.cuh) -------------------------------------------------------------------------
+int kv_fail(const char* who, const std::string& why) {
+    g_err = std::string(who) + ": " + why;
+    return -1;
+}
+// Every refusal that the cache's own description can earn, before a context is looked at; 0 and `a` filled otherwise.
+int check_kv(const char* who, const h3s_kv_cache* kv, bool weights, KvArgs& a) {
+    if (!kv) return kv_fail(who, "no cache");
+    if (!check_dt(kv->dt)) return kv_fail(who, "unknown element type " + std::to_string(kv->dt));
+    if (kv->dim != 64 && kv->dim != 128) return kv_fail(who, "heads of 64 or 128 features (got " + std::to_string(kv->dim) + ")");
+    if (kv->pages < 0 || kv->seqs < 1 || kv->width < 0 || kv->heads < 1 || kv->pages > INT32_MAX || kv->seqs > INT32_MAX ||
+        kv->heads > INT32_MAX || kv->width >= (1 << 25) || kv->seqs > INT32_MAX / kv->heads)
+        return kv_fail(who, "the cache's sizes are out of range");
+    if ((kv->pages > 0 && (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale)) || !kv->tail_k || !kv->tail_v ||
+        (kv->width > 0 && !kv->table) || !kv->lens)
+        return kv_fail(who, "a part of the cache is null");
+    if (!aligned16(kv->k) || !aligned16(kv->v) || !aligned16(kv->tail_k) || !aligned16(kv->tail_v))
+        return kv_fail(who, "codes and tails must start on 16 bytes");
+    if (kv->pages > 0 ? !kv->weight != !kv->tail_weight : kv->weight && !kv->tail_weight) return kv_fail(who, "weight and tail_weight come together");
+    if (weights && !kv->tail_weight) return kv_fail(who, "the cache keeps no weights");
+    a.k = kv->k;
+    a.v = kv->v;
+    a.ks = kv->k_scale;
+    a.vs = kv->v_scale;
+    a.tk = kv->tail_k;
+    a.tv = kv->tail_v;
+    a.w = kv->weight;
+    a.tw = kv->tail_weight;
+    a.table = kv->table;
+    a.lens = kv->lens;
+    a.pages = kv->pages;
+    a.seqs = (int) kv->seqs;
+    a.width = (int) kv->width;
+    a.heads = (int) kv->heads;
+    a.dim = (int) kv->dim;
+    a.dt = kv->dt;
+    return 0;
+}
+
 // h3s_rms_rope's refusals (kernels/h3sycl.cpp:1279-1283)
 bool check_rope(const char* who, int64_t D, int rot_dim) {
     if (rot_dim < 0 || rot_dim > D || rot_dim % 2 != 0 || (D - rot_dim) % 2 != 0) {
@@ -653,11 +705,20 @@ int h3s_wait(void* ctx) {
     DeviceGuard g(c.device);
     cudaError_t e = cudaStreamSynchronize(c.st);
     if (e != cudaSuccess) return cuda_fail("h3s_wait", e);
-    int code = 0;
-    e = cudaMemcpy(&code, c.err, sizeof(int), cudaMemcpyDeviceToHost);
+    int codes[2] = {0, 0};
+    e = cudaMemcpy(codes, c.err, sizeof(codes), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return cuda_fail("h3s_wait", e);
+    const int code = codes[0];
+    if (code || codes[1]) cudaMemset(c.err, 0, sizeof(codes));
+    if (codes[1] && !code) {
+        g_err = std::string("h3s_wait: a call found ") +
+                (codes[1] == kErrPage ? "a page id outside the cache's pool"
+                 : codes[1] == kErrLen ? "lengths or row starts out of range"
+                                       : "a page id outside the cache's pool, and lengths or row starts out of range") +
+                "; what it names was left out";
+        return -1;
+    }
     if (code) {
-        cudaMemset(c.err, 0, sizeof(int));
         g_err = "h3s_wait: a wait inside a kernel gave up after " + std::to_string(c.wait_ns / 1000000) +
                 " ms (code " + std::to_string(code) + "); its results are not valid";
         return -1;
@@ -1110,6 +1171,151 @@ int h3s_attention_sage_static(void* stream, const void* q, const void* k, const 
     a.D = (int) D;
     if ((e = launch_sage(mq, mk, mv, a, st)) != cudaSuccess) return cuda_fail("h3s_attention_sage_static", e);
     return 0;
+}
+
+// ---- the text model's cache (kvcache.cu); refusals first, so that they need no context -------------------------------
+int h3s_kv_append(void* ctx, const h3s_kv_cache* kv, const void* k, const void* v, int64_t T, int64_t stride,
+                  const int32_t* starts, int64_t max_new) {
+    constexpr const char* who = "h3s_kv_append";
+    KvArgs a{};
+    if (check_kv(who, kv, false, a) != 0) return -1;
+    if (T <= 0) return 0;
+    if (!k || !v || !starts) return kv_fail(who, "a null pointer");
+    if (stride < kv->heads * kv->dim) return kv_fail(who, "the row stride is shorter than a row");
+    if (T > INT32_MAX) return kv_fail(who, "too many rows");
+    if (max_new <= 0 || max_new > T) max_new = T;
+    // the blocks of the longest sequence, as far as the grid goes; a CTA takes more of them where that is not all
+    const int64_t most = INT32_MAX / 2 / (kv->heads * kv->seqs);
+    if (most < 1) return kv_fail(who, "too many sequences and heads");
+    max_new = std::min(max_new, most * kPage);
+    auto& c = *static_cast<Ctx*>(ctx);
+    DeviceGuard g(c.device);
+    a.err = c.err + 1;
+    const bool vec = aligned16(k) && aligned16(v) && (stride * esize(kv->dt)) % 16 == 0;
+    const cudaError_t e = launch_kv_append(a, k, v, T, stride, starts, max_new, vec, c.st);
+    return e == cudaSuccess ? 0 : cuda_fail(who, e);
+}
+
+// The hints of an attention call made whole, and its division of the work; the same for the work's size and the call.
+static AttendPlan attend_hints(const Ctx& c, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int64_t& max_new, int64_t& max_len) {
+    if (max_new <= 0 || max_new > T) max_new = T;
+    const int64_t cap = kv->width * kPage + kPage - 1;
+    if (max_len <= 0 || max_len > cap) max_len = cap;
+    return attend_plan(c.n_sm, kv->seqs, kv->heads, Hq / kv->heads, T, max_new, max_len);
+}
+static uint64_t attend_bytes(const AttendPlan& p, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate) {
+    const uint64_t rows = (uint64_t) T * (uint64_t) Hq;
+    return (p.nz > 1 ? rows * p.nz * (kv->dim + 2) * 4 : 0) + (accumulate ? rows * 4 : 0);
+}
+static int check_attend(const char* who, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate, KvArgs& a) {
+    if (check_kv(who, kv, accumulate != 0, a) != 0) return -1;
+    if (Hq < 1 || Hq % kv->heads != 0) return kv_fail(who, "the query heads must be a multiple of the cache's heads");
+    if (T > INT32_MAX || Hq > INT32_MAX || (T > 0 && Hq > ((int64_t) 1 << 40) / T)) return kv_fail(who, "too many rows");
+    return 0;
+}
+
+uint64_t h3s_attention_cached_work(void* ctx, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int64_t max_new,
+                                   int64_t max_len, int accumulate) {
+    KvArgs a{};
+    if (check_attend("h3s_attention_cached_work", kv, T, Hq, accumulate, a) != 0 || T <= 0) return 0;
+    return attend_bytes(attend_hints(*static_cast<Ctx*>(ctx), kv, T, Hq, max_new, max_len), kv, T, Hq, accumulate);
+}
+
+int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64_t T, int64_t Hq, int64_t qs,
+                         const int32_t* starts, int64_t max_new, int64_t max_len, void* out, int accumulate, void* work,
+                         uint64_t work_bytes) {
+    constexpr const char* who = "h3s_attention_cached";
+    AttendArgs a{};
+    if (check_attend(who, kv, T, Hq, accumulate, a.kv) != 0) return -1;
+    if (T <= 0) return 0;
+    if (!q || !starts || !out) return kv_fail(who, "a null pointer");
+    if (qs < Hq * kv->dim) return kv_fail(who, "the row stride is shorter than a row");
+    auto& c = *static_cast<Ctx*>(ctx);
+    a.plan = attend_hints(c, kv, T, Hq, max_new, max_len);
+    const uint64_t need = attend_bytes(a.plan, kv, T, Hq, accumulate);
+    if (need > 0 && (!work || !aligned16(work) || work_bytes < need))
+        return kv_fail(who, "work of " + std::to_string(need) + " bytes on 16 bytes needed, " + std::to_string(work ? work_bytes : 0) + " given");
+    if (kv->seqs * kv->heads > INT32_MAX / a.plan.nz / a.plan.tiles) return kv_fail(who, "too many sequences, heads and rows for one call");
+    DeviceGuard g(c.device);
+    a.kv.err = c.err + 1;
+    a.q = q;
+    a.T = T;
+    a.qs = qs;
+    a.Hq = (int) Hq;
+    a.starts = starts;
+    a.out = out;
+    a.lse = accumulate ? static_cast<float*>(work) : nullptr;
+    a.part = static_cast<float*>(work) + (accumulate ? T * Hq : 0);
+    a.max_new = max_new;
+    a.scale_log2 = (1.0f / std::sqrt((float) kv->dim)) * 1.4426950408889634f;
+    a.q_vec = aligned16(q) && (qs * esize(kv->dt)) % 16 == 0;
+    const cudaError_t e = launch_attend(a, c.n_sm, c.st);
+    return e == cudaSuccess ? 0 : cuda_fail(who, e);
+}
+
+int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budget, int64_t sinks, int64_t recent,
+                 void* work, uint64_t work_bytes) {
+    constexpr const char* who = "h3s_kv_evict";
+    KvArgs a{};
+    if (check_kv(who, kv, true, a) != 0) return -1;
+    if (budget <= 0 || budget % kPage != 0) return kv_fail(who, "the budget must be a multiple of 64");
+    if (sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
+        return kv_fail(who, "sinks and recent tokens must fit the budget");
+    if (budget / kPage > kv->width) return 0;               // no sequence can be longer
+    if (!spare) return kv_fail(who, "a null pointer");
+    const uint64_t need = (uint64_t) (kv->seqs * kv->heads) * budget * 4;
+    if (!work || work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 3))
+        return kv_fail(who, "work of " + std::to_string(need) + " bytes needed, " + std::to_string(work ? work_bytes : 0) + " given");
+    if (kv->seqs * kv->heads > INT32_MAX / 2 / (budget / kPage)) return kv_fail(who, "too many sequences, heads and pages for one call");
+    auto& c = *static_cast<Ctx*>(ctx);
+    DeviceGuard g(c.device);
+    a.err = c.err + 1;
+    const cudaError_t e = launch_kv_evict(a, spare, (int) budget, (int) sinks, (int) recent, static_cast<int*>(work), c.st);
+    return e == cudaSuccess ? 0 : cuda_fail(who, e);
+}
+
+// ---- 4-bit linear layers (int4lin.cu) --------------------------------------------------------------------------------
+int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, const void* tiles, int64_t N,
+                    const void* scale, const void* zero, int s_dt, int group, const float* bias, void* out, int out_dt) {
+    constexpr const char* who = "h3s_int4_linear";
+    if (M <= 0 || K <= 0 || N <= 0) return 0;
+    if (group != 0 && group != 32 && group != 64 && group != 128) return kv_fail(who, "groups of 32, 64 or 128 inputs, or 0");
+    if (!check_dt(x_dt) || !check_dt(s_dt) || !check_dt(out_dt)) return kv_fail(who, "unknown element type");
+    if (!x || !tiles || !scale || !out) return kv_fail(who, "a null pointer");
+    if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
+    if (N > INT32_MAX - 16 || K > INT32_MAX - 64 || M > 65535ll * 8) return kv_fail(who, "too large");
+    auto& c = *static_cast<Ctx*>(ctx);
+    DeviceGuard g(c.device);
+    Int4Args a{};
+    a.x = x;
+    a.tiles = static_cast<const uint4*>(tiles);
+    a.scale = scale;
+    a.zero = zero;
+    a.bias = bias;
+    a.out = out;
+    a.M = M;
+    a.N = (int) N;
+    a.K = (int) K;
+    a.group = group ? group : (int) ((K + 63) / 64 * 64);
+    a.x_dt = x_dt;
+    a.s_dt = s_dt;
+    a.out_dt = out_dt;
+    a.x_vec = aligned16(x) && (K * esize(x_dt)) % 16 == 0;
+    const cudaError_t e = launch_int4_linear(a, c.n_sm, c.st);
+    return e == cudaSuccess ? 0 : cuda_fail(who, e);
+}
+
+int h3s_int4_pack(void* ctx, const uint8_t* codes, int64_t N, int64_t K, void* tiles) {
+    constexpr const char* who = "h3s_int4_pack";
+    if (K <= 0 || N <= 0) return 0;
+    if (K % 2 != 0) return kv_fail(who, "the inputs must be even in number: two codes to a byte");
+    if (!codes || !tiles) return kv_fail(who, "a null pointer");
+    if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
+    if (N > INT32_MAX - 16 || K > INT32_MAX - 64) return kv_fail(who, "too large");
+    auto& c = *static_cast<Ctx*>(ctx);
+    DeviceGuard g(c.device);
+    const cudaError_t e = launch_int4_pack(codes, N, K, tiles, c.n_sm, c.st);
+    return e == cudaSuccess ? 0 : cuda_fail(who, e);
 }
 
 }  // extern "C"

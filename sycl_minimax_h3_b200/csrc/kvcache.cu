@@ -1,0 +1,1047 @@
+// kvcache.cu - a key/value cache in 8 bits, with one scale for each 64-token page and head, for the text model's
+// grouped heads: writing to it, causal attention over it, and eviction by the weight that tokens received.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "attn_common.cuh"
+#include "kvcache.cuh"
+#include "prepass.cuh"
+
+namespace h3 {
+namespace {
+
+// ---- shared pieces -------------------------------------------------------------------------------------------------
+
+// Sequence b's new rows [s0, s0 + n) and its length L, checked against the call's rows and the table's width.
+struct Seq {
+    int s0, n, L;
+    bool ok;
+};
+__device__ __forceinline__ Seq load_seq(const KvArgs& kv, const int* starts, long long T, int b) {
+    Seq s;
+    s.s0 = starts[b];
+    const int s1 = starts[b + 1];
+    s.n = s1 - s.s0;
+    s.L = kv.lens[b];
+    s.ok = s.s0 >= 0 && s1 >= s.s0 && s1 <= T && s.L >= 0 && s.L / kPage <= kv.width;
+    return s;
+}
+__device__ __forceinline__ bool page_ok(const KvArgs& kv, int page) { return page >= 0 && page < kv.pages; }
+
+template <int DT>
+__device__ __forceinline__ void st1(void* p, size_t i, float x) {
+    if constexpr (DT == F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+    else if constexpr (DT == BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+    else reinterpret_cast<float*>(p)[i] = x;
+}
+// 8 consecutive values at element i, with 16-byte loads where vec
+template <int DT>
+__device__ __forceinline__ void ld8(const void* p, size_t i, bool vec, float* x) {
+    if (vec) {
+        const char* c = reinterpret_cast<const char*>(p) + i * DtInfo<DT>::ES;
+        ld16<DT>(c, x);
+        if constexpr (DT == F32) ld16<DT>(c + 16, x + 4);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = ld1<DT>(p, i + u);
+    }
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// The code of x in a block whose largest magnitude is a > 0: 127 x / a rounded to the nearest whole number, half way to
+// even, as if the ratio were exact. x and a of 16-bit types have at most 11 bits: 127 x has 18, and where 127 x / a is
+// not exactly half way it is at least 2^4 roundings of a float away from it, so one float division decides right.
+// Where x and a have 24 bits or more, a ratio within 1e-4 of half way is taken again in 64 bits.
+// num = 127 and den = a, both times 2^-8 where 127 a could overflow.
+template <bool WIDE>
+__device__ __forceinline__ int code_of(float x, float num, float den, double exact_x, double exact_a) {
+    const float r = __fdiv_rn(x * num, den);
+    float n = rintf(r);
+    if constexpr (WIDE) {
+        if (fabsf(fabsf(r - n) - 0.5f) < 1e-4f) n = (float) rint(exact_x * 127.0 / exact_a);
+    }
+    return (int) fminf(fmaxf(n, -127.0f), 127.0f);
+}
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return (uint32_t) (a & 255) | (uint32_t) (b & 255) << 8 | (uint32_t) (c & 255) << 16 | (uint32_t) d << 24;
+}
+
+template <typename T>
+__device__ __forceinline__ T block_max(T x, T* red) {     // over 256 threads; every thread gets the result
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const T y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = y > x ? y : x;
+    }
+    __syncthreads();                                       // red may still be read from the call before
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) x = red[i] > x ? red[i] : x;
+    return x;
+}
+
+// ---- writing ---------------------------------------------------------------------------------------------------------
+// A block of 64 slots that is full becomes a page: a = max|x| over its 64 x D values of a head, scale = a / 127, codes as
+// code_of. What does not fill a block stays in the tail in its own type, so a token is rounded once, when its block is
+// full, and the cache does not depend on how the tokens were spread over calls. Infinities take the code +-127 and NaN 0;
+// neither counts for a.
+// One CTA per (sequence, head, block, K or V). The CTA of the sequence's first block reads the old tail and, after that,
+// writes the new one: the two share slots.
+constexpr int kAppThreads = 256;
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kAppThreads) kv_append(const KvArgs kv, const void* __restrict__ krows,
+                                                         const void* __restrict__ vrows, long long T, long long stride,
+                                                         const int* __restrict__ starts, int J, int vec) {
+    constexpr int C8 = D / 8;                              // 8-value chunks of a row
+    constexpr int PER = 64 * C8 / kAppThreads;
+    __shared__ float red[8];
+    const long long unit = blockIdx.x;
+    const int which = (int) (unit & 1);
+    const int j = (int) ((unit >> 1) % J);
+    const int h = (int) ((unit >> 1) / J % kv.heads);
+    const int b = (int) ((unit >> 1) / J / kv.heads);
+    const Seq s = load_seq(kv, starts, T, b);
+    if (!s.ok || s.L < s.n) {
+        if (threadIdx.x == 0) atomicOr(kv.err, kErrLen);
+        return;
+    }
+    if (s.n == 0) return;
+    const int L0 = s.L - s.n, first = L0 / kPage, full = s.L / kPage;
+    const void* rows = which ? vrows : krows;
+    void* tail = which ? kv.tv : kv.tk;
+    const size_t tbase = ((size_t) b * kv.heads + h) * kPage;
+    auto row = [&](int slot) { return (size_t) (s.s0 + (slot - L0)) * stride + (size_t) h * D; };
+    for (int blk = first + j; blk < full; blk += J) {
+        const int page = kv.table[(size_t) b * kv.width + blk];
+        const bool ok = page_ok(kv, page);
+        if (!ok) {
+            if (threadIdx.x == 0) atomicOr(kv.err, kErrPage);
+            continue;
+        }
+        float x[PER][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * kAppThreads, r = c / C8, d = c % C8 * 8, slot = blk * kPage + r;
+            if (slot < L0) ld8<DT>(tail, (tbase + r) * D + d, true, x[i]);
+            else ld8<DT>(rows, row(slot) + d, vec, x[i]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (finite(x[i][u])) top = fmaxf(top, fabsf(x[i][u]));
+        }
+        top = block_max(top, red);
+        const size_t pbase = (size_t) page * kv.heads + h;
+        if (threadIdx.x == 0) (which ? kv.vs : kv.ks)[pbase] = __fdiv_rn(top, 127.0f);
+        const bool big = top > 1e36f;
+        const float num = big ? 127.0f / 256.0f : 127.0f, den = big ? top / 256.0f : top;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * kAppThreads, r = c / C8, d = c % C8 * 8;
+            int q[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float y = x[i][u];
+                if (top == 0.0f || y != y) q[u] = 0;
+                else if (!finite(y)) q[u] = y > 0.0f ? 127 : -127;
+                else q[u] = code_of<DT == F32>(y, num, den, (double) y, (double) top);
+            }
+            uint2 o;
+            o.x = pack4(q[0], q[1], q[2], q[3]);
+            o.y = pack4(q[4], q[5], q[6], q[7]);
+            *reinterpret_cast<uint2*>((which ? kv.v : kv.k) + (pbase * kPage + r) * D + d) = o;
+        }
+        if (kv.tw && which == 0 && threadIdx.x < kPage)
+            kv.w[pbase * kPage + threadIdx.x] = blk * kPage + (int) threadIdx.x < L0 ? kv.tw[tbase + threadIdx.x] : 0.0f;
+    }
+    if (j != 0 || s.L == full * kPage) return;
+    __syncthreads();                                       // the old tail has been read
+    const int from = max(L0, full * kPage);
+    for (int c = threadIdx.x; c < (s.L - from) * C8; c += kAppThreads) {
+        const int slot = from + c / C8, d = c % C8 * 8;
+        float x[8];
+        ld8<DT>(rows, row(slot) + d, vec, x);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) st1<DT>(tail, (tbase + slot % kPage) * D + d + u, x[u]);
+    }
+    if (kv.tw && which == 0)
+        for (int slot = from + threadIdx.x; slot < s.L; slot += kAppThreads) kv.tw[tbase + slot % kPage] = 0.0f;
+}
+
+// ---- attention -------------------------------------------------------------------------------------------------------
+// The query rows of a kv head are its group's heads of every new token, row r = token * group + head, in tiles of 16: the
+// rows of an m16n8k16 product. Keys and values are codes, which fp16 holds exactly, so the products are q . code and
+// p . code on the fp16 tensor path with 32-bit sums, and a page's scales multiply the results:
+//   s_ij = (q_i . kc_j) * ks * log2(e)/sqrt(D)     p_ij = 2^(s_ij - m_i)     acc_i = acc_i 2^(m_old - m_i) + vs * sum_j p_ij vc_j
+// q is brought to fp16 times a power of two per row, so that the row's largest value lies in [2^13, 2^14): exact for
+// fp16 and bf16 (what is more than 2^27 times smaller than the row's largest loses bits that a 32-bit sum would not
+// hold either); float32 takes two terms, 22 bits. p is rounded to fp16 (at most 2^-11 of it, beside 2^-8 or 2^-11 of the
+// output); for float32 it takes two terms too.
+//
+// Nothing is ordered inside a row's features: lane (g, t) of a warp reads 16-byte pieces of K (key g, features 16 t..),
+// and the query's fragment uses the same order. For P.V it reads features D/8 g.. of four keys, and accumulator i of a
+// lane is feature D/8 (2 t) + i and D/8 (2 t + 1) + i of rows g and g + 8.
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// four int8 -> two half2: the byte plus 128 in the low bits of 1024's mantissa, minus 1152
+__device__ __forceinline__ void i8x4_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    lo = sub1152(__byte_perm(w, 0x64646464u, 0x4140));
+    hi = sub1152(__byte_perm(w, 0x64646464u, 0x4342));
+}
+
+// The keys that a tile of query rows sees, and how they are divided: np whole pages in pieces of cz pages, and the tail
+// (when seen) as a piece of its own, or with the last piece where no split is left.
+struct Pieces {
+    int np, cz, nu, tail_at;           // nu pieces; the tail is read by piece tail_at (-1: not seen)
+};
+constexpr int kMinPages = 4;           // a split has at least a page per warp
+__device__ __forceinline__ Pieces pieces(int L, int last_pos, int nz) {
+    Pieces p;
+    const int seen = min(L, last_pos + 1), full = L / kPage;
+    if (seen <= 0) { p.np = 0; p.cz = 1; p.nu = 0; p.tail_at = -1; return p; }
+    p.np = min(full, (seen + kPage - 1) / kPage);
+    p.cz = max(kMinPages, (p.np + nz - 1) / nz);
+    const int nc = (p.np + p.cz - 1) / p.cz;
+    const bool tail = seen > full * kPage;
+    p.nu = tail ? min(nc + 1, nz) : nc;
+    p.tail_at = tail ? p.nu - 1 : -1;
+    return p;
+}
+
+constexpr int kAttWarps = 4;
+// p is 2^(s - m) with m the largest score less this, so at most 2^14: fp16 then keeps its 11 bits of every p down to
+// 2^-28 of the row's largest (2^-14 without it), and 2^-39 of the largest is what it drops
+constexpr float kPTop = 14.0f;
+
+template <int D, bool TWO>
+struct QFrag {
+    uint32_t hi[D / 16][4];
+    uint32_t lo[TWO ? D / 16 : 1][4];
+    float rs[2];                       // rows g and g + 8: 2^-e log2(e)/sqrt(D)
+};
+
+// rows g and g + 8 of a tile as A fragments; NULL rows are zero. qrow: element offsets, or -1.
+template <int DT, int D, bool TWO>
+__device__ __forceinline__ void load_q(QFrag<D, TWO>& f, const void* q, const long long (&qrow)[2], bool vec, float scale) {
+    const int t = threadIdx.x & 3;
+    float x[2][D / 4];                 // features 64 c + 16 t .. + 15 of both rows
+    float top[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int u = 0; u < 16; u += 8) {
+                float* y = &x[r][c * 16 + u];
+                if (qrow[r] >= 0) ld8<DT>(q, (size_t) qrow[r] + c * 64 + t * 16 + u, vec, y);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = 0.0f;
+            }
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i)
+            if (finite(x[r][i])) top[r] = fmaxf(top[r], fabsf(x[r][i]));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        // 2^e in two factors: each is a normal float, whatever the row's size (e from -152 to 114)
+        int e = 0;
+        if (top[r] > 0.0f) e = ilogbf(top[r]) - 13;
+        const int e1 = e / 2, e2 = e - e1;
+        const float m1 = __int_as_float((127 - e1) << 23), m2 = __int_as_float((127 - e2) << 23);
+        f.rs[r] = scale * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) x[r][i] = x[r][i] * m1 * m2;
+    }
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const float* y = &x[a & 1][ks * 4 + (a >> 1) * 2];
+            const __half2 h = __floats2half2_rn(y[0], y[1]);
+            f.hi[ks][a] = *reinterpret_cast<const uint32_t*>(&h);
+            if constexpr (TWO) {
+                const float2 back = __half22float2(h);
+                const __half2 l = __floats2half2_rn(finite(y[0]) ? y[0] - back.x : 0.0f, finite(y[1]) ? y[1] - back.y : 0.0f);
+                f.lo[ks][a] = *reinterpret_cast<const uint32_t*>(&l);
+            }
+        }
+}
+
+// s[nt] = the scores of keys 8 nt + {2 t, 2 t + 1} of rows g (c0, c1) and g + 8 (c2, c3) over a page's codes, unscaled
+template <int D, bool TWO>
+__device__ __forceinline__ void page_scores(const QFrag<D, TWO>& f, const int8_t* kp, float (&s)[8][4]) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(kp + (nt * 8 + g) * D + c * 64 + t * 16);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t b0, b1;
+                i8x4_half(u[i], b0, b1);
+                const int ks = c * 4 + i;
+                mma16816(s[nt], f.hi[ks][0], f.hi[ks][1], f.hi[ks][2], f.hi[ks][3], b0, b1);
+                if constexpr (TWO) mma16816(s[nt], f.lo[ks][0], f.lo[ks][1], f.lo[ks][2], f.lo[ks][3], b0, b1);
+            }
+        }
+    }
+}
+
+// Scores of the tail's keys in plain 32-bit arithmetic, sc[row][key] in log2 units: qf [16][D] as floats, kt the tail's
+// rows of this head in dt. 128 threads; rows at or past nrow and keys at or past nkey are left alone.
+template <int DT, int D>
+__device__ __forceinline__ void tail_scores(const float* qf, const void* kt, size_t kbase, int nrow, int nkey, float scale,
+                                            float (*sc)[kPage]) {
+    const int key = threadIdx.x & 63, half = threadIdx.x >> 6, per = (nrow + 1) / 2;
+    const int r0 = half * per, r1 = min(nrow, r0 + per);
+    if (key >= nkey) return;
+    float acc[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) acc[r] = 0.0f;
+    for (int d = 0; d < D; d += 8) {
+        float x[8];
+        ld8<DT>(kt, kbase + (size_t) key * D + d, true, x);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (r0 + r >= r1) break;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) acc[r] = fmaf(qf[(r0 + r) * D + d + u], x[u], acc[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+        if (r0 + r < r1) sc[r0 + r][key] = acc[r] * scale;
+}
+
+template <int D>
+struct AttSmem {
+    float acc[kAttWarps + 1][16][D];   // the warps' accumulators, then the tail's
+    float m[kAttWarps + 1][16], l[kAttWarps + 1][16];
+    float q[16][D];
+    float sc[16][kPage];
+    int pos[16];
+    long long row[16];                 // global row (token * Hq + head), or -1
+};
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kAttWarps * 32) attend(const AttendArgs a) {
+    constexpr bool TWO = DT == F32;
+    constexpr int DG = D / 8;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    AttSmem<D>& sm = *reinterpret_cast<AttSmem<D>*>(smem_raw);
+    const KvArgs& kv = a.kv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int group = a.Hq / kv.heads, nz = a.plan.nz;
+    long long unit = blockIdx.x;
+    const int tile0 = (int) (unit % a.plan.tiles);
+    unit /= a.plan.tiles;
+    const int z = (int) (unit % nz);
+    unit /= nz;
+    const int h = (int) (unit % kv.heads), b = (int) (unit / kv.heads);
+    const Seq s = load_seq(kv, a.starts, a.T, b);
+    if (!s.ok) {
+        if (threadIdx.x == 0) atomicOr(kv.err, kErrLen);
+        return;
+    }
+    const long long R = (long long) s.n * group;
+    for (long long r0 = (long long) tile0 * 16; r0 < R; r0 += (long long) a.plan.tiles * 16) {
+        const int nrow = (int) min(R - r0, 16ll);
+        const int last_pos = s.L - s.n + (int) ((r0 + nrow - 1) / group);
+        const Pieces pc = pieces(s.L, last_pos, nz);
+        if (z >= max(pc.nu, 1)) continue;
+        __syncthreads();                                   // the tile before has been written
+        if (threadIdx.x < 16) {
+            const int r = threadIdx.x;
+            const bool in = r < nrow;
+            const int tok = in ? (int) ((r0 + r) / group) : 0, hq = h * group + (in ? (int) ((r0 + r) % group) : 0);
+            sm.pos[r] = in ? s.L - s.n + tok : -1;
+            sm.row[r] = in ? (long long) (s.s0 + tok) * a.Hq + hq : -1;
+        }
+        __syncthreads();
+        auto qoff = [&](int r) {
+            const long long gr = sm.row[r];
+            return gr < 0 ? -1ll : gr / a.Hq * a.qs + gr % a.Hq * D;
+        };
+        float acc[DG][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < DG; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[i][u] = 0.0f;
+        const int p0 = z * pc.cz, p1 = min(pc.np, p0 + pc.cz);
+        if (p0 < p1) {
+            QFrag<D, TWO> f;
+            const long long qrow[2] = {qoff(g), qoff(g + 8)};
+            load_q<DT, D, TWO>(f, a.q, qrow, a.q_vec, a.scale_log2);
+            const int pos[2] = {sm.pos[g], sm.pos[g + 8]};
+            const int first_pos = sm.pos[0];
+            for (int p = p0 + warp; p < p1; p += kAttWarps) {
+                const int page = kv.table[(size_t) b * kv.width + p];
+                if (!page_ok(kv, page)) {
+                    if (lane == 0) atomicOr(kv.err, kErrPage);
+                    continue;
+                }
+                const size_t pb = (size_t) page * kv.heads + h;
+                float sc[8][4];
+                page_scores<D, TWO>(f, kv.k + pb * kPage * D, sc);
+                const float ks = kv.ks[pb], vs = kv.vs[pb];
+                const float f0 = ks * f.rs[0], f1 = ks * f.rs[1];
+                float mx[2] = {-INFINITY, -INFINITY};
+                const bool mask = nrow < 16 || p * kPage + kPage - 1 > first_pos;
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x = sc[nt][i] * (i < 2 ? f0 : f1);
+                        if (mask && p * kPage + nt * 8 + 2 * t + (i & 1) > pos[i >> 1]) x = -INFINITY;
+                        sc[nt][i] = x;
+                        mx[i >> 1] = fmaxf(mx[i >> 1], x);
+                    }
+                float al[2], mu[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                    const float mn = fmaxf(m[r], mx[r] - kPTop);
+                    mu[r] = mn == -INFINITY ? 0.0f : mn;   // a row that sees nothing yet: every p is 2^-inf = 0
+                    al[r] = ex2(m[r] - mu[r]);
+                    m[r] = mn;
+                    l[r] *= al[r];
+                }
+                uint32_t ph[8][2], pl[TWO ? 8 : 1][2];
+#pragma unroll
+                for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float e0 = ex2(sc[nt][2 * r] - mu[r]), e1 = ex2(sc[nt][2 * r + 1] - mu[r]);
+                        l[r] += e0 + e1;
+                        const __half2 hh = __floats2half2_rn(e0, e1);
+                        ph[nt][r] = *reinterpret_cast<const uint32_t*>(&hh);
+                        if constexpr (TWO) {
+                            const float2 back = __half22float2(hh);
+                            const __half2 ll = __floats2half2_rn(e0 - back.x, e1 - back.y);
+                            pl[nt][r] = *reinterpret_cast<const uint32_t*>(&ll);
+                        }
+                    }
+                const int8_t* vp = kv.v + pb * kPage * D;
+#pragma unroll
+                for (int hf = 0; hf < DG / 8; ++hf) {      // 8 features of each lane's DG at a time
+                    uint32_t w[4][4][2];                   // 16 keys x 4 of them in this lane x 8 features
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const int key = jj * 16 + (kk >> 1) * 8 + 2 * t + (kk & 1);
+                            const uint2 u = *reinterpret_cast<const uint2*>(vp + key * D + g * DG + hf * 8);
+                            w[jj][kk][0] = u.x ^ 0x80808080u;
+                            w[jj][kk][1] = u.y ^ 0x80808080u;
+                        }
+#pragma unroll
+                    for (int wd = 0; wd < 2; ++wd) {
+                        float c[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) c[i][u] = 0.0f;
+#pragma unroll
+                        for (int jj = 0; jj < 4; ++jj) {
+                            uint32_t bb[2][4];             // [keys 2t.. / 8 + 2t..][feature of the word]
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; ++k2) {
+                                const uint32_t x = w[jj][2 * k2][wd], y = w[jj][2 * k2 + 1][wd];
+                                const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);
+                                bb[k2][0] = sub1152(__byte_perm(lo, 0x64646464u, 0x4140));
+                                bb[k2][1] = sub1152(__byte_perm(lo, 0x64646464u, 0x4342));
+                                bb[k2][2] = sub1152(__byte_perm(hi, 0x64646464u, 0x4140));
+                                bb[k2][3] = sub1152(__byte_perm(hi, 0x64646464u, 0x4342));
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                mma16816(c[i], ph[2 * jj][0], ph[2 * jj][1], ph[2 * jj + 1][0], ph[2 * jj + 1][1], bb[0][i], bb[1][i]);
+                                if constexpr (TWO)
+                                    mma16816(c[i], pl[2 * jj][0], pl[2 * jj][1], pl[2 * jj + 1][0], pl[2 * jj + 1][1], bb[0][i], bb[1][i]);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                float& y = acc[hf * 8 + wd * 4 + i][u];
+                                y = fmaf(vs, c[i][u], y * al[u >> 1]);
+                            }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (t == 0) {
+                sm.m[warp][g + 8 * r] = m[r];
+                sm.l[warp][g + 8 * r] = l[r];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DG; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sm.acc[warp][g + 8 * (u >> 1)][DG * (2 * t + (u & 1)) + i] = acc[i][u];
+        const bool tail = z == pc.tail_at;
+        if (tail) {                                        // CUDA cores: the tail is in its own type, at most 63 keys
+            for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32)
+                sm.q[i / D][i % D] = ld1<DT>(a.q, (size_t) qoff(i / D) + i % D);
+            __syncthreads();
+            const int full = s.L / kPage, nkey = s.L - full * kPage;
+            const size_t tb = ((size_t) b * kv.heads + h) * kPage * D;
+            tail_scores<DT, D>(&sm.q[0][0], kv.tk, tb, nrow, nkey, a.scale_log2, sm.sc);
+            __syncthreads();
+            for (int r = warp; r < nrow; r += kAttWarps) {
+                const int see = min(nkey, sm.pos[r] + 1 - full * kPage);
+                const float x0 = lane < see ? sm.sc[r][lane] : -INFINITY, x1 = lane + 32 < see ? sm.sc[r][lane + 32] : -INFINITY;
+                float mx = fmaxf(x0, x1);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const float mu = mx == -INFINITY ? 0.0f : mx;
+                const float e0 = ex2(x0 - mu), e1 = ex2(x1 - mu);
+                float sum = e0 + e1;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                sm.sc[r][lane] = e0;
+                sm.sc[r][lane + 32] = e1;
+                if (lane == 0) { sm.m[kAttWarps][r] = mx; sm.l[kAttWarps][r] = sum; }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32) {
+                const int r = i / D, d = i % D, see = min(nkey, sm.pos[r] + 1 - full * kPage);
+                float o = 0.0f;
+                for (int key = 0; key < see; ++key) o = fmaf(sm.sc[r][key], ld1<DT>(kv.tv, tb + (size_t) key * D + d), o);
+                sm.acc[kAttWarps][r][d] = o;
+            }
+        }
+        __syncthreads();
+        // the pieces of this CTA as one: rows straight out, or a partial result per split
+        const int parts = kAttWarps + (tail ? 1 : 0);
+        for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32) {
+            const int r = i / D, d = i % D;
+            float mx = -INFINITY;
+            for (int p = 0; p < parts; ++p) mx = fmaxf(mx, sm.m[p][r]);
+            // NaN scores leave the maximum alone and come out of the sums
+            const float mu = mx == -INFINITY ? 0.0f : mx;
+            float sum = 0.0f, o = 0.0f;
+            for (int p = 0; p < parts; ++p) {
+                const float e = ex2(sm.m[p][r] - mu);
+                sum = fmaf(e, sm.l[p][r], sum);
+                o = fmaf(e, sm.acc[p][r][d], o);
+            }
+            const size_t gr = (size_t) sm.row[r];
+            if (pc.nu <= 1) {
+                st1<DT>(a.out, gr * D + d, sum == 0.0f ? 0.0f : o / sum);
+                if (a.lse && d == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);
+            } else {
+                a.part[(gr * nz + z) * D + d] = o;
+                if (d == 0) {
+                    float* ml = a.part + (size_t) a.T * a.Hq * nz * D + (gr * nz + z) * 2;
+                    ml[0] = mx;
+                    ml[1] = sum;
+                }
+            }
+        }
+    }
+}
+
+// The splits' partial results of a row as one, in the order of the splits: a warp per row.
+template <int DT, int D>
+__global__ void __launch_bounds__(128) attend_join(const AttendArgs a) {
+    const KvArgs& kv = a.kv;
+    const int lane = threadIdx.x & 31, nz = a.plan.nz, group = a.Hq / kv.heads;
+    const long long per = a.max_new * a.Hq, unit = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (unit >= per * kv.seqs) return;
+    const int b = (int) (unit / per);
+    const Seq s = load_seq(kv, a.starts, a.T, b);
+    if (!s.ok) return;
+    const float* mls = a.part + (size_t) a.T * a.Hq * nz * D;
+    for (long long i = unit % per; i < (long long) s.n * a.Hq; i += per) {
+        const int tok = (int) (i / a.Hq), hq = (int) (i % a.Hq);
+        const long long R = (long long) s.n * group, r0 = ((long long) tok * group + hq % group) / 16 * 16;
+        const int last_pos = s.L - s.n + (int) ((min(R, r0 + 16) - 1) / group);
+        const Pieces pc = pieces(s.L, last_pos, nz);
+        if (pc.nu <= 1) continue;
+        const size_t gr = (size_t) (s.s0 + tok) * a.Hq + hq;
+        float mx = -INFINITY;
+        for (int z = 0; z < pc.nu; ++z) mx = fmaxf(mx, mls[(gr * nz + z) * 2]);
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, o[D / 32];
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) o[u] = 0.0f;
+        for (int z = 0; z < pc.nu; ++z) {
+            const float e = ex2(mls[(gr * nz + z) * 2] - mu);
+            sum = fmaf(e, mls[(gr * nz + z) * 2 + 1], sum);
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) o[u] = fmaf(e, a.part[(gr * nz + z) * D + lane + 32 * u], o[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) st1<DT>(a.out, gr * D + lane + 32 * u, sum == 0.0f ? 0.0f : o[u] / sum);
+        if (a.lse && lane == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);
+    }
+}
+
+// weight[slot] += the sum over the group's query rows of p = 2^(s - lse): the scores once more, against the finished
+// sums. One CTA per (sequence, kv head, piece of the pages), the last piece also the tail; a page's sums stay in one warp.
+template <int DT, int D>
+__global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const AttendArgs a, int nzw) {
+    constexpr bool TWO = DT == F32;
+    __shared__ float qs[16][D];
+    __shared__ float sc[16][kPage];
+    const KvArgs& kv = a.kv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int group = a.Hq / kv.heads;
+    const int z = (int) (blockIdx.x % nzw), h = (int) (blockIdx.x / nzw % kv.heads), b = (int) (blockIdx.x / nzw / kv.heads);
+    const Seq s = load_seq(kv, a.starts, a.T, b);
+    if (!s.ok || s.n == 0) return;
+    const long long R = (long long) s.n * group;
+    const int full = s.L / kPage;
+    auto place = [&](long long r, int& pos, long long& off, float& lse) {
+        pos = -1;
+        off = -1;
+        lse = INFINITY;
+        if (r >= R) return;
+        const int tok = (int) (r / group), hq = h * group + (int) (r % group);
+        pos = s.L - s.n + tok;
+        off = (long long) (s.s0 + tok) * a.qs + (long long) hq * D;
+        lse = a.lse[(size_t) (s.s0 + tok) * a.Hq + hq];
+    };
+    for (int p = z * kAttWarps + warp; p < full; p += nzw * kAttWarps) {
+        const int page = kv.table[(size_t) b * kv.width + p];
+        if (!page_ok(kv, page)) continue;                  // already recorded by the attention
+        const size_t pb = (size_t) page * kv.heads + h;
+        const float ks = kv.ks[pb];
+        float sum[8][2];
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) sum[nt][0] = sum[nt][1] = 0.0f;
+        // the first row that sees slot 64 p
+        const long long from = max(0ll, (long long) (p * kPage - (s.L - s.n)) * group) / 16 * 16;
+        for (long long r0 = from; r0 < R; r0 += 16) {
+            int pos[2];
+            long long off[2];
+            float lse[2];
+            place(r0 + g, pos[0], off[0], lse[0]);
+            place(r0 + g + 8, pos[1], off[1], lse[1]);
+            QFrag<D, TWO> f;
+            load_q<DT, D, TWO>(f, a.q, off, a.q_vec, a.scale_log2);
+            float x[8][4];
+            page_scores<D, TWO>(f, kv.k + pb * kPage * D, x);
+#pragma unroll
+            for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = ex2(x[nt][i] * (ks * f.rs[i >> 1]) - lse[i >> 1]);
+                    if (p * kPage + nt * 8 + 2 * t + (i & 1) <= pos[i >> 1]) sum[nt][i & 1] += e;
+                }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float y = sum[nt][i];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+                if (g == 0) atomicAdd(&kv.w[pb * kPage + nt * 8 + 2 * t + i], y);
+            }
+    }
+    const int nkey = s.L - full * kPage;
+    if (z != nzw - 1 || nkey == 0) return;
+    const size_t tb = ((size_t) b * kv.heads + h) * kPage;
+    float sum = 0.0f;
+    const long long from = max(0ll, (long long) (full * kPage - (s.L - s.n)) * group) / 16 * 16;
+    for (long long r0 = from; r0 < R; r0 += 16) {
+        const int nrow = (int) min(R - r0, 16ll);
+        __syncthreads();
+        for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32) {
+            int pos;
+            long long off;
+            float lse;
+            place(r0 + i / D, pos, off, lse);
+            qs[i / D][i % D] = ld1<DT>(a.q, (size_t) off + i % D);
+        }
+        __syncthreads();
+        tail_scores<DT, D>(&qs[0][0], kv.tk, tb * D, nrow, nkey, a.scale_log2, sc);
+        __syncthreads();
+        if (threadIdx.x < nkey)
+            for (int r = 0; r < nrow; ++r) {
+                int pos;
+                long long off;
+                float lse;
+                place(r0 + r, pos, off, lse);
+                if (full * kPage + (int) threadIdx.x <= pos) sum += ex2(sc[r][threadIdx.x] - lse);
+            }
+    }
+    if (threadIdx.x < nkey) kv.tw[tb + threadIdx.x] += sum;
+}
+
+// ---- eviction --------------------------------------------------------------------------------------------------------
+// Of a sequence longer than the budget, each kv head keeps its first `sinks` and last `recent` tokens and, of the ones
+// between, those with the largest weight (of equal ones the earlier), in their order, budget tokens in all. They are
+// quantised again, 64 to a page with a new scale, into the sequence's spare pages.
+
+// weights in an order of whole numbers: larger weight, larger key; NaN below everything
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 0;
+    const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelThreads = 1024;
+
+// kept[seq, head, 0..budget): the kept slots in order; kept[..][0] = -1 where the sequence is left alone. One CTA per
+// (sequence, head): the weight of the last kept one among equals by four passes over 8 bits of the keys each, then one
+// pass that writes the slots down.
+__global__ void __launch_bounds__(kSelThreads) evict_select(const KvArgs kv, const int* __restrict__ spare, int budget,
+                                                            int sinks, int recent, int* __restrict__ kept) {
+    __shared__ int hist[256];
+    __shared__ int wsum[32];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_need, s_bad;
+    const int h = (int) (blockIdx.x % kv.heads), b = (int) (blockIdx.x / kv.heads);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int L = kv.lens[b];
+    int* out = kept + (size_t) blockIdx.x * budget;
+    const int* table = kv.table + (size_t) b * kv.width;
+    const int full = L / kPage;
+    if (L <= budget || full > kv.width) {
+        if (tid == 0) {
+            out[0] = -1;
+            if (L < 0 || full > kv.width) atomicOr(kv.err, kErrLen);
+        }
+        return;
+    }
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    for (int i = tid; i < full; i += kSelThreads)
+        if (!page_ok(kv, table[i])) s_bad = 1;
+    for (int i = tid; i < budget / kPage; i += kSelThreads)
+        if (!page_ok(kv, spare[(size_t) b * (budget / kPage) + i])) s_bad = 1;
+    __syncthreads();
+    if (s_bad) {
+        if (tid == 0) {
+            out[0] = -1;
+            atomicOr(kv.err, kErrPage);
+        }
+        return;
+    }
+    const int lo = sinks, hi = L - recent;                 // sinks + recent <= budget < L: lo < hi
+    auto key = [&](int slot) {
+        const float w = slot < full * kPage ? kv.w[((size_t) table[slot / kPage] * kv.heads + h) * kPage + slot % kPage]
+                                            : kv.tw[((size_t) b * kv.heads + h) * kPage + slot - full * kPage];
+        return weight_key(w);
+    };
+    // the need-th largest key of the middle
+    uint32_t prefix = 0;
+    int need = budget - sinks - recent;
+    if (need > 0) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+            __syncthreads();
+            for (int i = lo + tid; i < hi; i += kSelThreads) {
+                const uint32_t k = key(i);
+                if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+            }
+            __syncthreads();
+            if (warp == 0) {                               // from the top: the bin in which the need-th falls
+                int mine = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mine += hist[255 - lane * 8 - i];
+                int above = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, above, o);
+                    if (lane >= o) above += y;
+                }
+                above -= mine;                             // keys in higher bins than this lane's
+                if (above < need && above + mine >= need) {
+                    int left = need - above;
+                    for (int i = 0; i < 8; ++i) {
+                        const int c = hist[255 - lane * 8 - i];
+                        if (left <= c) {
+                            s_prefix = prefix | (uint32_t) (255 - lane * 8 - i) << shift;
+                            s_need = left;
+                            break;
+                        }
+                        left -= c;
+                    }
+                }
+            }
+            __syncthreads();
+            prefix = s_prefix;
+            need = s_need;
+            __syncthreads();
+        }
+    }
+    // now `need` of the keys equal to prefix are kept (the first ones), and all larger ones
+    const bool any = budget - sinks - recent > 0;
+    int done = 0, equal = 0;                               // kept so far; equal ones so far
+    for (int base = 0; base < L; base += kSelThreads) {
+        const int i = base + tid;
+        int sure = 0, eq = 0;
+        if (i < L) {
+            if (i < lo || i >= hi) sure = 1;
+            else if (any) {
+                const uint32_t k = key(i);
+                sure = k > prefix;
+                eq = k == prefix;
+            }
+        }
+        // an inclusive scan over the block of both counts, in one word; at most 1,024 of each
+        int both = sure | eq << 16;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, both, o);
+            if (lane >= o) both += y;
+        }
+        if (lane == 31) wsum[warp] = both;
+        __syncthreads();
+        if (warp == 0) {
+            int x = wsum[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            wsum[lane] = x;
+        }
+        __syncthreads();
+        if (warp > 0) both += wsum[warp - 1];
+        const int all = wsum[31];
+        const int eq_before = equal + (both >> 16) - eq;   // equal ones before this slot
+        const bool keep = sure || (eq && eq_before < need);
+        const int at = done + (both & 0xffff) - sure + (min(eq_before, need) - min(equal, need));
+        if (keep) out[at] = i;
+        const int eq_all = all >> 16;
+        done += (all & 0xffff) + min(equal + eq_all, need) - min(equal, need);
+        equal += eq_all;
+        __syncthreads();
+    }
+}
+
+// 64 kept tokens of a (sequence, head), K or V, into one spare page
+template <int DT, int D>
+__global__ void __launch_bounds__(256) evict_gather(const KvArgs kv, const int* __restrict__ spare, int budget,
+                                                    const int* __restrict__ kept) {
+    constexpr int C8 = D / 8;
+    constexpr int PER = 64 * C8 / 256;
+    __shared__ double red[8];
+    __shared__ int slots[kPage];
+    __shared__ int pages[kPage];
+    const int nb = budget / kPage;
+    long long unit = blockIdx.x;
+    const int which = (int) (unit & 1);
+    unit >>= 1;
+    const int blk = (int) (unit % nb);
+    unit /= nb;
+    const int h = (int) (unit % kv.heads), b = (int) (unit / kv.heads);
+    const int* mine = kept + ((size_t) b * kv.heads + h) * budget;
+    if (mine[0] < 0) return;
+    const int full = kv.lens[b] / kPage;
+    if (threadIdx.x < kPage) {
+        const int slot = mine[blk * kPage + threadIdx.x];
+        slots[threadIdx.x] = slot;
+        pages[threadIdx.x] = slot < full * kPage ? kv.table[(size_t) b * kv.width + slot / kPage] : -1;
+    }
+    __syncthreads();
+    const int8_t* codes = which ? kv.v : kv.k;
+    const float* scales = which ? kv.vs : kv.ks;
+    const void* tail = which ? kv.tv : kv.tk;
+    const size_t tbase = ((size_t) b * kv.heads + h) * kPage;
+    float x[PER][8];                   // a page's codes, or the tail's values
+    float sc[PER];                     // their scale (1 for the tail)
+    double top = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = threadIdx.x + i * 256, r = c / C8, d = c % C8 * 8, page = pages[r], slot = slots[r];
+        if (page >= 0) {
+            const size_t pb = (size_t) page * kv.heads + h;
+            const uint2 u = *reinterpret_cast<const uint2*>(codes + (pb * kPage + slot % kPage) * D + d);
+            sc[i] = scales[pb];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[i][e] = (float) (int8_t) (u.x >> (8 * e));
+                x[i][4 + e] = (float) (int8_t) (u.y >> (8 * e));
+            }
+        } else {
+            ld8<DT>(tail, (tbase + slot - full * kPage) * D + d, true, x[i]);
+            sc[i] = 1.0f;
+        }
+        float m = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (finite(x[i][u])) m = fmaxf(m, fabsf(x[i][u]));
+        const double v = (double) m * (double) sc[i];      // exact: 24 bits times 24 at most
+        if (v > top) top = v;
+    }
+    top = block_max(top, red);
+    const size_t pb = (size_t) spare[(size_t) b * nb + blk] * kv.heads + h;
+    if (threadIdx.x == 0) (which ? kv.vs : kv.ks)[pb] = (float) (top / 127.0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = threadIdx.x + i * 256, r = c / C8, d = c % C8 * 8;
+        const double ratio = top > 0.0 ? (double) sc[i] * 127.0 / top : 0.0;
+        int q[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float y = x[i][u];
+            if (top == 0.0 || y != y) q[u] = 0;
+            else if (!finite(y)) q[u] = y > 0.0f ? 127 : -127;
+            else {
+                const double e = (double) y * ratio;
+                double n = rint(e);
+                if (fabs(fabs(e - n) - 0.5) < 1e-6) n = rint((double) y * (double) sc[i] * 127.0 / top);
+                q[u] = (int) fmin(fmax(n, -127.0), 127.0);
+            }
+        }
+        uint2 o;
+        o.x = pack4(q[0], q[1], q[2], q[3]);
+        o.y = pack4(q[4], q[5], q[6], q[7]);
+        *reinterpret_cast<uint2*>((which ? kv.v : kv.k) + (pb * kPage + r) * D + d) = o;
+    }
+    if (which == 0 && threadIdx.x < kPage) {
+        const int slot = slots[threadIdx.x], page = pages[threadIdx.x];
+        kv.w[pb * kPage + threadIdx.x] =
+            page >= 0 ? kv.w[((size_t) page * kv.heads + h) * kPage + slot % kPage] : kv.tw[tbase + slot - full * kPage];
+    }
+}
+
+// the new pages take the old ones' place in the table, which take theirs among the spare ones
+__global__ void __launch_bounds__(256) evict_swap(const KvArgs kv, int* __restrict__ spare, int budget, const int* __restrict__ kept) {
+    const int b = (int) blockIdx.x, nb = budget / kPage;
+    if (kept[(size_t) b * kv.heads * budget] < 0) return;
+    for (int i = threadIdx.x; i < nb; i += 256) {
+        int* p = kv.table + (size_t) b * kv.width + i;
+        int* q = spare + (size_t) b * nb + i;
+        const int x = *p;
+        *p = *q;
+        *q = x;
+    }
+    if (threadIdx.x == 0) kv.lens[b] = budget;
+}
+
+}  // namespace
+
+// ---- launchers -------------------------------------------------------------------------------------------------------
+
+template <int DT>
+cudaError_t append_dt(const KvArgs& kv, const void* k, const void* v, long long T, long long stride, const int* starts,
+                      long long max_new, bool vec, cudaStream_t st) {
+    const long long J = std::max(1ll, (max_new + kPage - 1) / kPage);
+    const unsigned grid = (unsigned) (2 * J * kv.heads * kv.seqs);
+    if (kv.dim == 64) kv_append<DT, 64><<<grid, kAppThreads, 0, st>>>(kv, k, v, T, stride, starts, (int) J, vec);
+    else kv_append<DT, 128><<<grid, kAppThreads, 0, st>>>(kv, k, v, T, stride, starts, (int) J, vec);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, long long T, long long stride, const int* starts,
+                             long long max_new, bool vec, cudaStream_t st) {
+    switch (kv.dt) {
+        case F16: return append_dt<F16>(kv, k, v, T, stride, starts, max_new, vec, st);
+        case BF16: return append_dt<BF16>(kv, k, v, T, stride, starts, max_new, vec, st);
+        default: return append_dt<F32>(kv, k, v, T, stride, starts, max_new, vec, st);
+    }
+}
+
+AttendPlan attend_plan(int n_sm, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
+    AttendPlan p;
+    const int64_t rows = std::min(max_new, T) * group;
+    p.tiles = (int) std::max<int64_t>(1, (rows + 15) / 16);
+    const int64_t pages = (max_len + kPage - 1) / kPage, units = seqs * heads * p.tiles;
+    const int64_t most = (pages + kMinPages - 1) / kMinPages;
+    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, (n_sm * 8 + units - 1) / units, 512}));
+    return p;
+}
+
+template <typename F>
+cudaError_t allow_smem(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+template <int DT, int D>
+cudaError_t attend_dt(const AttendArgs& a, int n_sm, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
+    cudaError_t e = allow_smem(ready, attend<DT, D>, sizeof(AttSmem<D>));
+    if (e != cudaSuccess) return e;
+    const KvArgs& kv = a.kv;
+    const long long grid = (long long) kv.seqs * kv.heads * a.plan.nz * a.plan.tiles;
+    attend<DT, D><<<(unsigned) grid, kAttWarps * 32, sizeof(AttSmem<D>), st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    if (a.plan.nz > 1) {
+        const long long rows = a.max_new * a.Hq * kv.seqs;
+        attend_join<DT, D><<<(unsigned) ((rows + 3) / 4), 128, 0, st>>>(a);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    if (a.lse) {
+        const long long units = (long long) kv.seqs * kv.heads;
+        const int nzw = (int) std::max(1ll, std::min<long long>((kv.width + kAttWarps - 1) / kAttWarps, (n_sm * 4 + units - 1) / units));
+        attend_weights<DT, D><<<(unsigned) (units * nzw), kAttWarps * 32, 0, st>>>(a, nzw);
+        e = cudaGetLastError();
+    }
+    return e;
+}
+
+cudaError_t launch_attend(const AttendArgs& a, int n_sm, cudaStream_t st) {
+    const bool narrow = a.kv.dim == 64;
+    switch (a.kv.dt) {
+        case F16: return narrow ? attend_dt<F16, 64>(a, n_sm, st) : attend_dt<F16, 128>(a, n_sm, st);
+        case BF16: return narrow ? attend_dt<BF16, 64>(a, n_sm, st) : attend_dt<BF16, 128>(a, n_sm, st);
+        default: return narrow ? attend_dt<F32, 64>(a, n_sm, st) : attend_dt<F32, 128>(a, n_sm, st);
+    }
+}
+
+template <int DT>
+cudaError_t evict_dt(const KvArgs& kv, const int* spare, int budget, const int* kept, unsigned grid, cudaStream_t st) {
+    if (kv.dim == 64) evict_gather<DT, 64><<<grid, 256, 0, st>>>(kv, spare, budget, kept);
+    else evict_gather<DT, 128><<<grid, 256, 0, st>>>(kv, spare, budget, kept);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_kv_evict(const KvArgs& kv, int* spare, int budget, int sinks, int recent, int* kept, cudaStream_t st) {
+    const unsigned units = (unsigned) (kv.seqs * kv.heads);
+    evict_select<<<units, kSelThreads, 0, st>>>(kv, spare, budget, sinks, recent, kept);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const unsigned grid = units * (unsigned) (budget / kPage) * 2;
+    switch (kv.dt) {
+        case F16: e = evict_dt<F16>(kv, spare, budget, kept, grid, st); break;
+        case BF16: e = evict_dt<BF16>(kv, spare, budget, kept, grid, st); break;
+        default: e = evict_dt<F32>(kv, spare, budget, kept, grid, st); break;
+    }
+    if (e != cudaSuccess) return e;
+    evict_swap<<<(unsigned) kv.seqs, 256, 0, st>>>(kv, spare, budget, kept);
+    return cudaGetLastError();
+}
+
+}  // namespace h3

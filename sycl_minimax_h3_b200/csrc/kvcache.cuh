@@ -1,0 +1,59 @@
+// kvcache.cuh - the argument block and the launchers of the 8-bit key/value cache (kvcache.cu): h3s_kv_append,
+// h3s_attention_cached, h3s_kv_evict. The layout and the meaning of every field stand at h3s_kv_cache in
+// include/h3cuda.h.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace h3 {
+
+constexpr int kPage = 64;              // tokens of a page: the Sage quantiser's block, with one scale per head
+constexpr int kErrPage = 1;            // index errors (the second word of a context's error words): a page id
+constexpr int kErrLen = 2;             //   lens or starts out of range
+
+struct KvArgs {
+    int8_t* k;                         // [pages, heads, 64, dim]
+    int8_t* v;
+    float* ks;                         // [pages, heads]
+    float* vs;
+    void* tk;                          // [seqs, heads, 64, dim] in dt: the tokens that do not fill a page yet
+    void* tv;
+    float* w;                          // [pages, heads, 64] or NULL: the attention weight that each token received
+    float* tw;                         // [seqs, heads, 64]
+    int* table;                        // [seqs, width] page ids
+    int* lens;                         // [seqs]
+    long long pages;
+    int seqs, width, heads, dim, dt;
+    int* err;                          // index errors
+};
+
+// How a call's queries and keys are divided (the same on the host and in every kernel of one call).
+struct AttendPlan {
+    int tiles;                         // 16-row query tiles per (sequence, kv head); more are looped over
+    int nz;                            // splits of the keys
+};
+AttendPlan attend_plan(int n_sm, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len);
+
+struct AttendArgs {
+    KvArgs kv;
+    const void* q;
+    long long T, qs;                   // query rows, their stride (elements)
+    int Hq;
+    const int* starts;                 // [seqs + 1]
+    void* out;                         // [T, Hq * dim]
+    float* part;                       // [T * Hq, nz, dim] accumulators and, behind them, [T * Hq, nz, 2] (max, sum); nz > 1
+    float* lse;                        // [T * Hq] or NULL: log2 of the softmax's sum, for the weights
+    AttendPlan plan;
+    long long max_new;
+    float scale_log2;                  // log2(e) / sqrt(dim)
+    int q_vec;                         // 16-byte loads of q's rows allowed
+};
+cudaError_t launch_attend(const AttendArgs& a, int n_sm, cudaStream_t st);
+
+cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, long long T, long long stride, const int* starts,
+                             long long max_new, bool vec, cudaStream_t st);
+cudaError_t launch_kv_evict(const KvArgs& kv, int* spare, int budget, int sinks, int recent, int* kept, cudaStream_t st);
+
+}  // namespace h3

@@ -17,6 +17,14 @@ F32, F16, BF16 = 0, 1, 2  # kernels/h3sycl.h:21
 
 P, I, I64, U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64
 
+
+class KVCacheStruct(ctypes.Structure):
+    """``h3s_kv_cache`` of include/h3cuda.h."""
+
+    _fields_ = ([(n, P) for n in ("k", "v", "k_scale", "v_scale", "tail_k", "tail_v", "weight", "tail_weight", "table", "lens")]
+                + [(n, I64) for n in ("pages", "seqs", "width", "heads", "dim")] + [("dt", ctypes.c_int32)])
+
+
 # (name, restype, argtypes): every entry point of include/h3cuda.h
 CUDA_SYMBOLS = [
     ("h3s_last_error", ctypes.c_char_p, []),
@@ -57,6 +65,12 @@ CUDA_SYMBOLS = [
     ("h3s_stream", P, [P]),
     ("h3s_selftest_wait_timeout", I, [P, U64]),
     ("h3s_attention_sage_static", I, [P, P, P, P, I64, I64, I64, I64, P, I, P]),
+    ("h3s_kv_append", I, [P, P, P, P, I64, I64, P, I64]),
+    ("h3s_attention_cached", I, [P, P, P, I64, I64, I64, P, I64, I64, P, I, P, U64]),
+    ("h3s_attention_cached_work", U64, [P, P, I64, I64, I64, I64, I]),
+    ("h3s_kv_evict", I, [P, P, P, I64, I64, I64, P, U64]),
+    ("h3s_int4_linear", I, [P, P, I, I64, I64, P, I64, P, P, I, I, P, P, I]),
+    ("h3s_int4_pack", I, [P, P, I64, I64, P]),
 ]
 # every entry point of include/h3sage.h
 SAGE_SYMBOLS = [
@@ -262,6 +276,30 @@ class Context:
                            out_dt: int, wq: int, wk: int, eps: float, cs: int, rot_dim: int) -> None:
         check(self._lib.h3s_attention_rms_rope(self.handle, q, k, v, dt, S, H, D, stride, out, out_dt, wq, wk, eps, cs,
                                                rot_dim), "h3s_attention_rms_rope")
+
+    # ---- the text model's cache and 4-bit layers (kv: the address of a KVCacheStruct) ----
+    def kv_append(self, kv: int, k: int, v: int, T: int, stride: int, starts: int, max_new: int) -> None:
+        check(self._lib.h3s_kv_append(self.handle, kv, k, v, T, stride, starts, max_new), "h3s_kv_append")
+
+    def attention_cached(self, kv: int, q: int, T: int, Hq: int, qs: int, starts: int, max_new: int, max_len: int, out: int,
+                         accumulate: int, work: int, work_bytes: int) -> None:
+        check(self._lib.h3s_attention_cached(self.handle, kv, q, T, Hq, qs, starts, max_new, max_len, out, accumulate, work,
+                                             work_bytes), "h3s_attention_cached")
+
+    def attention_cached_work(self, kv: int, T: int, Hq: int, max_new: int, max_len: int, accumulate: int) -> int:
+        return self._lib.h3s_attention_cached_work(self.handle, kv, T, Hq, max_new, max_len, accumulate)
+
+    def kv_evict(self, kv: int, spare: int, budget: int, sinks: int, recent: int, work: int,
+                 work_bytes: int) -> None:
+        check(self._lib.h3s_kv_evict(self.handle, kv, spare, budget, sinks, recent, work, work_bytes), "h3s_kv_evict")
+
+    def int4_linear(self, x: int, x_dt: int, M: int, K: int, tiles: int, N: int, scale: int, zero: int, s_dt: int, group: int,
+                    bias: int, out: int, out_dt: int) -> None:
+        check(self._lib.h3s_int4_linear(self.handle, x, x_dt, M, K, tiles, N, scale, zero, s_dt, group, bias, out, out_dt),
+              "h3s_int4_linear")
+
+    def int4_pack(self, codes: int, N: int, K: int, tiles: int) -> None:
+        check(self._lib.h3s_int4_pack(self.handle, codes, N, K, tiles), "h3s_int4_pack")
 
     def selftest_wait_timeout(self, wait_ns: int) -> None:
         check(self._lib.h3s_selftest_wait_timeout(self.handle, wait_ns), "h3s_selftest_wait_timeout")

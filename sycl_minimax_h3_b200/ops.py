@@ -7,24 +7,25 @@ the layouts exactly as the reference does, then call ``h3s_attention`` / ``h3s_a
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
 
-from .native import Context, H3Error, dt_code
+from .native import Context, H3Error, KVCacheStruct, dt_code
 
 _ctx: dict[tuple[int, int], Context] = {}
 
 
 def context(device=None) -> Context:
     """The h3s context of a device around PyTorch's current stream on it (made once per (device, stream))."""
-    dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
-    with torch.cuda.device(dev):
-        s = torch.cuda.current_stream()
-        key = (dev.index, int(s.cuda_stream))
-        if key not in _ctx:
+    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    s = torch.cuda.current_stream(index)
+    key = (index, int(s.cuda_stream))
+    if key not in _ctx:
+        with torch.cuda.device(index):
             _ctx[key] = Context(s)
-        return _ctx[key]
+    return _ctx[key]
 
 
 @dataclass(frozen=True)
@@ -174,3 +175,214 @@ def attention_rms_rope(q: Rows, k: Rows, v: Rows, out: torch.Tensor, q_norm: tor
                            out.data_ptr(), dt_code(out.dtype), _floats(q_norm, "the q norm weight", q.dim),
                            _floats(k_norm, "the k norm weight", q.dim), eps,
                            _floats(cs, "the rotation table", q.tokens * rot_dim), rot_dim)
+
+
+# ---- the text model token by token: an 8-bit key/value cache and 4-bit linear layers (include/h3cuda.h) ----
+
+PAGE = 64  # tokens of a page
+
+
+def _part(t: torch.Tensor, what: str, dtype: torch.dtype, shape, device) -> int:
+    """The address of a contiguous tensor of this type, shape and device."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+        raise H3Error(f"{what}: contiguous {dtype} {list(shape)} on {device} expected, got {t.dtype} {list(t.shape)} on "
+                      f"{t.device}")
+    return t.data_ptr()
+
+
+def _on_gpu(device: torch.device, what: str) -> None:
+    if device.type != "cuda":
+        raise H3Error(f"{what}: the tensors must be on a GPU, not on {device}")
+
+
+@dataclass(frozen=True, eq=False)
+class KVCache:
+    """The keys and values of a batch of growing sequences in 8 bits (``h3s_kv_cache``): ``k``, ``v`` int8 [pages, heads,
+    64, dim] with ``k_scale``, ``v_scale`` float32 [pages, heads]; ``tail_k``, ``tail_v`` [seqs, heads, 64, dim] in the
+    rows' type, the tokens that do not fill a page yet; ``table`` int32 [seqs, width] page ids, ``lens`` int32 [seqs] tokens
+    (those of the current call included); ``weight`` float32 [pages, heads, 64] and ``tail_weight`` [seqs, heads, 64], the
+    attention weight that each token has received, where tokens are evicted by it. dim is 64 or 128.
+
+    ``lens`` and ``table`` are the caller's to change, on the device, between calls; which pages are free is the caller's
+    to keep. The tensors themselves stay: their addresses are taken down once."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    tail_k: torch.Tensor
+    tail_v: torch.Tensor
+    table: torch.Tensor
+    lens: torch.Tensor
+    weight: torch.Tensor | None = None
+    tail_weight: torch.Tensor | None = None
+
+    def __post_init__(self):
+        if self.k.dim() != 4 or self.k.shape[2] != PAGE or self.table.dim() != 2:
+            raise H3Error(f"KVCache: k [pages, heads, {PAGE}, dim] and table [seqs, width] expected, got {list(self.k.shape)} "
+                          f"and {list(self.table.shape)}")
+        pages, heads, _, dim = self.k.shape
+        seqs, width = self.table.shape
+        dt, dev, i8, f32, i32 = self.tail_k.dtype, self.k.device, torch.int8, torch.float32, torch.int32
+        if dim not in (64, 128):
+            raise H3Error(f"KVCache: heads of 64 or 128 features (got {dim})")
+        if (self.weight is None) != (self.tail_weight is None):
+            raise H3Error("KVCache: weight and tail_weight come together")
+        s = KVCacheStruct(
+            _part(self.k, "KVCache: k", i8, self.k.shape, dev), _part(self.v, "KVCache: v", i8, self.k.shape, dev),
+            _part(self.k_scale, "KVCache: k_scale", f32, (pages, heads), dev),
+            _part(self.v_scale, "KVCache: v_scale", f32, (pages, heads), dev),
+            _part(self.tail_k, "KVCache: tail_k", dt, (seqs, heads, PAGE, dim), dev),
+            _part(self.tail_v, "KVCache: tail_v", dt, (seqs, heads, PAGE, dim), dev),
+            None if self.weight is None else _part(self.weight, "KVCache: weight", f32, (pages, heads, PAGE), dev),
+            None if self.tail_weight is None else _part(self.tail_weight, "KVCache: tail_weight", f32, (seqs, heads, PAGE), dev),
+            _part(self.table, "KVCache: table", i32, (seqs, width), dev), _part(self.lens, "KVCache: lens", i32, (seqs,), dev),
+            pages, seqs, width, heads, dim, dt_code(dt))
+        object.__setattr__(self, "_struct", s)
+        object.__setattr__(self, "_ptr", ctypes.addressof(s))
+        object.__setattr__(self, "_work", {})
+
+    @staticmethod
+    def empty(pages: int, seqs: int, width: int, heads: int, dim: int, dtype: torch.dtype, device="cuda",
+              weights: bool = False) -> "KVCache":
+        """A cache without a token: room for ``pages`` pages, ``width`` of them at most for each of ``seqs`` sequences. The
+        table is -1 throughout: pages are given out by writing their ids into it."""
+        f32, kw = torch.float32, {"device": device}
+        return KVCache(torch.zeros(pages, heads, PAGE, dim, dtype=torch.int8, **kw),
+                       torch.zeros(pages, heads, PAGE, dim, dtype=torch.int8, **kw),
+                       torch.zeros(pages, heads, dtype=f32, **kw), torch.zeros(pages, heads, dtype=f32, **kw),
+                       torch.zeros(seqs, heads, PAGE, dim, dtype=dtype, **kw),
+                       torch.zeros(seqs, heads, PAGE, dim, dtype=dtype, **kw),
+                       torch.full((seqs, width), -1, dtype=torch.int32, **kw), torch.zeros(seqs, dtype=torch.int32, **kw),
+                       torch.zeros(pages, heads, PAGE, dtype=f32, **kw) if weights else None,
+                       torch.zeros(seqs, heads, PAGE, dtype=f32, **kw) if weights else None)
+
+    def _rows(self, what: str, x: Rows) -> int:
+        if x.dim != self.k.shape[3] or x.t.dtype != self.tail_k.dtype or x.t.device != self.k.device:
+            raise H3Error(f"{what}: {x.t.dtype} rows with heads of {x.dim} on {x.t.device}, but the cache has {self.tail_k.dtype} "
+                          f"and {self.k.shape[3]} on {self.k.device}")
+        return x.ptr()
+
+    def _starts(self, what: str, starts: torch.Tensor) -> int:
+        return _part(starts, f"{what}: starts", torch.int32, (self.table.shape[0] + 1,), self.k.device)
+
+
+def kv_append(cache: KVCache, k: Rows, v: Rows, starts: torch.Tensor, max_new: int | None = None) -> None:
+    """The rows of new tokens into the cache (``h3s_kv_append``): sequence b's are the rows starts[b] .. starts[b+1] - 1 of
+    k and v, and the last ones of its ``cache.lens[b]`` tokens. A block of 64 tokens that is full is quantised, the others
+    stay in the tail as they are. ``max_new`` (about the most that one sequence gets) only divides the work."""
+    if k.layout() != v.layout():
+        raise H3Error("kv_append: k and v must have the same layout")
+    if k.heads != cache.k.shape[1]:
+        raise H3Error(f"kv_append: {k.heads} heads for a cache of {cache.k.shape[1]}")
+    kp, vp, sp = cache._rows("kv_append", k), cache._rows("kv_append", v), cache._starts("kv_append", starts)
+    _on_gpu(cache.k.device, "kv_append")
+    context(cache.k.device).kv_append(cache._ptr, kp, vp, k.tokens, k.stride, sp, max_new or 0)
+
+
+def attention_cached(q: Rows, cache: KVCache, starts: torch.Tensor, out: torch.Tensor, max_new: int | None = None,
+                     max_len: int | None = None, accumulate: bool = False) -> None:
+    """Causal attention with grouped heads over the cache (``h3s_attention_cached``): query rows starts[b] .. starts[b+1] - 1
+    are the last tokens of sequence b and see every token up to their own; out [q.tokens, q.heads * dim]. A row that sees
+    nothing is 0; rows behind the last sequence are left as they were. ``accumulate`` adds the weight that every token
+    receives to ``cache.weight``. ``max_new`` and ``max_len`` (about the most new tokens, and the longest sequence) only
+    divide the work."""
+    heads, dim = cache.k.shape[1], cache.k.shape[3]
+    if q.heads == 0 or q.heads % heads != 0:
+        raise H3Error(f"attention_cached: {q.heads} query heads over {heads} key/value heads")
+    if accumulate and cache.weight is None:
+        raise H3Error("attention_cached: the cache keeps no weights")
+    if out.dtype != q.t.dtype or out.numel() != q.tokens * q.heads * dim or not out.is_contiguous() or out.device != q.t.device:
+        raise H3Error(f"attention_cached: out {list(out.shape)} {out.dtype} for {q.tokens} tokens of {q.heads} x {dim} in "
+                      f"{q.t.dtype}")
+    qp, sp = cache._rows("attention_cached", q), cache._starts("attention_cached", starts)
+    _on_gpu(cache.k.device, "attention_cached")
+    ctx = context(cache.k.device)
+    key = (q.tokens, q.heads, max_new, max_len, accumulate)
+    nbytes = cache._work.get(key)
+    if nbytes is None:
+        if len(cache._work) >= 256:
+            cache._work.clear()
+        nbytes = cache._work[key] = ctx.attention_cached_work(cache._ptr, q.tokens, q.heads, max_new or 0, max_len or 0, accumulate)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=cache.k.device) if nbytes else None
+    ctx.attention_cached(cache._ptr, qp, q.tokens, q.heads, q.stride, sp, max_new or 0, max_len or 0, out.data_ptr(),
+                         int(accumulate), work.data_ptr() if nbytes else 0, nbytes)
+
+
+def kv_evict(cache: KVCache, spare: torch.Tensor, budget: int, sinks: int = 4, recent: int = PAGE) -> None:
+    """Cuts every sequence longer than ``budget`` tokens (a multiple of 64) to it (``h3s_kv_evict``): each head keeps its
+    first ``sinks`` and last ``recent`` tokens and those of the others with the largest ``cache.weight``. They move to the
+    pages ``spare`` int32 [seqs, budget / 64], which change places with the sequence's old ones in ``cache.table``."""
+    if cache.weight is None:
+        raise H3Error("kv_evict: the cache keeps no weights")
+    if budget <= 0 or budget % PAGE:
+        raise H3Error(f"kv_evict: the budget must be a multiple of {PAGE} (got {budget})")
+    if sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise H3Error(f"kv_evict: {sinks} first and {recent} last tokens do not fit a budget of {budget}")
+    seqs, heads = cache.table.shape[0], cache.k.shape[1]
+    sp = _part(spare, "kv_evict: spare", torch.int32, (seqs, budget // PAGE), cache.k.device)
+    _on_gpu(cache.k.device, "kv_evict")
+    nbytes = 4 * seqs * heads * budget
+    work = torch.empty(nbytes, dtype=torch.uint8, device=cache.k.device)
+    context(cache.k.device).kv_evict(cache._ptr, sp, budget, sinks, recent, work.data_ptr(), nbytes)
+
+
+@dataclass(frozen=True, eq=False)
+class Int4Linear:
+    """A linear layer with 4-bit weights W[n, k] = scale[k // group, n] * (code[n, k] - zero[k // group, n]) for a few rows
+    at a time (``h3s_int4_linear``): ``tiles`` the codes as ``pack`` lays them out, ``scale`` (and ``zero``, or None: 8)
+    [ceil(inputs / group), outputs] in a float type, ``group`` 32, 64, 128 or 0 (one scale per output), ``bias`` float32
+    [outputs] or None."""
+
+    tiles: torch.Tensor
+    scale: torch.Tensor
+    n: int
+    k: int
+    group: int
+    zero: torch.Tensor | None = None
+    bias: torch.Tensor | None = None
+
+    def __post_init__(self):
+        if self.group not in (0, 32, 64, 128):
+            raise H3Error(f"int4_linear: groups of 32, 64 or 128 inputs, or 0 (got {self.group})")
+        dev, groups = self.tiles.device, -(-self.k // self.group) if self.group else 1
+        _part(self.tiles, "int4_linear: tiles", torch.int32, (-(-self.n // 16), -(-self.k // 64), 128), dev)
+        dt_code(self.scale.dtype)
+        _part(self.scale, "int4_linear: scale", self.scale.dtype, (groups, self.n), dev)
+        if self.zero is not None:
+            _part(self.zero, "int4_linear: zero", self.scale.dtype, (groups, self.n), dev)
+        if self.bias is not None:
+            _part(self.bias, "int4_linear: bias", torch.float32, (self.n,), dev)
+
+    @staticmethod
+    def pack(codes: torch.Tensor, scale: torch.Tensor, group: int, zero: torch.Tensor | None = None,
+             bias: torch.Tensor | None = None) -> "Int4Linear":
+        """From codes uint8 [outputs, inputs / 2], input 2 i in the low four bits of byte i (``h3s_int4_pack``)."""
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
+            raise H3Error(f"int4_linear: contiguous uint8 codes [outputs, inputs / 2] expected, got {list(codes.shape)} {codes.dtype}")
+        _on_gpu(codes.device, "int4_linear")
+        n, k = codes.shape[0], codes.shape[1] * 2
+        tiles = torch.empty(-(-n // 16), -(-k // 64), 128, dtype=torch.int32, device=codes.device)
+        context(codes.device).int4_pack(codes.data_ptr(), n, k, tiles.data_ptr())
+        return Int4Linear(tiles, scale, n, k, group, zero, bias)
+
+    def inputs(self) -> int:
+        return self.k
+
+    def outputs(self) -> int:
+        return self.n
+
+    def forward(self, x: torch.Tensor, out: torch.Tensor) -> None:
+        """``out = linear(x)``: x [M, inputs] in a float type, out [M, outputs] in out's type."""
+        m = x.numel() // self.k if self.k else 0
+        if x.numel() != m * self.k or out.numel() != m * self.n:
+            raise H3Error(f"int4_linear: x {list(x.shape)} and out {list(out.shape)} do not fit a [{self.n}, {self.k}] weight")
+        for t, what in ((x, "x"), (out, "out")):
+            if not t.is_contiguous() or t.device != self.tiles.device:
+                raise H3Error(f"int4_linear: {what} must be contiguous, on {self.tiles.device}")
+        x_dt, out_dt = dt_code(x.dtype), dt_code(out.dtype)
+        _on_gpu(self.tiles.device, "int4_linear")
+        context(self.tiles.device).int4_linear(
+            x.data_ptr(), x_dt, m, self.k, self.tiles.data_ptr(), self.n, self.scale.data_ptr(),
+            self.zero.data_ptr() if self.zero is not None else 0, dt_code(self.scale.dtype), self.group,
+            self.bias.data_ptr() if self.bias is not None else 0, out.data_ptr(), out_dt)

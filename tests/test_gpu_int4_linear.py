@@ -1,0 +1,135 @@
+"""h3s_int4_linear and h3s_int4_pack on the GPU against the formula in 64 bits.
+
+Tolerance: the products are exact (a code less 8 is, and x enters whole), so an output is off by its own rounding (half a
+step of its type) and by the 32-bit sums: with A = sum |x| scale (|code - 8| + |zero - 8|), at most (K / 64 + 64) 2^-22 A: a warp
+adds a few of every 64 products in a row, cutting off instead of rounding at most, then come the group's scale, the other
+warps' sums and the bias."""
+import pytest
+import torch
+
+from sycl_minimax_h3_b200 import native, ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def make(M, N, K, group, x_dt, s_dt, zero, bias, device, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    groups = -(-K // group) if group else 1
+    codes = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8)
+    scale = (0.01 + 0.05 * torch.rand(groups, N, generator=g)).to(s_dt)
+    z = (5 + 6 * torch.rand(groups, N, generator=g)).to(s_dt) if zero else None
+    b = torch.randn(N, generator=g) if bias else None
+    x = torch.randn(M, K, generator=g).to(x_dt)
+    packed = (codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous().to(device)
+    lin = ops.Int4Linear.pack(packed, scale.to(device), group, None if z is None else z.to(device), None if b is None else b.to(device))
+    return codes, scale, z, b, x, lin
+
+
+def check(codes, scale, z, b, x, group, out):
+    K = codes.shape[1]
+    at = torch.arange(K) // (group or K)
+    s = scale.double().t()[:, at]
+    zero = torch.full_like(s, 8.0) if z is None else z.double().t()[:, at]
+    w = s * (codes.double() - zero)
+    xd = x.double()
+    want = xd @ w.t() + (0 if b is None else b.double())
+    A = xd.abs() @ (s * ((codes.double() - 8).abs() + (zero - 8).abs())).t() + (0 if b is None else b.double().abs())
+    bound = (K / 64 + 64) * 2.0 ** -22 * A
+    bound = bound + (want.abs() + bound) * (torch.finfo(out.dtype).eps / 2) + torch.finfo(out.dtype).tiny
+    off = (out.double().cpu() - want).abs() - bound
+    assert float(off.max()) <= 0, f"off by {float(off.max()):.3g} more than the roundings"
+
+
+@pytest.mark.parametrize("x_dt", TYPES)
+@pytest.mark.parametrize("group,zero", [(0, False), (32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 64), (1, 1, 2), (3, 33, 130), (8, 40, 512), (9, 100, 1000), (17, 64, 768), (70, 130, 448)])
+def test_linear(x_dt, group, zero, M, N, K, cuda):
+    s_dt = TYPES[(M + N) % 3]
+    codes, scale, z, b, x, lin = make(M, N, K, group, x_dt, s_dt, zero, M % 2 == 1, cuda, seed=M + N + K)
+    out = torch.empty(M, N, dtype=x_dt, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    check(codes, scale, z, b, x, group, out)
+
+
+@pytest.mark.parametrize("x_dt", TYPES)
+@pytest.mark.parametrize("out_dt", TYPES)
+def test_output_types_and_unaligned_x(x_dt, out_dt, cuda):
+    M, N, K = 5, 50, 264
+    codes, scale, z, b, x, lin = make(M, N, K, 32, x_dt, torch.float32, True, True, cuda, seed=1)
+    buf = torch.empty(M * K + 1, dtype=x_dt, device=cuda)
+    buf[1:] = x.reshape(-1).to(cuda)
+    room = torch.full((M * N + 5,), 7.0, dtype=out_dt, device=cuda)
+    lin.forward(buf[1:].view(M, K), room[3:3 + M * N].view(M, N))
+    ops.context(cuda).wait()
+    check(codes, scale, z, b, x, 32, room[3:3 + M * N].view(M, N))
+    assert bool((room[:3] == 7).all()) and bool((room[3 + M * N:] == 7).all())
+
+
+@pytest.mark.parametrize("M", [1, 4, 16, 33])
+def test_long_and_wide(M, cuda):
+    codes, scale, z, b, x, lin = make(M, 2000, 4096, 128, torch.bfloat16, torch.bfloat16, False, True, cuda, seed=2)
+    out = torch.empty(M, 2000, dtype=torch.float32, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    check(codes, scale, z, b, x, 128, out)
+
+
+def test_float32_keeps_all_its_bits(cuda):
+    """x of 24 bits against codes that pick one input each: the output is x times the scale, to the last bit."""
+    K, N = 64, 64
+    codes = torch.full((N, K), 8, dtype=torch.uint8)
+    codes[torch.arange(N), torch.arange(K)] = 9
+    scale = torch.ones(1, N)
+    packed = (codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous().to(cuda)
+    lin = ops.Int4Linear.pack(packed, scale.to(cuda), 0)
+    x = torch.randn(2, K, generator=torch.Generator().manual_seed(3))
+    x[0, :4] = torch.tensor([1 + 2.0 ** -23, -3.0e38, 1e-30, 0.0])
+    out = torch.empty(2, N, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    assert torch.equal(out.cpu(), x)
+
+
+@pytest.mark.parametrize("x_dt", TYPES)
+def test_nan_and_infinity_stay_in_their_row(x_dt, cuda):
+    codes, scale, z, b, x, lin = make(4, 32, 96, 32, x_dt, torch.float32, False, False, cuda, seed=4)
+    x[1, 7], x[2, 9] = float("nan"), float("inf")
+    out = torch.empty(4, 32, dtype=x_dt, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    assert bool(out[1].isnan().all()) and not bool(out[2].isfinite().any())
+    w = scale.double().t()[:, torch.arange(96) // 32] * (codes.double() - 8)
+    assert torch.equal(out[2].cpu().isnan(), (w[:, 9] == 0) | (x[2].double() @ w.t()).isnan())
+    keep = [0, 3]
+    check(codes, scale, z, b, x[keep], 32, out[keep])
+
+
+def test_pack_is_the_documented_layout(cuda):
+    """Lane (g, t), word w, nibble j + 4 e: output g + 8 (j % 2), input 32 (w / 2) + 8 t + 4 (w % 2) + 2 (j / 2) + e."""
+    N, K = 19, 70
+    codes = torch.randint(0, 16, (N, K), generator=torch.Generator().manual_seed(5), dtype=torch.uint8)
+    lin = ops.Int4Linear.pack((codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous().to(cuda), torch.ones(1, N, device=cuda), 0)
+    ops.context(cuda).wait()
+    tiles = lin.tiles.cpu()
+    for nt in range(2):
+        for kt in range(2):
+            for lane in range(32):
+                for w in range(4):
+                    word = int(tiles[nt, kt, lane * 4 + w]) & 0xffffffff
+                    for j in range(4):
+                        for e in range(2):
+                            n = nt * 16 + lane // 4 + 8 * (j % 2)
+                            k = kt * 64 + 32 * (w // 2) + 8 * (lane % 4) + 4 * (w % 2) + 2 * (j // 2) + e
+                            assert (word >> (4 * (j + 4 * e))) & 15 == (int(codes[n, k]) if n < N and k < K else 8)
+
+
+def test_refusals(cuda):
+    ctx = ops.context(cuda)
+    L = native.lib()
+    call = lambda **kw: L.h3s_int4_linear(ctx.handle, *{**dict(x=16, x_dt=0, M=1, K=64, t=16, N=16, s=16, z=0, s_dt=0, group=32, b=0, o=16, o_dt=0), **kw}.values())  # noqa: E731
+    assert call(M=0) == 0 and call(N=0) == 0 and call(K=0) == 0
+    for kw, why in (({"group": 16}, "groups"), ({"x_dt": 3}, "type"), ({"t": 8}, "16 bytes"), ({"s": 0}, "null")):
+        assert call(**kw) == -1 and why in native.last_error()
