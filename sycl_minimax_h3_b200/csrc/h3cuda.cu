@@ -1210,7 +1210,7 @@ static uint64_t attend_bytes(const AttendPlan& p, const h3s_kv_cache* kv, int64_
 static int check_attend(const char* who, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate, KvArgs& a) {
     if (check_kv(who, kv, accumulate != 0, a) != 0) return -1;
     if (Hq < 1 || Hq % kv->heads != 0) return kv_fail(who, "the query heads must be a multiple of the cache's heads");
-    if (T > INT32_MAX || Hq > INT32_MAX || (T > 0 && Hq > ((int64_t) 1 << 40) / T)) return kv_fail(who, "too many rows");
+    if (Hq > INT32_MAX - 16 || (T > 0 && T > (INT32_MAX - 16) / Hq)) return kv_fail(who, "too many rows");
     return 0;
 }
 
@@ -1235,7 +1235,6 @@ int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64
     const uint64_t need = attend_bytes(a.plan, kv, T, Hq, accumulate);
     if (need > 0 && (!work || !aligned16(work) || work_bytes < need))
         return kv_fail(who, "work of " + std::to_string(need) + " bytes on 16 bytes needed, " + std::to_string(work ? work_bytes : 0) + " given");
-    if (kv->seqs * kv->heads > INT32_MAX / a.plan.nz / a.plan.tiles) return kv_fail(who, "too many sequences, heads and rows for one call");
     DeviceGuard g(c.device);
     a.kv.err = c.err + 1;
     a.q = q;
@@ -1249,6 +1248,8 @@ int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64
     a.max_new = max_new;
     a.scale_log2 = (1.0f / std::sqrt((float) kv->dim)) * 1.4426950408889634f;
     a.q_vec = aligned16(q) && (qs * esize(kv->dt)) % 16 == 0;
+    a.wait_err = c.err;
+    a.wait_ns = c.wait_ns;
     const cudaError_t e = launch_attend(a, c.n_sm, c.st);
     return e == cudaSuccess ? 0 : cuda_fail(who, e);
 }

@@ -176,35 +176,55 @@ __global__ void __launch_bounds__(kAppThreads) kv_append(const KvArgs kv, const 
 }
 
 // ---- attention -------------------------------------------------------------------------------------------------------
-// The query rows of a kv head are its group's heads of every new token, row r = token * group + head, in tiles of 16: the
-// rows of an m16n8k16 product. Keys and values are codes, which fp16 holds exactly, so the products are q . code and
-// p . code on the fp16 tensor path with 32-bit sums, and a page's scales multiply the results:
-//   s_ij = (q_i . kc_j) * ks * log2(e)/sqrt(D)     p_ij = 2^(s_ij - m_i)     acc_i = acc_i 2^(m_old - m_i) + vs * sum_j p_ij vc_j
+// The query rows of a kv head are its group's heads of every new token, row r = token * group + head, in tiles of 8 NB:
+// the columns of m16n8k16 products whose 16 rows are keys (scores) or features (output), so that one tile of codes
+// serves 8 or 16 queries and a step's few queries leave little of a product empty.
+//   s_ji = (kc_j . q_i) * ks * log2(e)/sqrt(D)     p_ji = 2^(s_ji - m_i)     acc_i = acc_i 2^(m_old - m_i) + vs * sum_j vc_j p_ji
+//
+// Codes as fp16 operands: u = code + 128 in the low bits of 1024's mantissa, less 1152, is exact; one logic instruction
+// places u (flipped top bit, mask and the bits of 1024 at once), one subtracts. For the scores of 16-bit rows the
+// subtraction is saved: the bits 0x00 uu of a half are u 2^-24 exactly, and sum_d q_d (u_d - 128) starts from -128 sum q
+// instead of 0. Its partial sums are some four times as large, 2^-21 of the score or less beside the 2^-11 of p's
+// rounding; not so for P.V, whose p have one sign (sums of 128 p are 2^5 and more times the result), nor for float32.
 // q is brought to fp16 times a power of two per row, so that the row's largest value lies in [2^13, 2^14): exact for
 // fp16 and bf16 (what is more than 2^27 times smaller than the row's largest loses bits that a 32-bit sum would not
 // hold either); float32 takes two terms, 22 bits. p is rounded to fp16 (at most 2^-11 of it, beside 2^-8 or 2^-11 of the
 // output); for float32 it takes two terms too.
 //
 // Nothing is ordered inside a row's features: lane (g, t) of a warp reads 16-byte pieces of K (key g, features 16 t..),
-// and the query's fragment uses the same order. For P.V it reads features D/8 g.. of four keys, and accumulator i of a
-// lane is feature D/8 (2 t) + i and D/8 (2 t + 1) + i of rows g and g + 8.
+// and the query's fragment uses the same order. For P.V it reads features D/8 g.. of four keys, and accumulators
+// [i][..][e] of a lane are feature D/8 g + 2 i + e / 2 of query 2 t + e % 2.
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
+// an 8 x 8 matrix of halves, lane (g, t) holding row g's columns 2 t and 2 t + 1, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
-// four int8 -> two half2: the byte plus 128 in the low bits of 1024's mantissa, minus 1152
-__device__ __forceinline__ void i8x4_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    w ^= 0x80808080u;
-    lo = sub1152(__byte_perm(w, 0x64646464u, 0x4140));
-    hi = sub1152(__byte_perm(w, 0x64646464u, 0x4342));
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// per bit: 0 where m and k are 0, 1 where only k is, x where only m is, ~x where both are
+__device__ __forceinline__ uint32_t place(uint32_t x, uint32_t m, uint32_t k) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(m), "r"(k));
+    return y;
 }
+// bytes 0 and 2 of x as two halves: their codes, or (SHORT) code + 128 in units of 2^-24
+template <bool SHORT>
+__device__ __forceinline__ uint32_t codes02(uint32_t x) {
+    if constexpr (SHORT) return place(x, 0x00ff00ffu, 0x00800080u);
+    const uint32_t u = place(x, 0x00ff00ffu, 0x64806480u);
+    return half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480))));
+}
+constexpr float kCodeUnit = 16777216.0f;                   // 2^24
+// keeps the compiler from loading shared memory ahead of this point, which would cost more registers than there are
+__device__ __forceinline__ void load_fence() { asm volatile("" ::: "memory"); }
 
 // The keys that a tile of query rows sees, and how they are divided: np whole pages in pieces of cz pages, and the tail
 // (when seen) as a piece of its own, or with the last piece where no split is left.
@@ -230,294 +250,426 @@ constexpr int kAttWarps = 4;
 // 2^-28 of the row's largest (2^-14 without it), and 2^-39 of the largest is what it drops
 constexpr float kPTop = 14.0f;
 
-template <int D, bool TWO>
+template <int D, int NB, bool TWO>
 struct QFrag {
-    uint32_t hi[D / 16][4];
-    uint32_t lo[TWO ? D / 16 : 1][4];
-    float rs[2];                       // rows g and g + 8: 2^-e log2(e)/sqrt(D)
+    uint32_t hi[NB][D / 16][2];
+    uint32_t lo[TWO ? NB : 1][TWO ? D / 16 : 1][2];
+    float rs[NB][2];                   // queries 8 nb + 2 t and + 1: what their scores are multiplied by, with a page's scale
+    float s0[NB][2];                   //   and where their sums start
 };
 
-// rows g and g + 8 of a tile as A fragments; NULL rows are zero. qrow: element offsets, or -1.
-template <int DT, int D, bool TWO>
-__device__ __forceinline__ void load_q(QFrag<D, TWO>& f, const void* q, const long long (&qrow)[2], bool vec, float scale) {
+// rows 8 nb + g of a tile as B fragments; qrow: element offsets, or -1 for a row of zeros
+template <int DT, int D, int NB, bool TWO>
+__device__ __forceinline__ void load_q(QFrag<D, NB, TWO>& f, const void* q, const long long (&qrow)[NB], bool vec, float scale) {
     const int t = threadIdx.x & 3;
-    float x[2][D / 4];                 // features 64 c + 16 t .. + 15 of both rows
-    float top[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int nb = 0; nb < NB; ++nb) {
+        float x[D / 4];                // features 64 c + 16 t .. + 15
+        float top = 0.0f;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
 #pragma unroll
             for (int u = 0; u < 16; u += 8) {
-                float* y = &x[r][c * 16 + u];
-                if (qrow[r] >= 0) ld8<DT>(q, (size_t) qrow[r] + c * 64 + t * 16 + u, vec, y);
+                float* y = &x[c * 16 + u];
+                if (qrow[nb] >= 0) ld8<DT>(q, (size_t) qrow[nb] + c * 64 + t * 16 + u, vec, y);
                 else
 #pragma unroll
                     for (int i = 0; i < 8; ++i) y[i] = 0.0f;
             }
 #pragma unroll
         for (int i = 0; i < D / 4; ++i)
-            if (finite(x[r][i])) top[r] = fmaxf(top[r], fabsf(x[r][i]));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        // 2^e in two factors: each is a normal float, whatever the row's size (e from -152 to 114)
+            if (finite(x[i])) top = fmaxf(top, fabsf(x[i]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^e in two factors: each is a normal float, whatever the row's size (e from -162 to 114)
         int e = 0;
-        if (top[r] > 0.0f) e = ilogbf(top[r]) - 13;
+        if (top > 0.0f) e = ilogbf(top) - 13;
         const int e1 = e / 2, e2 = e - e1;
         const float m1 = __int_as_float((127 - e1) << 23), m2 = __int_as_float((127 - e2) << 23);
-        f.rs[r] = scale * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
+        float rs = scale * (TWO ? 1.0f : kCodeUnit) * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
+        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i) x[r][i] = x[r][i] * m1 * m2;
-    }
+        for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const float* y = &x[a & 1][ks * 4 + (a >> 1) * 2];
-            const __half2 h = __floats2half2_rn(y[0], y[1]);
-            f.hi[ks][a] = *reinterpret_cast<const uint32_t*>(&h);
-            if constexpr (TWO) {
+            for (int u = 0; u < 2; ++u) {                  // features 0 and 2, 1 and 3 of four, as codes02 has them
+                const float y0 = x[ks * 4 + u] * m1 * m2, y1 = x[ks * 4 + u + 2] * m1 * m2;
+                const __half2 h = __floats2half2_rn(y0, y1);
                 const float2 back = __half22float2(h);
-                const __half2 l = __floats2half2_rn(finite(y[0]) ? y[0] - back.x : 0.0f, finite(y[1]) ? y[1] - back.y : 0.0f);
-                f.lo[ks][a] = *reinterpret_cast<const uint32_t*>(&l);
+                f.hi[nb][ks][u] = half2_bits(h);
+                if constexpr (TWO)
+                    f.lo[nb][ks][u] = half2_bits(__floats2half2_rn(finite(y0) ? y0 - back.x : 0.0f, finite(y1) ? y1 - back.y : 0.0f));
+                else sum += back.x + back.y;
             }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= -128.0f / kCodeUnit;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f.rs[nb][u] = __shfl_sync(0xffffffffu, rs, 8 * t + 4 * u);
+            f.s0[nb][u] = TWO ? 0.0f : __shfl_sync(0xffffffffu, sum, 8 * t + 4 * u);
         }
+    }
 }
 
-// s[nt] = the scores of keys 8 nt + {2 t, 2 t + 1} of rows g (c0, c1) and g + 8 (c2, c3) over a page's codes, unscaled
-template <int D, bool TWO>
-__device__ __forceinline__ void page_scores(const QFrag<D, TWO>& f, const int8_t* kp, float (&s)[8][4]) {
+// s[mt][nb] = the scores of keys 16 mt + g (elements 0, 1) and + 8 (2, 3) with queries 8 nb + 2 t + {0, 1}, unscaled
+template <int D, int NB, bool TWO>
+__device__ __forceinline__ void page_scores(const QFrag<D, NB, TWO>& f, const int8_t* kp, float (&s)[4][NB][4]) {
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt) {
+    for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] = 0.0f;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(kp + (nt * 8 + g) * D + c * 64 + t * 16);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            for (int i = 0; i < 4; ++i) s[mt][nb][i] = f.s0[nb][i & 1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t b0, b1;
-                i8x4_half(u[i], b0, b1);
-                const int ks = c * 4 + i;
-                mma16816(s[nt], f.hi[ks][0], f.hi[ks][1], f.hi[ks][2], f.hi[ks][3], b0, b1);
-                if constexpr (TWO) mma16816(s[nt], f.lo[ks][0], f.lo[ks][1], f.lo[ks][2], f.lo[ks][3], b0, b1);
+    for (int c = 0; c < D / 64; ++c) {
+        load_fence();
+        uint32_t w[4][2][4];
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint4 u = *reinterpret_cast<const uint4*>(kp + (mt * 16 + r * 8 + g) * D + c * 64 + t * 16);
+                w[mt][r][0] = u.x; w[mt][r][1] = u.y; w[mt][r][2] = u.z; w[mt][r][3] = u.w;
             }
-        }
+        // the key tiles' products side by side: sums that do not wait for one another
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                const uint32_t a0 = codes02<!TWO>(w[mt][0][i]), a2 = codes02<!TWO>(w[mt][0][i] >> 8);
+                const uint32_t a1 = codes02<!TWO>(w[mt][1][i]), a3 = codes02<!TWO>(w[mt][1][i] >> 8);
+                const int ks = c * 4 + i;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    mma16816(s[mt][nb], a0, a1, a2, a3, f.hi[nb][ks][0], f.hi[nb][ks][1]);
+                    if constexpr (TWO) mma16816(s[mt][nb], a0, a1, a2, a3, f.lo[nb][ks][0], f.lo[nb][ks][1]);
+                }
+            }
     }
 }
 
-// Scores of the tail's keys in plain 32-bit arithmetic, sc[row][key] in log2 units: qf [16][D] as floats, kt the tail's
-// rows of this head in dt. 128 threads; rows at or past nrow and keys at or past nkey are left alone.
-template <int DT, int D>
-__device__ __forceinline__ void tail_scores(const float* qf, const void* kt, size_t kbase, int nrow, int nkey, float scale,
-                                            float (*sc)[kPage]) {
+// A page's codes come into shared memory by bulk copies, K and V of a page in turn through a ring of two 64 x D tiles per
+// warp: one or two are in flight while one is read.
+constexpr int kSlots = 2;
+
+template <int D, int NB>
+struct AttSmem {
+    union {
+        int8_t ring[kAttWarps][kSlots][kPage * D];
+        float acc[kAttWarps + 1][8 * NB][D];               // the warps' accumulators, then the tail's
+        unsigned char tail[2][(kPage - 1) * D * 4];        // the tail's keys and values
+    };
+    float q[8 * NB][D];
+    float sc[kPage][8 * NB];                               // the tail's scores, then its p: [key][row]
+    float m[kAttWarps + 1][8 * NB], l[kAttWarps + 1][8 * NB];
+    int pos[8 * NB];
+    int row[8 * NB];                                       // token * Hq + head, or -1
+    long long qoff[8 * NB];                                // the query row's first element, or -1
+    uint64_t full[kAttWarps][kSlots];
+    uint64_t tail_full;
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// Scores of the tail's keys in plain 32-bit arithmetic, sc[key][row] in log2 units: qf [rows][D] as floats, kt the tail's
+// rows in dt (shared memory). 128 threads, each a key and half of the rows; a thread starts at the 16-byte piece that its
+// key's number names, so that neighbouring keys, whose rows start in the same banks, read different ones.
+template <int DT, int D, int ROWS>
+__device__ __forceinline__ void tail_scores(const float (*qf)[D], const unsigned char* kt, int nrow, int nkey, float scale,
+                                            float (*sc)[ROWS]) {
+    constexpr int E = 16 / DtInfo<DT>::ES, N = D / E;      // elements of a piece, pieces of a row
     const int key = threadIdx.x & 63, half = threadIdx.x >> 6, per = (nrow + 1) / 2;
     const int r0 = half * per, r1 = min(nrow, r0 + per);
     if (key >= nkey) return;
-    float acc[8];
+    float acc[ROWS / 2];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) acc[r] = 0.0f;
-    for (int d = 0; d < D; d += 8) {
-        float x[8];
-        ld8<DT>(kt, kbase + (size_t) key * D + d, true, x);
+    for (int r = 0; r < ROWS / 2; ++r) acc[r] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+        const int d = (i + key) % N * E;
+        float x[E];
+        cvt16<DT>(*reinterpret_cast<const uint4*>(kt + (key * D + d) * DtInfo<DT>::ES), x);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+        for (int r = 0; r < ROWS / 2; ++r) {
             if (r0 + r >= r1) break;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) acc[r] = fmaf(qf[(r0 + r) * D + d + u], x[u], acc[r]);
+            for (int u = 0; u < E; u += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(&qf[r0 + r][d + u]);
+                acc[r] = fmaf(y.x, x[u], acc[r]);
+                acc[r] = fmaf(y.y, x[u + 1], acc[r]);
+                acc[r] = fmaf(y.z, x[u + 2], acc[r]);
+                acc[r] = fmaf(y.w, x[u + 3], acc[r]);
+            }
         }
     }
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-        if (r0 + r < r1) sc[r0 + r][key] = acc[r] * scale;
+    for (int r = 0; r < ROWS / 2; ++r)
+        if (r0 + r < r1) sc[key][r0 + r] = acc[r] * scale;
 }
 
-template <int D>
-struct AttSmem {
-    float acc[kAttWarps + 1][16][D];   // the warps' accumulators, then the tail's
-    float m[kAttWarps + 1][16], l[kAttWarps + 1][16];
-    float q[16][D];
-    float sc[16][kPage];
-    int pos[16];
-    long long row[16];                 // global row (token * Hq + head), or -1
-};
-
-template <int DT, int D>
-__global__ void __launch_bounds__(kAttWarps * 32) attend(const AttendArgs a) {
+template <int DT, int D, int NB>
+__global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const __grid_constant__ AttendArgs a) {
     constexpr bool TWO = DT == F32;
-    constexpr int DG = D / 8;
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    AttSmem<D>& sm = *reinterpret_cast<AttSmem<D>*>(smem_raw);
+    constexpr int DG = D / 8, ROWS = 8 * NB;
+    constexpr uint32_t TILE = kPage * D;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    AttSmem<D, NB>& sm = *reinterpret_cast<AttSmem<D, NB>*>(smem_raw);
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.Hq / kv.heads, nz = a.plan.nz;
-    long long unit = blockIdx.x;
-    const int tile0 = (int) (unit % a.plan.tiles);
-    unit /= a.plan.tiles;
-    const int z = (int) (unit % nz);
-    unit /= nz;
-    const int h = (int) (unit % kv.heads), b = (int) (unit / kv.heads);
+    const int b = (int) (blockIdx.x / kv.heads), h = (int) (blockIdx.x % kv.heads), z = blockIdx.y;
     const Seq s = load_seq(kv, a.starts, a.T, b);
     if (!s.ok) {
         if (threadIdx.x == 0) atomicOr(kv.err, kErrLen);
         return;
     }
-    const long long R = (long long) s.n * group;
-    for (long long r0 = (long long) tile0 * 16; r0 < R; r0 += (long long) a.plan.tiles * 16) {
-        const int nrow = (int) min(R - r0, 16ll);
-        const int last_pos = s.L - s.n + (int) ((r0 + nrow - 1) / group);
+    const int R = s.n * group;
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < kAttWarps; ++w)
+            for (int i = 0; i < kSlots; ++i) mbar_init(&sm.full[w][i], 1);
+        mbar_init(&sm.tail_full, 1);
+        fence_barrier_init();
+    }
+    uint32_t used = 0, issued = 0, tails = 0;              // tiles of this warp read and asked for; tails waited for
+    for (int tile = blockIdx.z; tile < (R + ROWS - 1) / ROWS; tile += gridDim.z) {
+        const int r0 = tile * ROWS, nrow = min(R - r0, ROWS);
+        const int last_pos = s.L - s.n + (r0 + nrow - 1) / group;
         const Pieces pc = pieces(s.L, last_pos, nz);
         if (z >= max(pc.nu, 1)) continue;
-        __syncthreads();                                   // the tile before has been written
-        if (threadIdx.x < 16) {
+        __syncthreads();                                   // the tile before has been written; the barriers are made
+        if (threadIdx.x < ROWS) {
             const int r = threadIdx.x;
             const bool in = r < nrow;
-            const int tok = in ? (int) ((r0 + r) / group) : 0, hq = h * group + (in ? (int) ((r0 + r) % group) : 0);
+            const int tok = (r0 + r) / group, hq = h * group + (r0 + r) % group;
             sm.pos[r] = in ? s.L - s.n + tok : -1;
-            sm.row[r] = in ? (long long) (s.s0 + tok) * a.Hq + hq : -1;
+            sm.row[r] = in ? (s.s0 + tok) * a.Hq + hq : -1;
+            sm.qoff[r] = in ? (long long) (s.s0 + tok) * a.qs + hq * D : -1;
         }
+        fence_proxy_async_smem();                          // the ring was written as accumulators
         __syncthreads();
-        auto qoff = [&](int r) {
-            const long long gr = sm.row[r];
-            return gr < 0 ? -1ll : gr / a.Hq * a.qs + gr % a.Hq * D;
-        };
-        float acc[DG][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        float acc[DG / 2][NB][4], m[NB][2], l[NB][2];
 #pragma unroll
-        for (int i = 0; i < DG; ++i)
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.0f;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) acc[i][u] = 0.0f;
+            for (int i = 0; i < DG / 2; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc[i][nb][u] = 0.0f;
+        }
         const int p0 = z * pc.cz, p1 = min(pc.np, p0 + pc.cz);
         if (p0 < p1) {
-            QFrag<D, TWO> f;
-            const long long qrow[2] = {qoff(g), qoff(g + 8)};
-            load_q<DT, D, TWO>(f, a.q, qrow, a.q_vec, a.scale_log2);
-            const int pos[2] = {sm.pos[g], sm.pos[g + 8]};
+            QFrag<D, NB, TWO> f;
+            int pos[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                pos[nb][0] = sm.pos[8 * nb + 2 * t];
+                pos[nb][1] = sm.pos[8 * nb + 2 * t + 1];
+            }
             const int first_pos = sm.pos[0];
-            for (int p = p0 + warp; p < p1; p += kAttWarps) {
-                const int page = kv.table[(size_t) b * kv.width + p];
-                if (!page_ok(kv, page)) {
-                    if (lane == 0) atomicOr(kv.err, kErrPage);
-                    continue;
+            bool have_q = false;
+            for (int sub = p0; sub < p1; sub += 32 * kAttWarps) {
+                // up to 32 pages of this warp: lane i keeps the i-th one's id and scales
+                const int mine = sub + warp + kAttWarps * lane;
+                int id = -1;
+                float ks = 0.0f, vs = 0.0f;
+                if (mine < p1) {
+                    id = kv.table[(size_t) b * kv.width + mine];
+                    if (!page_ok(kv, id)) {
+                        atomicOr(kv.err, kErrPage);
+                        id = -1;
+                    }
                 }
-                const size_t pb = (size_t) page * kv.heads + h;
-                float sc[8][4];
-                page_scores<D, TWO>(f, kv.k + pb * kPage * D, sc);
-                const float ks = kv.ks[pb], vs = kv.vs[pb];
-                const float f0 = ks * f.rs[0], f1 = ks * f.rs[1];
-                float mx[2] = {-INFINITY, -INFINITY};
-                const bool mask = nrow < 16 || p * kPage + kPage - 1 > first_pos;
-#pragma unroll
-                for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = sc[nt][i] * (i < 2 ? f0 : f1);
-                        if (mask && p * kPage + nt * 8 + 2 * t + (i & 1) > pos[i >> 1]) x = -INFINITY;
-                        sc[nt][i] = x;
-                        mx[i >> 1] = fmaxf(mx[i >> 1], x);
+                uint32_t ask = __ballot_sync(0xffffffffu, id >= 0), todo = ask;
+                bool ask_v = false;
+                auto next = [&]() {                        // the next tile into the slot that was freed last
+                    if (ask == 0) return;
+                    const int i = __ffs((int) ask) - 1, pid = __shfl_sync(0xffffffffu, id, i), slot = (int) (issued % kSlots);
+                    if (lane == 0) {
+                        mbar_expect_tx(&sm.full[warp][slot], TILE);
+                        bulk_load(sm.ring[warp][slot], (ask_v ? kv.v : kv.k) + ((size_t) pid * kv.heads + h) * TILE, TILE,
+                                  &sm.full[warp][slot]);
                     }
-                float al[2], mu[2];
+                    ++issued;
+                    if (ask_v) ask &= ask - 1;
+                    ask_v = !ask_v;
+                };
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    const float mn = fmaxf(m[r], mx[r] - kPTop);
-                    mu[r] = mn == -INFINITY ? 0.0f : mn;   // a row that sees nothing yet: every p is 2^-inf = 0
-                    al[r] = ex2(m[r] - mu[r]);
-                    m[r] = mn;
-                    l[r] *= al[r];
+                for (int i = 0; i < kSlots; ++i) next();
+                if (id >= 0) {
+                    ks = kv.ks[(size_t) id * kv.heads + h];
+                    vs = kv.vs[(size_t) id * kv.heads + h];
                 }
-                uint32_t ph[8][2], pl[TWO ? 8 : 1][2];
+                if (!have_q) {
+                    long long qrow[NB];
 #pragma unroll
-                for (int nt = 0; nt < 8; ++nt)
+                    for (int nb = 0; nb < NB; ++nb) qrow[nb] = sm.qoff[8 * nb + g];
+                    load_q<DT, D, NB, TWO>(f, a.q, qrow, a.q_vec, a.scale_log2);
+                    have_q = true;
+                }
+                auto arrived = [&]() {
+                    if (warp_wait(&sm.full[warp][used % kSlots], (used / kSlots) & 1, a.wait_ns, nullptr)) return true;
+                    if (lane == 0) atomicOr(a.wait_err, kErrCache);
+                    // give up: the copies in flight land before the memory is used for anything else
+                    for (uint32_t u = used; u < issued; ++u)
+                        warp_wait(&sm.full[warp][u % kSlots], (u / kSlots) & 1, a.wait_ns, nullptr);
+                    return false;
+                };
+                while (todo) {
+                    const int i = __ffs((int) todo) - 1, p = sub + warp + kAttWarps * i;
+                    todo &= todo - 1;
+                    const float kscale = __shfl_sync(0xffffffffu, ks, i), vscale = __shfl_sync(0xffffffffu, vs, i);
+                    if (!arrived()) { used = issued; break; }
+                    float sc[4][NB][4];
+                    page_scores<D, NB, TWO>(f, sm.ring[warp][used % kSlots], sc);
+                    __syncwarp();
+                    ++used;
+                    next();
+                    const bool mask = nrow < ROWS || p * kPage + kPage - 1 > first_pos;
+                    float al[NB][2];
+                    uint32_t ph[4][NB][2], pl[TWO ? 4 : 1][NB][2];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float e0 = ex2(sc[nt][2 * r] - mu[r]), e1 = ex2(sc[nt][2 * r + 1] - mu[r]);
-                        l[r] += e0 + e1;
-                        const __half2 hh = __floats2half2_rn(e0, e1);
-                        ph[nt][r] = *reinterpret_cast<const uint32_t*>(&hh);
-                        if constexpr (TWO) {
-                            const float2 back = __half22float2(hh);
-                            const __half2 ll = __floats2half2_rn(e0 - back.x, e1 - back.y);
-                            pl[nt][r] = *reinterpret_cast<const uint32_t*>(&ll);
+                    for (int nb = 0; nb < NB; ++nb) {
+                        float mu[2];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float fs = kscale * f.rs[nb][c];
+                            float mx = -INFINITY;
+#pragma unroll
+                            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) {
+                                    float x = sc[mt][nb][2 * r + c] * fs;
+                                    if (mask && p * kPage + mt * 16 + r * 8 + g > pos[nb][c]) x = -INFINITY;
+                                    sc[mt][nb][2 * r + c] = x;
+                                    mx = fmaxf(mx, x);
+                                }
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            const float mn = fmaxf(m[nb][c], mx - kPTop);
+                            mu[c] = mn == -INFINITY ? 0.0f : mn;   // a query that sees nothing yet: every p is 2^-inf = 0
+                            al[nb][c] = ex2(m[nb][c] - mu[c]);
+                            m[nb][c] = mn;
+                            l[nb][c] *= al[nb][c];
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float e0 = ex2(sc[mt][nb][2 * r] - mu[0]), e1 = ex2(sc[mt][nb][2 * r + 1] - mu[1]);
+                                l[nb][0] += e0;
+                                l[nb][1] += e1;
+                                const __half2 hh = __floats2half2_rn(e0, e1);
+                                ph[mt][nb][r] = transpose8(half2_bits(hh));
+                                if constexpr (TWO) {
+                                    const float2 back = __half22float2(hh);
+                                    pl[mt][nb][r] = transpose8(half2_bits(__floats2half2_rn(e0 - back.x, e1 - back.y)));
+                                }
+                            }
+                    }
+                    if (!arrived()) { used = issued; break; }
+                    const int8_t* vp = sm.ring[warp][used % kSlots];
+#pragma unroll
+                    for (int hf = 0; hf < DG / 8; ++hf) {  // 8 features of each lane's DG at a time
+                        load_fence();
+                        uint32_t w[4][4][2];               // 16 keys x 4 of them in this lane x 8 features
+#pragma unroll
+                        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                const int key = mt * 16 + (kk >> 1) * 8 + 2 * t + (kk & 1);
+                                const uint2 u = *reinterpret_cast<const uint2*>(vp + key * D + g * DG + hf * 8);
+                                w[mt][kk][0] = u.x;
+                                w[mt][kk][1] = u.y;
+                            }
+#pragma unroll
+                        for (int wd = 0; wd < 2; ++wd) {
+                            float c[2][NB][4];
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) c[u][nb][e] = 0.0f;
+#pragma unroll
+                            for (int mt = 0; mt < 4; ++mt) {
+                                uint32_t v[2][4];          // [keys 2t.. / 8 + 2t..][feature of the word]
+#pragma unroll
+                                for (int k2 = 0; k2 < 2; ++k2) {
+                                    const uint32_t x = w[mt][2 * k2][wd], y = w[mt][2 * k2 + 1][wd];
+                                    v[k2][0] = codes02<false>(__byte_perm(x, y, 0x5410));   // x's byte, y's byte at 0 and 2
+                                    v[k2][1] = codes02<false>(__byte_perm(x, y, 0x6521));
+                                    v[k2][2] = codes02<false>(__byte_perm(x, y, 0x7632));
+                                    v[k2][3] = codes02<false>(__byte_perm(x, y, 0x3743));
+                                }
+#pragma unroll
+                                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                    for (int nb = 0; nb < NB; ++nb) {
+                                        mma16816(c[u][nb], v[0][2 * u], v[0][2 * u + 1], v[1][2 * u], v[1][2 * u + 1], ph[mt][nb][0], ph[mt][nb][1]);
+                                        if constexpr (TWO)
+                                            mma16816(c[u][nb], v[0][2 * u], v[0][2 * u + 1], v[1][2 * u], v[1][2 * u + 1], pl[mt][nb][0], pl[mt][nb][1]);
+                                    }
+                            }
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        float& y = acc[hf * 4 + wd * 2 + u][nb][e];
+                                        y = fmaf(vscale, c[u][nb][e], y * al[nb][e & 1]);
+                                    }
                         }
                     }
-                const int8_t* vp = kv.v + pb * kPage * D;
-#pragma unroll
-                for (int hf = 0; hf < DG / 8; ++hf) {      // 8 features of each lane's DG at a time
-                    uint32_t w[4][4][2];                   // 16 keys x 4 of them in this lane x 8 features
-#pragma unroll
-                    for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            const int key = jj * 16 + (kk >> 1) * 8 + 2 * t + (kk & 1);
-                            const uint2 u = *reinterpret_cast<const uint2*>(vp + key * D + g * DG + hf * 8);
-                            w[jj][kk][0] = u.x ^ 0x80808080u;
-                            w[jj][kk][1] = u.y ^ 0x80808080u;
-                        }
-#pragma unroll
-                    for (int wd = 0; wd < 2; ++wd) {
-                        float c[4][4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) c[i][u] = 0.0f;
-#pragma unroll
-                        for (int jj = 0; jj < 4; ++jj) {
-                            uint32_t bb[2][4];             // [keys 2t.. / 8 + 2t..][feature of the word]
-#pragma unroll
-                            for (int k2 = 0; k2 < 2; ++k2) {
-                                const uint32_t x = w[jj][2 * k2][wd], y = w[jj][2 * k2 + 1][wd];
-                                const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);
-                                bb[k2][0] = sub1152(__byte_perm(lo, 0x64646464u, 0x4140));
-                                bb[k2][1] = sub1152(__byte_perm(lo, 0x64646464u, 0x4342));
-                                bb[k2][2] = sub1152(__byte_perm(hi, 0x64646464u, 0x4140));
-                                bb[k2][3] = sub1152(__byte_perm(hi, 0x64646464u, 0x4342));
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                mma16816(c[i], ph[2 * jj][0], ph[2 * jj][1], ph[2 * jj + 1][0], ph[2 * jj + 1][1], bb[0][i], bb[1][i]);
-                                if constexpr (TWO)
-                                    mma16816(c[i], pl[2 * jj][0], pl[2 * jj][1], pl[2 * jj + 1][0], pl[2 * jj + 1][1], bb[0][i], bb[1][i]);
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                float& y = acc[hf * 8 + wd * 4 + i][u];
-                                y = fmaf(vs, c[i][u], y * al[u >> 1]);
-                            }
-                    }
+                    __syncwarp();
+                    ++used;
+                    next();
                 }
             }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (t == 0) {
-                sm.m[warp][g + 8 * r] = m[r];
-                sm.l[warp][g + 8 * r] = l[r];
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x = l[nb][c];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g == 0) {
+                    sm.m[warp][8 * nb + 2 * t + c] = m[nb][c];
+                    sm.l[warp][8 * nb + 2 * t + c] = x;
+                }
             }
-        }
-#pragma unroll
-        for (int i = 0; i < DG; ++i)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) sm.acc[warp][g + 8 * (u >> 1)][DG * (2 * t + (u & 1)) + i] = acc[i][u];
         const bool tail = z == pc.tail_at;
+        constexpr int TR = ROWS * D / (kAttWarps * 32);    // the tail's rows in a thread, of one feature
+        float ot[TR];
         if (tail) {                                        // CUDA cores: the tail is in its own type, at most 63 keys
-            for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32)
-                sm.q[i / D][i % D] = ld1<DT>(a.q, (size_t) qoff(i / D) + i % D);
-            __syncthreads();
             const int full = s.L / kPage, nkey = s.L - full * kPage;
-            const size_t tb = ((size_t) b * kv.heads + h) * kPage * D;
-            tail_scores<DT, D>(&sm.q[0][0], kv.tk, tb, nrow, nkey, a.scale_log2, sm.sc);
+            __syncthreads();                               // the ring has been read
+            if (threadIdx.x == 0) {
+                const size_t tb = ((size_t) b * kv.heads + h) * kPage * D * DtInfo<DT>::ES;
+                const uint32_t bytes = (uint32_t) (nkey * D * DtInfo<DT>::ES);
+                mbar_expect_tx(&sm.tail_full, 2 * bytes);
+                bulk_load(sm.tail[0], static_cast<const char*>(kv.tk) + tb, bytes, &sm.tail_full);
+                bulk_load(sm.tail[1], static_cast<const char*>(kv.tv) + tb, bytes, &sm.tail_full);
+            }
+            for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32)
+                sm.q[i / D][i % D] = ld1<DT>(a.q, (size_t) sm.qoff[i / D] + i % D);
+            if (!mbar_wait(&sm.tail_full, tails & 1, a.wait_ns, nullptr)) atomicOr(a.wait_err, kErrCache);
+            ++tails;
+            __syncthreads();
+            tail_scores<DT, D, ROWS>(sm.q, sm.tail[0], nrow, nkey, a.scale_log2, sm.sc);
             __syncthreads();
             for (int r = warp; r < nrow; r += kAttWarps) {
                 const int see = min(nkey, sm.pos[r] + 1 - full * kPage);
-                const float x0 = lane < see ? sm.sc[r][lane] : -INFINITY, x1 = lane + 32 < see ? sm.sc[r][lane + 32] : -INFINITY;
+                const float x0 = lane < see ? sm.sc[lane][r] : -INFINITY, x1 = lane + 32 < see ? sm.sc[lane + 32][r] : -INFINITY;
                 float mx = fmaxf(x0, x1);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -526,18 +678,50 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend(const AttendArgs a) {
                 float sum = e0 + e1;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                sm.sc[r][lane] = e0;
-                sm.sc[r][lane + 32] = e1;
+                sm.sc[lane][r] = e0;
+                sm.sc[lane + 32][r] = e1;
                 if (lane == 0) { sm.m[kAttWarps][r] = mx; sm.l[kAttWarps][r] = sum; }
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32) {
-                const int r = i / D, d = i % D, see = min(nkey, sm.pos[r] + 1 - full * kPage);
-                float o = 0.0f;
-                for (int key = 0; key < see; ++key) o = fmaf(sm.sc[r][key], ld1<DT>(kv.tv, tb + (size_t) key * D + d), o);
-                sm.acc[kAttWarps][r][d] = o;
+            // a thread has one feature and TR rows; a value that a row does not see is not multiplied by its p of 0
+            const int d = threadIdx.x % D, rb = threadIdx.x / D * TR;
+#pragma unroll
+            for (int r = 0; r < TR; ++r) ot[r] = 0.0f;
+            if (sm.pos[0] >= s.L - 1) {                    // every row sees the whole tail
+#pragma unroll
+                for (int r = 0; r < TR; r += 4) {
+                    if (rb + r >= nrow) break;
+#pragma unroll 8
+                    for (int key = 0; key < nkey; ++key) {
+                        const float x = ld1<DT>(sm.tail[1], (size_t) key * D + d);
+                        const float4 e = *reinterpret_cast<const float4*>(&sm.sc[key][rb + r]);
+                        ot[r] = fmaf(e.x, x, ot[r]);
+                        ot[r + 1] = fmaf(e.y, x, ot[r + 1]);
+                        ot[r + 2] = fmaf(e.z, x, ot[r + 2]);
+                        ot[r + 3] = fmaf(e.w, x, ot[r + 3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < TR; ++r) {
+                    if (rb + r >= nrow) break;
+                    const int see = min(nkey, sm.pos[rb + r] + 1 - full * kPage);
+#pragma unroll 4
+                    for (int key = 0; key < see; ++key) ot[r] = fmaf(sm.sc[key][rb + r], ld1<DT>(sm.tail[1], (size_t) key * D + d), ot[r]);
+                }
             }
         }
+        __syncthreads();                                   // ring and tail have been read: they become accumulators
+        if (tail)
+#pragma unroll
+            for (int r = 0; r < TR; ++r) sm.acc[kAttWarps][threadIdx.x / D * TR + r][threadIdx.x % D] = ot[r];
+#pragma unroll
+        for (int i = 0; i < DG / 2; ++i)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    *reinterpret_cast<float2*>(&sm.acc[warp][8 * nb + 2 * t + c][DG * g + 2 * i]) = make_float2(acc[i][nb][c], acc[i][nb][2 + c]);
         __syncthreads();
         // the pieces of this CTA as one: rows straight out, or a partial result per split
         const int parts = kAttWarps + (tail ? 1 : 0);
@@ -569,63 +753,77 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend(const AttendArgs a) {
     }
 }
 
-// The splits' partial results of a row as one, in the order of the splits: a warp per row.
+// The splits' partial results of a row as one: a CTA per row, whose warps take the splits in turn and then meet.
 template <int DT, int D>
-__global__ void __launch_bounds__(128) attend_join(const AttendArgs a) {
+__global__ void __launch_bounds__(128) attend_join(const __grid_constant__ AttendArgs a) {
+    __shared__ float so[4][D], sl[4];
     const KvArgs& kv = a.kv;
-    const int lane = threadIdx.x & 31, nz = a.plan.nz, group = a.Hq / kv.heads;
-    const long long per = a.max_new * a.Hq, unit = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit >= per * kv.seqs) return;
-    const int b = (int) (unit / per);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nz = a.plan.nz, group = a.Hq / kv.heads, rows = a.plan.rows;
+    const int b = blockIdx.x;
     const Seq s = load_seq(kv, a.starts, a.T, b);
     if (!s.ok) return;
     const float* mls = a.part + (size_t) a.T * a.Hq * nz * D;
-    for (long long i = unit % per; i < (long long) s.n * a.Hq; i += per) {
-        const int tok = (int) (i / a.Hq), hq = (int) (i % a.Hq);
-        const long long R = (long long) s.n * group, r0 = ((long long) tok * group + hq % group) / 16 * 16;
-        const int last_pos = s.L - s.n + (int) ((min(R, r0 + 16) - 1) / group);
+    for (int i = blockIdx.y; i < s.n * a.Hq; i += gridDim.y) {
+        const int tok = i / a.Hq, hq = i % a.Hq;
+        const int R = s.n * group, r0 = (tok * group + hq % group) / rows * rows;
+        const int last_pos = s.L - s.n + (min(R, r0 + rows) - 1) / group;
         const Pieces pc = pieces(s.L, last_pos, nz);
         if (pc.nu <= 1) continue;
         const size_t gr = (size_t) (s.s0 + tok) * a.Hq + hq;
+        const float* ml = mls + gr * nz * 2;
         float mx = -INFINITY;
-        for (int z = 0; z < pc.nu; ++z) mx = fmaxf(mx, mls[(gr * nz + z) * 2]);
+        for (int z = lane; z < pc.nu; z += 32) mx = fmaxf(mx, ml[2 * z]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float mu = mx == -INFINITY ? 0.0f : mx;
         float sum = 0.0f, o[D / 32];
 #pragma unroll
         for (int u = 0; u < D / 32; ++u) o[u] = 0.0f;
-        for (int z = 0; z < pc.nu; ++z) {
-            const float e = ex2(mls[(gr * nz + z) * 2] - mu);
-            sum = fmaf(e, mls[(gr * nz + z) * 2 + 1], sum);
+#pragma unroll 4
+        for (int z = warp; z < pc.nu; z += 4) {
+            const float e = ex2(ml[2 * z] - mu);
+            sum = fmaf(e, ml[2 * z + 1], sum);
 #pragma unroll
             for (int u = 0; u < D / 32; ++u) o[u] = fmaf(e, a.part[(gr * nz + z) * D + lane + 32 * u], o[u]);
         }
+        __syncthreads();                                   // the row before has been written
+        if (lane == 0) sl[warp] = sum;
 #pragma unroll
-        for (int u = 0; u < D / 32; ++u) st1<DT>(a.out, gr * D + lane + 32 * u, sum == 0.0f ? 0.0f : o[u] / sum);
-        if (a.lse && lane == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);
+        for (int u = 0; u < D / 32; ++u) so[warp][lane + 32 * u] = o[u];
+        __syncthreads();
+        sum = sl[0] + sl[1] + sl[2] + sl[3];
+        if (threadIdx.x < D) {
+            const int d = threadIdx.x;
+            const float y = so[0][d] + so[1][d] + so[2][d] + so[3][d];
+            st1<DT>(a.out, gr * D + d, sum == 0.0f ? 0.0f : y / sum);
+        }
+        if (a.lse && threadIdx.x == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);
     }
 }
 
 // weight[slot] += the sum over the group's query rows of p = 2^(s - lse): the scores once more, against the finished
 // sums. One CTA per (sequence, kv head, piece of the pages), the last piece also the tail; a page's sums stay in one warp.
 template <int DT, int D>
-__global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const AttendArgs a, int nzw) {
+__global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_constant__ AttendArgs a, int nzw) {
     constexpr bool TWO = DT == F32;
-    __shared__ float qs[16][D];
-    __shared__ float sc[16][kPage];
+    constexpr int NB = 1, ROWS = 8;
+    __shared__ __align__(16) float qs[ROWS][D];
+    __shared__ __align__(16) float sc[kPage][ROWS];
+    extern __shared__ __align__(16) unsigned char kt[];
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.Hq / kv.heads;
     const int z = (int) (blockIdx.x % nzw), h = (int) (blockIdx.x / nzw % kv.heads), b = (int) (blockIdx.x / nzw / kv.heads);
     const Seq s = load_seq(kv, a.starts, a.T, b);
     if (!s.ok || s.n == 0) return;
-    const long long R = (long long) s.n * group;
+    const int R = s.n * group;
     const int full = s.L / kPage;
-    auto place = [&](long long r, int& pos, long long& off, float& lse) {
+    auto place = [&](int r, int& pos, long long& off, float& lse) {
         pos = -1;
         off = -1;
         lse = INFINITY;
         if (r >= R) return;
-        const int tok = (int) (r / group), hq = h * group + (int) (r % group);
+        const int tok = r / group, hq = h * group + r % group;
         pos = s.L - s.n + tok;
         off = (long long) (s.s0 + tok) * a.qs + (long long) hq * D;
         lse = a.lse[(size_t) (s.s0 + tok) * a.Hq + hq];
@@ -635,46 +833,50 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const AttendArg
         if (!page_ok(kv, page)) continue;                  // already recorded by the attention
         const size_t pb = (size_t) page * kv.heads + h;
         const float ks = kv.ks[pb];
-        float sum[8][2];
+        float sum[4][2];
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt) sum[nt][0] = sum[nt][1] = 0.0f;
-        // the first row that sees slot 64 p
-        const long long from = max(0ll, (long long) (p * kPage - (s.L - s.n)) * group) / 16 * 16;
-        for (long long r0 = from; r0 < R; r0 += 16) {
-            int pos[2];
-            long long off[2];
-            float lse[2];
-            place(r0 + g, pos[0], off[0], lse[0]);
-            place(r0 + g + 8, pos[1], off[1], lse[1]);
-            QFrag<D, TWO> f;
-            load_q<DT, D, TWO>(f, a.q, off, a.q_vec, a.scale_log2);
-            float x[8][4];
-            page_scores<D, TWO>(f, kv.k + pb * kPage * D, x);
+        for (int mt = 0; mt < 4; ++mt) sum[mt][0] = sum[mt][1] = 0.0f;
+        // from the first row that sees slot 64 p on
+        for (int r0 = max(0, p * kPage - (s.L - s.n)) * group / ROWS * ROWS; r0 < R; r0 += ROWS) {
+            int pos, pos2[2];
+            long long off[1];
+            float lse, lse2[2];
+            place(r0 + g, pos, off[0], lse);
 #pragma unroll
-            for (int nt = 0; nt < 8; ++nt)
+            for (int c = 0; c < 2; ++c) {
+                pos2[c] = __shfl_sync(0xffffffffu, pos, 8 * t + 4 * c);
+                lse2[c] = __shfl_sync(0xffffffffu, lse, 8 * t + 4 * c);
+            }
+            QFrag<D, NB, TWO> f;
+            load_q<DT, D, NB, TWO>(f, a.q, off, a.q_vec, a.scale_log2);
+            float x[4][NB][4];
+            page_scores<D, NB, TWO>(f, kv.k + pb * kPage * D, x);
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = ex2(x[nt][i] * (ks * f.rs[i >> 1]) - lse[i >> 1]);
-                    if (p * kPage + nt * 8 + 2 * t + (i & 1) <= pos[i >> 1]) sum[nt][i & 1] += e;
+                    const float e = ex2(x[mt][0][i] * (ks * f.rs[0][i & 1]) - lse2[i & 1]);
+                    if (p * kPage + mt * 16 + (i >> 1) * 8 + g <= pos2[i & 1]) sum[mt][i >> 1] += e;
                 }
         }
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
+        for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float y = sum[nt][i];
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-                if (g == 0) atomicAdd(&kv.w[pb * kPage + nt * 8 + 2 * t + i], y);
+            for (int r = 0; r < 2; ++r) {
+                float y = sum[mt][r];
+                y += __shfl_xor_sync(0xffffffffu, y, 1);
+                y += __shfl_xor_sync(0xffffffffu, y, 2);
+                if (t == 0) atomicAdd(&kv.w[pb * kPage + mt * 16 + r * 8 + g], y);
             }
     }
     const int nkey = s.L - full * kPage;
     if (z != nzw - 1 || nkey == 0) return;
     const size_t tb = ((size_t) b * kv.heads + h) * kPage;
     float sum = 0.0f;
-    const long long from = max(0ll, (long long) (full * kPage - (s.L - s.n)) * group) / 16 * 16;
-    for (long long r0 = from; r0 < R; r0 += 16) {
-        const int nrow = (int) min(R - r0, 16ll);
+    for (int i = threadIdx.x; i < nkey * D * DtInfo<DT>::ES / 16; i += kAttWarps * 32)
+        reinterpret_cast<uint4*>(kt)[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(kv.tk) + tb * D * DtInfo<DT>::ES)[i];
+    for (int r0 = max(0, full * kPage - (s.L - s.n)) * group / ROWS * ROWS; r0 < R; r0 += ROWS) {
+        const int nrow = min(R - r0, ROWS);
         __syncthreads();
         for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32) {
             int pos;
@@ -684,7 +886,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const AttendArg
             qs[i / D][i % D] = ld1<DT>(a.q, (size_t) off + i % D);
         }
         __syncthreads();
-        tail_scores<DT, D>(&qs[0][0], kv.tk, tb * D, nrow, nkey, a.scale_log2, sc);
+        tail_scores<DT, D, ROWS>(qs, kt, nrow, nkey, a.scale_log2, sc);
         __syncthreads();
         if (threadIdx.x < nkey)
             for (int r = 0; r < nrow; ++r) {
@@ -692,7 +894,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const AttendArg
                 long long off;
                 float lse;
                 place(r0 + r, pos, off, lse);
-                if (full * kPage + (int) threadIdx.x <= pos) sum += ex2(sc[r][threadIdx.x] - lse);
+                if (full * kPage + (int) threadIdx.x <= pos) sum += ex2(sc[threadIdx.x][r] - lse);
             }
     }
     if (threadIdx.x < nkey) kv.tw[tb + threadIdx.x] += sum;
@@ -969,10 +1171,11 @@ cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, lon
 AttendPlan attend_plan(int n_sm, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
     AttendPlan p;
     const int64_t rows = std::min(max_new, T) * group;
-    p.tiles = (int) std::max<int64_t>(1, (rows + 15) / 16);
+    p.rows = rows <= 8 ? 8 : 16;
+    p.tiles = (int) std::min<int64_t>(std::max<int64_t>(1, (rows + p.rows - 1) / p.rows), 65535);
     const int64_t pages = (max_len + kPage - 1) / kPage, units = seqs * heads * p.tiles;
     const int64_t most = (pages + kMinPages - 1) / kMinPages;
-    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, (n_sm * 8 + units - 1) / units, 512}));
+    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, (n_sm * 3 * (units > n_sm ? 4 : 1) + units - 1) / units, 512}));
     return p;
 }
 
@@ -988,25 +1191,30 @@ cudaError_t allow_smem(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {
     return e;
 }
 
+template <int DT, int D, int NB>
+cudaError_t attend_nb(const AttendArgs& a, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
+    const cudaError_t e = allow_smem(ready, attend<DT, D, NB>, sizeof(AttSmem<D, NB>));
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned) (a.kv.seqs * a.kv.heads), (unsigned) a.plan.nz, (unsigned) a.plan.tiles);
+    attend<DT, D, NB><<<grid, kAttWarps * 32, sizeof(AttSmem<D, NB>), st>>>(a);
+    return cudaGetLastError();
+}
+
 template <int DT, int D>
 cudaError_t attend_dt(const AttendArgs& a, int n_sm, cudaStream_t st) {
-    static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
-    cudaError_t e = allow_smem(ready, attend<DT, D>, sizeof(AttSmem<D>));
-    if (e != cudaSuccess) return e;
     const KvArgs& kv = a.kv;
-    const long long grid = (long long) kv.seqs * kv.heads * a.plan.nz * a.plan.tiles;
-    attend<DT, D><<<(unsigned) grid, kAttWarps * 32, sizeof(AttSmem<D>), st>>>(a);
-    e = cudaGetLastError();
+    cudaError_t e = a.plan.rows == 8 ? attend_nb<DT, D, 1>(a, st) : attend_nb<DT, D, 2>(a, st);
     if (e != cudaSuccess) return e;
     if (a.plan.nz > 1) {
-        const long long rows = a.max_new * a.Hq * kv.seqs;
-        attend_join<DT, D><<<(unsigned) ((rows + 3) / 4), 128, 0, st>>>(a);
+        const unsigned rows = (unsigned) std::min(a.max_new * a.Hq, 65535ll);
+        attend_join<DT, D><<<dim3((unsigned) kv.seqs, rows), 128, 0, st>>>(a);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     if (a.lse) {
         const long long units = (long long) kv.seqs * kv.heads;
         const int nzw = (int) std::max(1ll, std::min<long long>((kv.width + kAttWarps - 1) / kAttWarps, (n_sm * 4 + units - 1) / units));
-        attend_weights<DT, D><<<(unsigned) (units * nzw), kAttWarps * 32, 0, st>>>(a, nzw);
+        attend_weights<DT, D><<<(unsigned) (units * nzw), kAttWarps * 32, (kPage - 1) * D * DtInfo<DT>::ES, st>>>(a, nzw);
         e = cudaGetLastError();
     }
     return e;

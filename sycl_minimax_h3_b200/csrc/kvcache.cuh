@@ -11,6 +11,7 @@ namespace h3 {
 
 constexpr int kPage = 64;              // tokens of a page: the Sage quantiser's block, with one scale per head
 constexpr int kErrPage = 1;            // index errors (the second word of a context's error words): a page id
+constexpr int kErrCache = 64;          // a wait of the attention over the cache gave up (the first error word)
 constexpr int kErrLen = 2;             //   lens or starts out of range
 
 struct KvArgs {
@@ -31,7 +32,8 @@ struct KvArgs {
 
 // How a call's queries and keys are divided (the same on the host and in every kernel of one call).
 struct AttendPlan {
-    int tiles;                         // 16-row query tiles per (sequence, kv head); more are looped over
+    int rows;                          // query rows of a tile: 8 or 16
+    int tiles;                         // tiles per (sequence, kv head); more are looped over
     int nz;                            // splits of the keys
 };
 AttendPlan attend_plan(int n_sm, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len);
@@ -49,6 +51,8 @@ struct AttendArgs {
     long long max_new;
     float scale_log2;                  // log2(e) / sqrt(dim)
     int q_vec;                         // 16-byte loads of q's rows allowed
+    int* wait_err;                     // device error word of waits that gave up
+    unsigned long long wait_ns;        // limit of every wait
 };
 cudaError_t launch_attend(const AttendArgs& a, int n_sm, cudaStream_t st);
 
