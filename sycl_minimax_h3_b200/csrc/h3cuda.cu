@@ -1284,7 +1284,7 @@ int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, co
     if (!check_dt(x_dt) || !check_dt(s_dt) || !check_dt(out_dt)) return kv_fail(who, "unknown element type");
     if (!x || !tiles || !scale || !out) return kv_fail(who, "a null pointer");
     if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
-    if (N > INT32_MAX - 16 || K > INT32_MAX - 64 || M > 65535ll * 8) return kv_fail(who, "too large");
+    if (N > INT32_MAX - 16 || K > (1 << 30) || M > 65535ll * 64) return kv_fail(who, "too large");
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     Int4Args a{};
@@ -1297,7 +1297,7 @@ int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, co
     a.M = M;
     a.N = (int) N;
     a.K = (int) K;
-    a.group = group ? group : (int) ((K + 63) / 64 * 64);
+    a.group_shift = group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 30;
     a.x_dt = x_dt;
     a.s_dt = s_dt;
     a.out_dt = out_dt;
@@ -1312,7 +1312,7 @@ int h3s_int4_pack(void* ctx, const uint8_t* codes, int64_t N, int64_t K, void* t
     if (K % 2 != 0) return kv_fail(who, "the inputs must be even in number: two codes to a byte");
     if (!codes || !tiles) return kv_fail(who, "a null pointer");
     if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
-    if (N > INT32_MAX - 16 || K > INT32_MAX - 64) return kv_fail(who, "too large");
+    if (N > INT32_MAX - 16 || K > (1 << 30)) return kv_fail(who, "too large");
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     const cudaError_t e = launch_int4_pack(codes, N, K, tiles, c.n_sm, c.st);

@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "attn_common.cuh"
 #include "int4lin.cuh"
@@ -25,30 +26,41 @@ namespace {
 
 constexpr int kI4Warps = 8;
 
-template <int DT>
+template <int XT>
 __device__ __forceinline__ void mma_x(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (DT == F16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (XT == F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the same from zero
+template <int XT>
+__device__ __forceinline__ void mma_x0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (XT == F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // a word of codes as an A fragment: code + 1024 (fp16) or + 128 (bf16) in the bits of a number, minus that and 8
-template <int DT>
+template <int XT>
 __device__ __forceinline__ void frag(uint32_t word, uint32_t (&a)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t v = (word >> (4 * j)) & 0x000f000fu;
-        if constexpr (DT == F16) {
-            const uint32_t u = v | 0x64006400u;
+        const uint32_t u = ((word >> (4 * j)) & 0x000f000fu) | (XT == F16 ? 0x64006400u : 0x43004300u);
+        if constexpr (XT == F16) {
             const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6408)));
             a[j] = *reinterpret_cast<const uint32_t*>(&h);
         } else {
-            const uint32_t u = v | 0x43004300u;
             const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
                                              __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
             a[j] = *reinterpret_cast<const uint32_t*>(&h);
@@ -56,51 +68,65 @@ __device__ __forceinline__ void frag(uint32_t word, uint32_t (&a)[4]) {
     }
 }
 
-// 8 inputs of x as B fragments of two steps: TERMS sets of four words
+// 8 inputs of x as they lie in memory: row m (one of x's) from input k on, past the inputs zeros. whole: all of them are
+// there, on 16 bytes.
+template <int DT>
+struct Raw {
+    uint4 u[DT == F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const Int4Args& a, const char* row, int k, bool whole) {
+    Raw<DT> r{};
+    const char* p = row + (size_t) k * DtInfo<DT>::ES;
+    if (whole) {
+        r.u[0] = *reinterpret_cast<const uint4*>(p);
+        if constexpr (DT == F32) r.u[1] = *reinterpret_cast<const uint4*>(p + 16);
+    } else {
+        uint32_t w[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < a.K) {
+                if constexpr (DT == F32) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+                else w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+            }
+        r.u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (DT == F32) r.u[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    return r;
+}
+// ... as B fragments of two steps: TERMS sets of four words
 template <int DT, int TERMS>
-__device__ __forceinline__ void load_x(const Int4Args& a, long long m, int k, uint32_t (&b)[TERMS][4]) {
-#pragma unroll
-    for (int e = 0; e < TERMS; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[e][i] = 0;
-    if (m >= a.M || k >= a.K) return;
-    const size_t at = (size_t) m * a.K + k;
-    const bool whole = k + 8 <= a.K;
+__device__ __forceinline__ void terms(const Raw<DT>& r, uint32_t (&b)[TERMS][4]) {
     if constexpr (DT == F32) {
-        float x[8];
-        if (whole && a.x_vec) {
-            ld16<F32>(reinterpret_cast<const float*>(a.x) + at, x);
-            ld16<F32>(reinterpret_cast<const float*>(a.x) + at + 4, x + 4);
-        } else
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = k + i < a.K ? ld1<F32>(a.x, at + i) : 0.0f;
+        for (int e = 0; e < TERMS; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[e][i] = 0;
+        const uint32_t w[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             // 8 bits at a time from the top, cut off: what is left over is exact. An infinity or a NaN stays in the first.
-            float r = x[i];
-            const bool fin = fabsf(r) <= 3.402823466e38f;
+            float x = __uint_as_float(w[i]);
+            const bool fin = fabsf(x) <= 3.402823466e38f;
 #pragma unroll
             for (int e = 0; e < TERMS; ++e) {
-                uint32_t u = __float_as_uint(r) >> 16;
-                if (!fin && e == 0 && r != r) u = 0x7fc0;
+                uint32_t u = __float_as_uint(x) >> 16;
+                if (!fin && e == 0 && x != x) u = 0x7fc0;
                 b[e][i / 2] |= u << (16 * (i & 1));
-                r = fin ? r - __uint_as_float(u << 16) : 0.0f;
+                x = fin ? x - __uint_as_float(u << 16) : 0.0f;
             }
         }
     } else {
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(a.x) + at;
-        if (whole && a.x_vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            b[0][0] = u.x; b[0][1] = u.y; b[0][2] = u.z; b[0][3] = u.w;
-        } else
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (k + i < a.K) b[0][i / 2] |= (uint32_t) p[i] << (16 * (i & 1));
+        b[0][0] = r.u[0].x; b[0][1] = r.u[0].y; b[0][2] = r.u[0].z; b[0][3] = r.u[0].w;
     }
 }
 
-__device__ __forceinline__ float ld_dt(const void* p, size_t i, int dt) {
-    return dt == F16 ? ld1<F16>(p, i) : dt == BF16 ? ld1<BF16>(p, i) : ld1<F32>(p, i);
+// A scale or zero point as its bits, and what they stand for: apart, so that the load is not waited for where it is made.
+__device__ __forceinline__ uint32_t ld_bits(const void* p, size_t i, int dt) {
+    return dt == F32 ? reinterpret_cast<const uint32_t*>(p)[i] : reinterpret_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float bits_value(uint32_t u, int dt) {
+    return dt == F16 ? __half2float(__ushort_as_half((uint16_t) u)) : __uint_as_float(dt == BF16 ? u << 16 : u);
 }
 __device__ __forceinline__ void st_dt(void* p, size_t i, float x, int dt) {
     if (dt == F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
@@ -108,66 +134,342 @@ __device__ __forceinline__ void st_dt(void* p, size_t i, float x, int dt) {
     else reinterpret_cast<float*>(p)[i] = x;
 }
 
-// 16 outputs x 8 rows of x per CTA; its warps take the 64-input tiles in turn and their sums meet in shared memory.
-template <int DT, bool ZERO>
-__global__ void __launch_bounds__(kI4Warps * 32) int4_rows(const Int4Args a) {
-    constexpr int TERMS = DT == F32 ? 3 : 1;
-    constexpr int XT = DT == F16 ? F16 : BF16;
-    __shared__ float red[kI4Warps][16][8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int nt = (int) blockIdx.x, KT = (a.K + 63) / 64;
-    const long long m0 = (long long) blockIdx.y * 8;
-    const int n0 = nt * 16 + g, n1 = n0 + 8;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const uint4* tiles = a.tiles + (size_t) nt * KT * 32 + lane;
-    const uint32_t ones[4] = {XT == F16 ? 0x3c003c00u : 0x3f803f80u, XT == F16 ? 0x3c003c00u : 0x3f803f80u,
-                              XT == F16 ? 0x3c003c00u : 0x3f803f80u, XT == F16 ? 0x3c003c00u : 0x3f803f80u};
-    for (int kt = warp; kt < KT; kt += kI4Warps) {
-        const uint4 wv = tiles[(size_t) kt * 32];
-        const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
+// Scales and zero points of two outputs for the halves of a 64-input tile (one for both where a group has more than 32
+// inputs), as bits. An output past the last reads the last one's: its sums are not stored.
+template <bool ZERO, bool G32>
+struct Scales {
+    uint32_t s[G32 ? 2 : 1][2];
+    uint32_t z[ZERO ? (G32 ? 2 : 1) : 1][2];
+};
+template <bool ZERO, bool G32>
+__device__ __forceinline__ void load_scales(const Int4Args& a, int kt, int n0, int n1, Scales<ZERO, G32>& sc) {
+    const size_t i = (size_t) ((kt * 64) >> a.group_shift) * a.N;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int k0 = kt * 64 + half * 32;
-            if (k0 >= a.K) break;
-            uint32_t b[TERMS][4];
-            load_x<DT, TERMS>(a, m0 + g, k0 + 8 * t, b);
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sx[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                uint32_t f[4];
-                frag<XT>(w[half * 2 + u], f);
-#pragma unroll
-                for (int e = 0; e < TERMS; ++e) {
-                    mma_x<XT>(c, f, b[e][2 * u], b[e][2 * u + 1]);
-                    if constexpr (ZERO) mma_x<XT>(sx, ones, b[e][2 * u], b[e][2 * u + 1]);
-                }
-            }
-            const size_t gi = (size_t) (k0 / a.group) * a.N;
-            const float s0 = n0 < a.N ? ld_dt(a.scale, gi + n0, a.s_dt) : 0.0f;
-            const float s1 = n1 < a.N ? ld_dt(a.scale, gi + n1, a.s_dt) : 0.0f;
-            if constexpr (ZERO) {
-                const float z0 = n0 < a.N ? ld_dt(a.zero, gi + n0, a.s_dt) - 8.0f : 0.0f;
-                const float z1 = n1 < a.N ? ld_dt(a.zero, gi + n1, a.s_dt) - 8.0f : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) c[i] = fmaf(-(i < 2 ? z0 : z1), sx[i], c[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(i < 2 ? s0 : s1, c[i], acc[i]);
+    for (int half = 0; half < (G32 ? 2 : 1); ++half) {
+        if (half == 1 && kt * 64 + 32 >= a.K) break;
+        const size_t at = i + (half ? a.N : 0);
+        sc.s[half][0] = ld_bits(a.scale, at + n0, a.s_dt);
+        sc.s[half][1] = ld_bits(a.scale, at + n1, a.s_dt);
+        if constexpr (ZERO) {
+            sc.z[half][0] = ld_bits(a.zero, at + n0, a.s_dt);
+            sc.z[half][1] = ld_bits(a.zero, at + n1, a.s_dt);
         }
     }
+}
+
+// ---- up to 8 rows ----------------------------------------------------------------------------------------------------
+// RT strips of 16 outputs per CTA; its 8 warps take the 64-input tiles in turn, each with the loads of the next one under
+// way, and their sums meet in shared memory.
+template <int DT, int SDT, bool ZERO, bool G32, int RT>
+__global__ void __launch_bounds__(kI4Warps * 32, DT == F32 ? 2 : 3) int4_few(const __grid_constant__ Int4Args a) {
+    constexpr int TERMS = DT == F32 ? 3 : 1, ES = DtInfo<DT>::ES, SES = DtInfo<SDT>::ES, NS = G32 ? 2 : 1;
+    constexpr int XT = DT == F16 ? F16 : BF16;
+    __shared__ float red[kI4Warps][16 * RT][8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int KT = (a.K + 63) / 64, strips = (a.N + 15) / 16;
+    float acc[RT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[warp][g + 8 * (i >> 1)][2 * t + (i & 1)] = acc[i];
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[r][i] = 0.0f;
+    // what this lane reads of tile kt = warp: codes, x, scales, zero points; each moves on by as much for every 8 tiles.
+    // A strip, an output or a row past the last repeats it, and is not stored.
+    const uint4* tp[RT];
+    int ns[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        tp[r] = a.tiles + ((size_t) min((int) blockIdx.x * RT + r, strips - 1) * KT + warp) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ns[r][i] = min((int) (blockIdx.x * RT + r) * 16 + g + 8 * i, a.N - 1) * SES;
+    }
+    const char* row = static_cast<const char*>(a.x) + (size_t) min((int) a.M - 1, g) * a.K * ES;
+    const char* xp = row + (warp * 64 + 8 * t) * ES;
+    const size_t grow = (size_t) a.N * SES;                // a group's scales
+    size_t sp = (size_t) ((warp * 64) >> a.group_shift) * grow;
+    const size_t sstep = (size_t) ((kI4Warps * 64) >> a.group_shift) * grow;
+    const int whole = a.x_vec ? a.K / 64 : 0;              // tiles whose inputs are all there, on 16 bytes
+    constexpr uint32_t one = XT == F16 ? 0x3c003c00u : 0x3f803f80u;
+    const uint32_t ones[4] = {one, one, one, one};
+    struct Stage {
+        uint4 w[RT];
+        Raw<DT> x[2];
+        uint32_t s[RT][NS][2], z[ZERO ? RT : 1][NS][2];
+    } st[2] = {};
+    auto bits = [](const char* p) -> uint32_t {
+        if constexpr (SDT == F32) return *reinterpret_cast<const uint32_t*>(p);
+        else return *reinterpret_cast<const uint16_t*>(p);
+    };
+    auto value = [](uint32_t u) { return bits_value(u, SDT); };
+    auto load = [&](int kt, Stage& s) {
+        if (kt >= KT) return;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            s.w[r] = __ldcs(tp[r]);
+            tp[r] += kI4Warps * 32;
+        }
+        // an odd last half of 32 inputs has no second group: its scales are read again (x is zero there)
+        const size_t next = G32 && kt * 64 + 32 < a.K ? grow : 0;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int h = 0; h < NS; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    s.s[r][h][i] = bits(static_cast<const char*>(a.scale) + sp + (h ? next : 0) + ns[r][i]);
+                    if constexpr (ZERO) s.z[r][h][i] = bits(static_cast<const char*>(a.zero) + sp + (h ? next : 0) + ns[r][i]);
+                }
+        sp += sstep;
+        if (kt < whole) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s.x[h].u[0] = *reinterpret_cast<const uint4*>(xp + 32 * h * ES);
+                if constexpr (DT == F32) s.x[h].u[1] = *reinterpret_cast<const uint4*>(xp + 32 * h * ES + 16);
+            }
+        } else {
+            s.x[0] = load_raw<DT>(a, row, kt * 64 + 8 * t, false);
+            s.x[1] = load_raw<DT>(a, row, kt * 64 + 32 + 8 * t, false);
+        }
+        xp += kI4Warps * 64 * ES;
+    };
+    auto add = [&](const Stage& s) {
+        uint32_t b[2][TERMS][4];
+        terms<DT, TERMS>(s.x[0], b[0]);
+        terms<DT, TERMS>(s.x[1], b[1]);
+        float sx[2][4];
+        if constexpr (ZERO) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < TERMS; ++e) {
+                    if (e == 0 && (G32 || h == 0)) mma_x0<XT>(sx[h], ones, b[h][e][0], b[h][e][1]);
+                    else mma_x<XT>(sx[G32 ? h : 0], ones, b[h][e][0], b[h][e][1]);
+                    mma_x<XT>(sx[G32 ? h : 0], ones, b[h][e][2], b[h][e][3]);
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const uint32_t w[4] = {s.w[r].x, s.w[r].y, s.w[r].z, s.w[r].w};
+            float c[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t f[4];
+                    frag<XT>(w[h * 2 + u], f);
+#pragma unroll
+                    for (int e = 0; e < TERMS; ++e) {
+                        if (u == 0 && e == 0 && (G32 || h == 0)) mma_x0<XT>(c, f, b[h][e][2 * u], b[h][e][2 * u + 1]);
+                        else mma_x<XT>(c, f, b[h][e][2 * u], b[h][e][2 * u + 1]);
+                    }
+                }
+                if (!G32 && h == 0) continue;
+                const int sh = G32 ? h : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (ZERO) c[i] = fmaf(8.0f - value(s.z[r][sh][i >> 1]), sx[sh][i], c[i]);
+                    acc[r][i] = fmaf(value(s.s[r][sh][i >> 1]), c[i], acc[r][i]);
+                }
+            }
+        }
+    };
+    load(warp, st[0]);
+    for (int kt = warp; kt < KT; kt += 2 * kI4Warps) {
+        load(kt + kI4Warps, st[1]);
+        add(st[0]);
+        if (kt + kI4Warps >= KT) break;
+        load(kt + 2 * kI4Warps, st[0]);
+        add(st[1]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[warp][r * 16 + g + 8 * (i >> 1)][2 * t + (i & 1)] = acc[r][i];
     __syncthreads();
-    if (threadIdx.x < 128) {
-        const int n = nt * 16 + (int) (threadIdx.x & 15), col = threadIdx.x >> 4;
-        const long long m = m0 + col;
+    if (threadIdx.x < 128 * RT) {
+        const int c = threadIdx.x % (16 * RT), n = (int) blockIdx.x * 16 * RT + c, m = threadIdx.x / (16 * RT);
         if (n < a.N && m < a.M) {
             float y = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kI4Warps; ++w) y += red[w][threadIdx.x & 15][col];
+            for (int w = 0; w < kI4Warps; ++w) y += red[w][c][m];
             if (a.bias) y += a.bias[n];
             st_dt(a.out, (size_t) m * a.N + n, y, a.out_dt);
         }
+    }
+}
+
+// ---- more rows -------------------------------------------------------------------------------------------------------
+// 128 outputs x up to 64 rows per CTA: a warp has 16 outputs and every row, so that a tile is unpacked once for all of
+// them; x comes through a ring in shared memory, 128 inputs at a time, of which warps 0-7 take the first 64 and warps
+// 8-15 the others. A cluster of `split` CTAs divides the inputs. The sums meet in shared memory, always in one order.
+constexpr int kRowsN = 128, kRowsM = 64, kRowsThreads = 512;
+
+template <int TERMS>
+struct RowsSmem {
+    static constexpr int STAGES = TERMS == 1 ? 4 : 3;
+    union {
+        // [row][16-byte piece of 8 inputs]: odd rows have the halves of every 64 exchanged, so that the 8 lanes that read
+        // together (two rows, four pieces) meet different banks
+        uint4 x[STAGES][TERMS][kRowsM][16];
+        float part[2 * kRowsM * kRowsN];                   // [source][row][output]
+    };
+};
+
+template <int DT, bool ZERO, bool G32, int MT>
+__global__ void __launch_bounds__(kRowsThreads) int4_rows(const __grid_constant__ Int4Args a, int split) {
+    constexpr int TERMS = DT == F32 ? 3 : 1;
+    constexpr int XT = DT == F16 ? F16 : BF16;
+    constexpr int ROWS = 8 * MT, STAGES = RowsSmem<TERMS>::STAGES, AHEAD = 3;
+    constexpr int PIECES = (ROWS * 16 + kRowsThreads - 1) / kRowsThreads;
+    constexpr uint32_t one = XT == F16 ? 0x3c003c00u : 0x3f803f80u;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    RowsSmem<TERMS>& sm = *reinterpret_cast<RowsSmem<TERMS>*>(smem_raw);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, wg = warp >> 3;
+    const int part = (int) (blockIdx.x % split), KT = (a.K + 63) / 64, KP = (KT + 1) / 2;
+    const int per = (KP + split - 1) / split, kp0 = min(KP, part * per), kp1 = min(KP, kp0 + per);
+    const int block = (int) (blockIdx.x / split), strips = (a.N + 15) / 16;
+    const int nt = min(block * (kRowsN / 16) + (warp & 7), strips - 1);    // a strip past the last repeats it, unstored
+    const int n0 = min(nt * 16 + g, a.N - 1), n1 = min(nt * 16 + g + 8, a.N - 1);
+    const long long m0 = (long long) blockIdx.y * ROWS;
+    const uint4* tiles = a.tiles + (size_t) nt * KT * 32 + lane;
+    const uint32_t ones[4] = {one, one, one, one};
+    float acc[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[i][u] = 0.0f;
+    // this thread's pieces of a stage: row and first input, where they lie and where they go
+    const char* src[PIECES];
+    int kc[PIECES], dst[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        const int i = threadIdx.x + j * kRowsThreads, r = i >> 4, c = i & 15;
+        const long long m = min(m0 + r, a.M - 1);
+        src[j] = static_cast<const char*>(a.x) + (size_t) m * a.K * DtInfo<DT>::ES;
+        kc[j] = r < ROWS ? c * 8 : 1 << 30;                // no such piece: never inside
+        dst[j] = r * 16 + (c ^ (4 * (r & 1)));
+    }
+    auto stage = [&](int kp, int slot) {                   // inputs 128 kp .. of x into a slot
+        if (kp < kp1) {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                const int k = kp * 128 + kc[j];
+                if (kc[j] > 128) continue;
+                uint4* to = &sm.x[slot][0][0][0] + dst[j];
+                if (DT != F32 && a.x_vec) {                // K is a multiple of 8: a piece is inside or outside
+                    const uint32_t bytes = k < a.K ? 16 : 0;
+                    const char* from = bytes ? src[j] + (size_t) k * 2 : src[j];
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
+                } else {
+                    uint32_t b[TERMS][4];
+                    terms<DT, TERMS>(load_raw<DT>(a, src[j], k, a.x_vec && k + 8 <= a.K), b);
+#pragma unroll
+                    for (int e = 0; e < TERMS; ++e) to[e * kRowsM * 16] = make_uint4(b[e][0], b[e][1], b[e][2], b[e][3]);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    uint4 w[AHEAD];
+    Scales<ZERO, G32> sc[AHEAD] = {};
+    auto fetch = [&](int kp, int u) {
+        const int kt = min(2 * kp + wg, KT - 1);           // past the last tile x is zeros
+        if (kp < kp1) {
+            w[u] = __ldcs(tiles + kt * 32);
+            load_scales<ZERO, G32>(a, kt, n0, n1, sc[u]);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) stage(kp0 + i, i);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) fetch(kp0 + u, u);
+    int slot = 0;
+    for (int base = kp0; base < kp1; base += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int kp = base + u;
+            if (kp >= kp1) break;
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncthreads();                               // this stage is here, and nobody reads the one before any more
+            stage(kp + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+            const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            float sv[G32 ? 2 : 1][2], zv[G32 ? 2 : 1][2];
+#pragma unroll
+            for (int i = 0; i < (G32 ? 2 : 1); ++i)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    sv[i][r] = bits_value(sc[u].s[i][r], a.s_dt);
+                    zv[i][r] = ZERO ? 8.0f - bits_value(sc[u].z[ZERO ? i : 0][r], a.s_dt) : 0.0f;
+                }
+            const uint4* xs = &sm.x[slot][0][0][0] + g * 16 + wg * 8 + t;
+            float c[MT][4], sx[ZERO ? MT : 1][4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int piece = 4 * (half ^ (g & 1));
+                uint32_t f[2][4];
+                frag<XT>(words[half * 2], f[0]);
+                frag<XT>(words[half * 2 + 1], f[1]);
+#pragma unroll
+                for (int e = 0; e < TERMS; ++e) {
+                    uint4 b[MT];                           // the rows' products side by side: MT sums that do not wait
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) b[i] = xs[e * kRowsM * 16 + i * 128 + piece];
+                    const bool first = e == 0 && (G32 || half == 0);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        if (first) mma_x0<XT>(c[i], f[0], b[i].x, b[i].y);
+                        else mma_x<XT>(c[i], f[0], b[i].x, b[i].y);
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) mma_x<XT>(c[i], f[1], b[i].z, b[i].w);
+                    if constexpr (ZERO) {
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            if (first) mma_x0<XT>(sx[i], ones, b[i].x, b[i].y);
+                            else mma_x<XT>(sx[i], ones, b[i].x, b[i].y);
+                        }
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) mma_x<XT>(sx[i], ones, b[i].z, b[i].w);
+                    }
+                }
+                if (!G32 && half == 0) continue;
+                const int sh = G32 ? half : 0;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if constexpr (ZERO) c[i][q] = fmaf(zv[sh][q >> 1], sx[i][q], c[i][q]);
+                        acc[i][q] = fmaf(sv[sh][q >> 1], c[i][q], acc[i][q]);
+                    }
+            }
+            fetch(kp + AHEAD, u);
+            slot = slot == STAGES - 1 ? 0 : slot + 1;
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    // x is no longer read, in any CTA of the cluster: its memory takes the sums. CTA p finishes the rows p, p + split, ...;
+    // every warp group of every CTA has a place there of its own, [source][row / split][output].
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    const int rows = ROWS / split, source = part * 2 + wg, col = (warp & 7) * 16 + g;
+    const uint32_t mine = smem_u32(&sm.part[0]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = 8 * i + 2 * t + (q & 1);
+            const uint32_t at = mine + (uint32_t) ((source * rows + r / split) * kRowsN + col + 8 * (q >> 1)) * 4;
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(at, (uint32_t) (r % split))), "f"(acc[i][q]) : "memory");
+        }
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    for (int i = threadIdx.x; i < rows * kRowsN; i += kRowsThreads) {
+        const int c = i % kRowsN, r = i / kRowsN, n = block * kRowsN + c;
+        const long long m = m0 + r * split + part;
+        if (n >= a.N || m >= a.M) continue;
+        float y = 0.0f;
+        for (int p = 0; p < 2 * split; ++p) y += sm.part[(p * rows + r) * kRowsN + c];
+        if (a.bias) y += a.bias[n];
+        st_dt(a.out, (size_t) m * a.N + n, y, a.out_dt);
     }
 }
 
@@ -194,19 +496,72 @@ __global__ void int4_pack(const uint8_t* __restrict__ codes, long long N, long l
 
 }  // namespace
 
-template <int DT>
-cudaError_t int4_dt(const Int4Args& a, cudaStream_t st) {
-    const dim3 grid((unsigned) ((a.N + 15) / 16), (unsigned) ((a.M + 7) / 8));
-    if (a.zero) int4_rows<DT, true><<<grid, kI4Warps * 32, 0, st>>>(a);
-    else int4_rows<DT, false><<<grid, kI4Warps * 32, 0, st>>>(a);
+template <int DT, bool ZERO, bool G32, int MT>
+cudaError_t rows_mt(const Int4Args& a, int n_sm, cudaStream_t st) {
+    constexpr int TERMS = DT == F32 ? 3 : 1;
+    static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(int4_rows<DT, ZERO, G32, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) sizeof(RowsSmem<TERMS>));
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    const int blocks = (a.N + kRowsN - 1) / kRowsN, KP = (a.K + 127) / 128;
+    const long long chunks = (a.M + 8 * MT - 1) / (8 * MT);
+    // as many CTAs as there are SMs, or half again as many; a part of the inputs has at least two stages
+    int split = 1;
+    while (split < 8 && blocks * chunks * split * 2 <= n_sm + n_sm / 2 && KP / (split * 2) >= 2) split *= 2;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned) (blocks * split), (unsigned) chunks);
+    c.blockDim = dim3(kRowsThreads);
+    c.dynamicSmemBytes = sizeof(RowsSmem<TERMS>);
+    c.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned) split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, int4_rows<DT, ZERO, G32, MT>, a, split);
+}
+
+template <int DT, int SDT, bool ZERO, bool G32>
+cudaError_t few_s(const Int4Args& a, int n_sm, cudaStream_t st) {
+    const int strips = (a.N + 15) / 16;
+    if (strips >= 4 * n_sm) int4_few<DT, SDT, ZERO, G32, 2><<<(unsigned) ((strips + 1) / 2), kI4Warps * 32, 0, st>>>(a);
+    else int4_few<DT, SDT, ZERO, G32, 1><<<(unsigned) strips, kI4Warps * 32, 0, st>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t launch_int4_linear(const Int4Args& a, int, cudaStream_t st) {
+template <int DT, bool ZERO, bool G32>
+cudaError_t int4_dt(const Int4Args& a, int n_sm, cudaStream_t st) {
+    if (a.M <= 8) {
+        switch (a.s_dt) {
+            case F16: return few_s<DT, F16, ZERO, G32>(a, n_sm, st);
+            case BF16: return few_s<DT, BF16, ZERO, G32>(a, n_sm, st);
+            default: return few_s<DT, F32, ZERO, G32>(a, n_sm, st);
+        }
+    }
+    if (a.M <= 16) return rows_mt<DT, ZERO, G32, 2>(a, n_sm, st);
+    if (a.M <= 32) return rows_mt<DT, ZERO, G32, 4>(a, n_sm, st);
+    if (a.M <= 48) return rows_mt<DT, ZERO, G32, 6>(a, n_sm, st);
+    return rows_mt<DT, ZERO, G32, 8>(a, n_sm, st);
+}
+
+template <int DT>
+cudaError_t int4_type(const Int4Args& a, int n_sm, cudaStream_t st) {
+    if (a.group_shift == 5) return a.zero ? int4_dt<DT, true, true>(a, n_sm, st) : int4_dt<DT, false, true>(a, n_sm, st);
+    return a.zero ? int4_dt<DT, true, false>(a, n_sm, st) : int4_dt<DT, false, false>(a, n_sm, st);
+}
+
+cudaError_t launch_int4_linear(const Int4Args& a, int n_sm, cudaStream_t st) {
     switch (a.x_dt) {
-        case F16: return int4_dt<F16>(a, st);
-        case BF16: return int4_dt<BF16>(a, st);
-        default: return int4_dt<F32>(a, st);
+        case F16: return int4_type<F16>(a, n_sm, st);
+        case BF16: return int4_type<BF16>(a, n_sm, st);
+        default: return int4_type<F32>(a, n_sm, st);
     }
 }
 

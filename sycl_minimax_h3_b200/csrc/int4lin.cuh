@@ -17,7 +17,7 @@ struct Int4Args {
     const float* bias;                 // [N] or NULL
     void* out;                         // [M, N] in out_dt
     long long M;
-    int N, K, group;                   // group: 32, 64, 128, or K rounded up to 64 (one scale for each output)
+    int N, K, group_shift;             // groups of 2^group_shift inputs: 5 to 7, or 30 (one scale for each output)
     int x_dt, s_dt, out_dt;
     int x_vec;                         // 16-byte loads of x's rows allowed
 };
