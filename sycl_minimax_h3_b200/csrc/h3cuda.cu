@@ -525,7 +525,7 @@ int check_kv(const char* who, const h3s_kv_cache* kv, bool weights, KvArgs& a) {
     if (!kv) return kv_fail(who, "no cache");
     if (!check_dt(kv->dt)) return kv_fail(who, "unknown element type " + std::to_string(kv->dt));
     if (kv->dim != 64 && kv->dim != 128) return kv_fail(who, "heads of 64 or 128 features (got " + std::to_string(kv->dim) + ")");
-    if (kv->pages < 0 || kv->seqs < 1 || kv->width < 0 || kv->heads < 1 || kv->pages > INT32_MAX || kv->seqs > INT32_MAX ||
+    if (kv->pages < 0 || kv->seqs < 1 || kv->width < 0 || kv->heads < 1 || kv->pages > INT32_MAX / kPage || kv->seqs > INT32_MAX ||
         kv->heads > INT32_MAX || kv->width >= (1 << 25) || kv->seqs > INT32_MAX / kv->heads)
         return kv_fail(who, "the cache's sizes are out of range");
     if ((kv->pages > 0 && (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale)) || !kv->tail_k || !kv->tail_v ||
@@ -1184,10 +1184,6 @@ int h3s_kv_append(void* ctx, const h3s_kv_cache* kv, const void* k, const void* 
     if (stride < kv->heads * kv->dim) return kv_fail(who, "the row stride is shorter than a row");
     if (T > INT32_MAX) return kv_fail(who, "too many rows");
     if (max_new <= 0 || max_new > T) max_new = T;
-    // the blocks of the longest sequence, as far as the grid goes; a CTA takes more of them where that is not all
-    const int64_t most = INT32_MAX / 2 / (kv->heads * kv->seqs);
-    if (most < 1) return kv_fail(who, "too many sequences and heads");
-    max_new = std::min(max_new, most * kPage);
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     a.err = c.err + 1;
@@ -1267,7 +1263,7 @@ int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budg
     const uint64_t need = (uint64_t) (kv->seqs * kv->heads) * budget * 4;
     if (!work || work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 3))
         return kv_fail(who, "work of " + std::to_string(need) + " bytes needed, " + std::to_string(work ? work_bytes : 0) + " given");
-    if (kv->seqs * kv->heads > INT32_MAX / 2 / (budget / kPage)) return kv_fail(who, "too many sequences, heads and pages for one call");
+    if (budget / kPage > 65535) return kv_fail(who, "the budget is out of range");
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     a.err = c.err + 1;

@@ -50,25 +50,72 @@ __device__ __forceinline__ void ld8(const void* p, size_t i, bool vec, float* x)
     }
 }
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
-
-// The code of x in a block whose largest magnitude is a > 0: 127 x / a rounded to the nearest whole number, half way to
-// even, as if the ratio were exact. x and a of 16-bit types have at most 11 bits: 127 x has 18, and where 127 x / a is
-// not exactly half way it is at least 2^4 roundings of a float away from it, so one float division decides right.
-// Where x and a have 24 bits or more, a ratio within 1e-4 of half way is taken again in 64 bits.
-// num = 127 and den = a, both times 2^-8 where 127 a could overflow.
-template <bool WIDE>
-__device__ __forceinline__ int code_of(float x, float num, float den, double exact_x, double exact_a) {
-    const float r = __fdiv_rn(x * num, den);
-    float n = rintf(r);
-    if constexpr (WIDE) {
-        if (fabsf(fabsf(r - n) - 0.5f) < 1e-4f) n = (float) rint(exact_x * 127.0 / exact_a);
+// 8 values as they lie in memory, and as floats
+template <int DT>
+struct Raw8 {
+    uint4 u[DT == F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> raw8(const void* p, size_t i, bool vec) {
+    Raw8<DT> r;
+    const char* c = reinterpret_cast<const char*>(p) + i * DtInfo<DT>::ES;
+    if (vec) {
+        r.u[0] = *reinterpret_cast<const uint4*>(c);
+        if constexpr (DT == F32) r.u[1] = *reinterpret_cast<const uint4*>(c + 16);
+    } else {
+        uint32_t w[8] = {};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if constexpr (DT == F32) w[u] = reinterpret_cast<const uint32_t*>(c)[u];
+            else w[u / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(c)[u] << (16 * (u & 1));
+        }
+        r.u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (DT == F32) r.u[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
-    return (int) fminf(fmaxf(n, -127.0f), 127.0f);
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void floats8(const Raw8<DT>& r, float (&x)[8]) {
+    cvt16<DT>(r.u[0], x);
+    if constexpr (DT == F32) cvt16<DT>(r.u[1], x + 4);
 }
 
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (uint32_t) (a & 255) | (uint32_t) (b & 255) << 8 | (uint32_t) (c & 255) << 16 | (uint32_t) d << 24;
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// The codes of eight values x times sc in a block whose largest magnitude is top > 0: 127 x sc / top rounded to the nearest
+// whole number, half way to even, as if the ratio were exact. ratio = 127 sc / top as a float is off by 2^-23 of itself at
+// most, so x * ratio by less than 4e-5: where it lies within 1e-4 of half way between two codes, the ratio is taken
+// again in 64 bits, which hold x sc 127 exactly (24 + 24 + 7 bits at most where x is a float and sc = 1, or x a code).
+// Adding 1.5 2^23 rounds to a whole number in the low bits. odd: x may hold infinities (+-127) and NaN (0).
+// The long way is a call of its own: inlined, its registers would halve the CTAs of an SM for one chunk in a few hundred.
+__device__ __noinline__ uint2 codes8_long(float4 lo, float4 hi, double sc, double top) {
+    const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    uint32_t o[2] = {0, 0};
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        int q = 0;
+        if (!finite(x[u])) q = x[u] > 0.0f ? 127 : x[u] < 0.0f ? -127 : 0;
+        else q = (int) fmin(fmax(rint((double) x[u] * sc * 127.0 / top), -127.0), 127.0);
+        o[u / 4] |= (uint32_t) (q & 255) << (8 * (u % 4));
+    }
+    return make_uint2(o[0], o[1]);
+}
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float ratio, double sc, double top, bool odd) {
+    constexpr float kRound = 12582912.0f;
+    int q[8];
+    float far = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const float n = fmaf(x[u], ratio, kRound);
+        q[u] = __float_as_int(n);
+        far = fmaxf(far, fabsf(fmaf(x[u], ratio, kRound - n)));
+    }
+    if (odd || far > 0.4999f)
+        return codes8_long(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), sc, top);
+    uint2 o;
+    o.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    o.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+    return o;
 }
 
 template <typename T>
@@ -89,25 +136,22 @@ __device__ __forceinline__ T block_max(T x, T* red) {     // over 256 threads; e
 
 // ---- writing ---------------------------------------------------------------------------------------------------------
 // A block of 64 slots that is full becomes a page: a = max|x| over its 64 x D values of a head, scale = a / 127, codes as
-// code_of. What does not fill a block stays in the tail in its own type, so a token is rounded once, when its block is
+// codes8. What does not fill a block stays in the tail in its own type, so a token is rounded once, when its block is
 // full, and the cache does not depend on how the tokens were spread over calls. Infinities take the code +-127 and NaN 0;
 // neither counts for a.
-// One CTA per (sequence, head, block, K or V). The CTA of the sequence's first block reads the old tail and, after that,
-// writes the new one: the two share slots.
+// One CTA per (sequence, head), block, and K or V. The CTA of the sequence's first block reads the old tail and, after
+// that, writes the new one: the two share slots.
 constexpr int kAppThreads = 256;
 
 template <int DT, int D>
-__global__ void __launch_bounds__(kAppThreads) kv_append(const KvArgs kv, const void* __restrict__ krows,
+__global__ void __launch_bounds__(kAppThreads, DT == F32 ? 3 : 4) kv_append(const __grid_constant__ KvArgs kv, const void* __restrict__ krows,
                                                          const void* __restrict__ vrows, long long T, long long stride,
-                                                         const int* __restrict__ starts, int J, int vec) {
+                                                         const int* __restrict__ starts, int vec) {
     constexpr int C8 = D / 8;                              // 8-value chunks of a row
     constexpr int PER = 64 * C8 / kAppThreads;
     __shared__ float red[8];
-    const long long unit = blockIdx.x;
-    const int which = (int) (unit & 1);
-    const int j = (int) ((unit >> 1) % J);
-    const int h = (int) ((unit >> 1) / J % kv.heads);
-    const int b = (int) ((unit >> 1) / J / kv.heads);
+    const int j = blockIdx.y, J = gridDim.y, which = blockIdx.z;
+    const int b = (int) (blockIdx.x / kv.heads), h = (int) (blockIdx.x % kv.heads);
     const Seq s = load_seq(kv, starts, T, b);
     if (!s.ok || s.L < s.n) {
         if (threadIdx.x == 0) atomicOr(kv.err, kErrLen);
@@ -122,40 +166,53 @@ __global__ void __launch_bounds__(kAppThreads) kv_append(const KvArgs kv, const 
     for (int blk = first + j; blk < full; blk += J) {
         const int page = kv.table[(size_t) b * kv.width + blk];
         const bool ok = page_ok(kv, page);
+        Raw8<DT> raw[PER];
+        float top = 0.0f, odd = 0.0f;                      // odd: NaN once a value is infinite or NaN
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * kAppThreads, r = c / C8, d = c % C8 * 8, slot = blk * kPage + r;
+            if (slot < L0) raw[i] = raw8<DT>(tail, (tbase + r) * D + d, true);
+            else raw[i] = raw8<DT>(rows, row(slot) + d, vec);
+        }
         if (!ok) {
             if (threadIdx.x == 0) atomicOr(kv.err, kErrPage);
             continue;
         }
-        float x[PER][8];
-        float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int c = threadIdx.x + i * kAppThreads, r = c / C8, d = c % C8 * 8, slot = blk * kPage + r;
-            if (slot < L0) ld8<DT>(tail, (tbase + r) * D + d, true, x[i]);
-            else ld8<DT>(rows, row(slot) + d, vec, x[i]);
+            float x[8];
+            floats8(raw[i], x);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (finite(x[i][u])) top = fmaxf(top, fabsf(x[i][u]));
+            for (int u = 0; u < 8; ++u) {
+                top = fmaxf(top, fabsf(x[u]));
+                odd = fmaf(x[u], 0.0f, odd);
+            }
+        }
+        const bool any_odd = __syncthreads_or(odd != 0.0f);
+        if (any_odd) {
+            top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                float x[8];
+                floats8(raw[i], x);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (finite(x[u])) top = fmaxf(top, fabsf(x[u]));
+            }
         }
         top = block_max(top, red);
         const size_t pbase = (size_t) page * kv.heads + h;
         if (threadIdx.x == 0) (which ? kv.vs : kv.ks)[pbase] = __fdiv_rn(top, 127.0f);
-        const bool big = top > 1e36f;
-        const float num = big ? 127.0f / 256.0f : 127.0f, den = big ? top / 256.0f : top;
+        // a largest value below 2^-100 has no float 127 / a: every code goes the long way
+        const bool small = top < 7.9e-31f;
+        const float ratio = small ? 0.0f : __fdiv_rn(127.0f, top);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = threadIdx.x + i * kAppThreads, r = c / C8, d = c % C8 * 8;
-            int q[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float y = x[i][u];
-                if (top == 0.0f || y != y) q[u] = 0;
-                else if (!finite(y)) q[u] = y > 0.0f ? 127 : -127;
-                else q[u] = code_of<DT == F32>(y, num, den, (double) y, (double) top);
-            }
-            uint2 o;
-            o.x = pack4(q[0], q[1], q[2], q[3]);
-            o.y = pack4(q[4], q[5], q[6], q[7]);
+            uint2 o = make_uint2(0, 0);
+            float x[8];
+            floats8(raw[i], x);
+            if (top > 0.0f) o = codes8(x, ratio, 1.0, (double) top, any_odd || small);
             *reinterpret_cast<uint2*>((which ? kv.v : kv.k) + (pbase * kPage + r) * D + d) = o;
         }
         if (kv.tw && which == 0 && threadIdx.x < kPage)
@@ -166,10 +223,10 @@ __global__ void __launch_bounds__(kAppThreads) kv_append(const KvArgs kv, const 
     const int from = max(L0, full * kPage);
     for (int c = threadIdx.x; c < (s.L - from) * C8; c += kAppThreads) {
         const int slot = from + c / C8, d = c % C8 * 8;
-        float x[8];
-        ld8<DT>(rows, row(slot) + d, vec, x);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) st1<DT>(tail, (tbase + slot % kPage) * D + d + u, x[u]);
+        const Raw8<DT> x = raw8<DT>(rows, row(slot) + d, vec);
+        uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(tail) + ((tbase + slot % kPage) * D + d) * DtInfo<DT>::ES);
+        to[0] = x.u[0];
+        if constexpr (DT == F32) to[1] = x.u[1];
     }
     if (kv.tw && which == 0)
         for (int slot = from + threadIdx.x; slot < s.L; slot += kAppThreads) kv.tw[tbase + slot % kPage] = 0.0f;
@@ -913,16 +970,21 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kSelThreads = 1024;
+constexpr int kLeftAlone = INT32_MIN;
+constexpr int kSelKeys = 48 * 1024;    // keys that fit shared memory; those of a longer sequence are read again each time
 
-// kept[seq, head, 0..budget): the kept slots in order; kept[..][0] = -1 where the sequence is left alone. One CTA per
-// (sequence, head): the weight of the last kept one among equals by four passes over 8 bits of the keys each, then one
-// pass that writes the slots down.
-__global__ void __launch_bounds__(kSelThreads) evict_select(const KvArgs kv, const int* __restrict__ spare, int budget,
-                                                            int sinks, int recent, int* __restrict__ kept) {
+// kept[seq, head, 0..budget): where the kept tokens are, in order: 64 page + place, or -1 - place in the tail;
+// kept[..][0] = kLeftAlone where the sequence is left alone. One CTA per
+// (sequence, head). The weights' keys are read once into shared memory; the key of the last kept one is found by four
+// passes over 8 bits of them each; then every thread counts the kept ones in a run of slots of its own, one scan over
+// the threads gives the places, and the runs are written down.
+__global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ KvArgs kv, const int* __restrict__ spare,
+                                                            int budget, int sinks, int recent, int* __restrict__ kept, int room) {
+    extern __shared__ uint32_t keys[];
     __shared__ int hist[256];
-    __shared__ int wsum[32];
+    __shared__ int ssum[32], esum[32];
     __shared__ uint32_t s_prefix;
-    __shared__ int s_need, s_bad;
+    __shared__ int s_need;
     const int h = (int) (blockIdx.x % kv.heads), b = (int) (blockIdx.x / kv.heads);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int L = kv.lens[b];
@@ -931,37 +993,41 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const KvArgs kv, con
     const int full = L / kPage;
     if (L <= budget || full > kv.width) {
         if (tid == 0) {
-            out[0] = -1;
+            out[0] = kLeftAlone;
             if (L < 0 || full > kv.width) atomicOr(kv.err, kErrLen);
         }
         return;
     }
-    if (tid == 0) s_bad = 0;
-    __syncthreads();
-    for (int i = tid; i < full; i += kSelThreads)
-        if (!page_ok(kv, table[i])) s_bad = 1;
-    for (int i = tid; i < budget / kPage; i += kSelThreads)
-        if (!page_ok(kv, spare[(size_t) b * (budget / kPage) + i])) s_bad = 1;
-    __syncthreads();
-    if (s_bad) {
+    bool bad = false;
+    for (int i = tid; i < full; i += kSelThreads) bad |= !page_ok(kv, table[i]);
+    for (int i = tid; i < budget / kPage; i += kSelThreads) bad |= !page_ok(kv, spare[(size_t) b * (budget / kPage) + i]);
+    if (__syncthreads_or(bad)) {
         if (tid == 0) {
-            out[0] = -1;
+            out[0] = kLeftAlone;
             atomicOr(kv.err, kErrPage);
         }
         return;
     }
-    const int lo = sinks, hi = L - recent;                 // sinks + recent <= budget < L: lo < hi
-    auto key = [&](int slot) {
+    auto read = [&](int slot) {
         const float w = slot < full * kPage ? kv.w[((size_t) table[slot / kPage] * kv.heads + h) * kPage + slot % kPage]
                                             : kv.tw[((size_t) b * kv.heads + h) * kPage + slot - full * kPage];
         return weight_key(w);
     };
+    const bool held = L <= room;
+    if (held) {
+#pragma unroll 4
+        for (int i = tid; i < L; i += kSelThreads) keys[i] = read(i);
+        __syncthreads();
+    }
+    auto key = [&](int slot) { return held ? keys[slot] : read(slot); };
+    const int lo = sinks, hi = L - recent;                 // sinks + recent <= budget < L: lo < hi
     // the need-th largest key of the middle
+    const int middle = budget - sinks - recent;
     uint32_t prefix = 0;
-    int need = budget - sinks - recent;
+    int need = middle;
     if (need > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+            if (tid < 256) hist[tid] = 0;
             __syncthreads();
             for (int i = lo + tid; i < hi; i += kSelThreads) {
                 const uint32_t k = key(i);
@@ -995,146 +1061,153 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const KvArgs kv, con
             __syncthreads();
             prefix = s_prefix;
             need = s_need;
-            __syncthreads();
         }
     }
-    // now `need` of the keys equal to prefix are kept (the first ones), and all larger ones
-    const bool any = budget - sinks - recent > 0;
-    int done = 0, equal = 0;                               // kept so far; equal ones so far
-    for (int base = 0; base < L; base += kSelThreads) {
-        const int i = base + tid;
-        int sure = 0, eq = 0;
-        if (i < L) {
-            if (i < lo || i >= hi) sure = 1;
-            else if (any) {
-                const uint32_t k = key(i);
-                sure = k > prefix;
-                eq = k == prefix;
-            }
+    // now `need` of the keys equal to prefix are kept (the first ones), and all larger ones. A thread's run has an odd
+    // length, so that the threads of a warp read different banks.
+    const int run = ((L + kSelThreads - 1) / kSelThreads) | 1, i0 = min(L, tid * run), i1 = min(L, i0 + run);
+    auto look = [&](int i, bool& sure, bool& equal) {
+        sure = i < lo || i >= hi;
+        equal = false;
+        if (!sure && middle > 0) {
+            const uint32_t k = key(i);
+            sure = k > prefix;
+            equal = k == prefix;
         }
-        // an inclusive scan over the block of both counts, in one word; at most 1,024 of each
-        int both = sure | eq << 16;
+    };
+    int n_sure = 0, n_equal = 0;
+    for (int i = i0; i < i1; ++i) {
+        bool sure, equal;
+        look(i, sure, equal);
+        n_sure += sure;
+        n_equal += equal;
+    }
+    int before_sure = n_sure, before_equal = n_equal;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, both, o);
-            if (lane >= o) both += y;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before_sure, o), y = __shfl_up_sync(0xffffffffu, before_equal, o);
+        if (lane >= o) {
+            before_sure += x;
+            before_equal += y;
         }
-        if (lane == 31) wsum[warp] = both;
-        __syncthreads();
-        if (warp == 0) {
-            int x = wsum[lane];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            wsum[lane] = x;
-        }
-        __syncthreads();
-        if (warp > 0) both += wsum[warp - 1];
-        const int all = wsum[31];
-        const int eq_before = equal + (both >> 16) - eq;   // equal ones before this slot
-        const bool keep = sure || (eq && eq_before < need);
-        const int at = done + (both & 0xffff) - sure + (min(eq_before, need) - min(equal, need));
-        if (keep) out[at] = i;
-        const int eq_all = all >> 16;
-        done += (all & 0xffff) + min(equal + eq_all, need) - min(equal, need);
-        equal += eq_all;
-        __syncthreads();
+    }
+    if (lane == 31) {
+        ssum[warp] = before_sure;
+        esum[warp] = before_equal;
+    }
+    __syncthreads();
+    before_sure -= n_sure;
+    before_equal -= n_equal;
+    for (int w = 0; w < warp; ++w) {
+        before_sure += ssum[w];
+        before_equal += esum[w];
+    }
+    int at = before_sure + min(before_equal, need);
+    for (int i = i0; i < i1; ++i) {
+        bool sure, equal;
+        look(i, sure, equal);
+        if (sure || (equal && before_equal < need)) out[at++] = i < full * kPage ? table[i / kPage] * kPage + i % kPage : full * kPage - 1 - i;
+        before_equal += equal;
     }
 }
 
-// 64 kept tokens of a (sequence, head), K or V, into one spare page
-template <int DT, int D>
-__global__ void __launch_bounds__(256) evict_gather(const KvArgs kv, const int* __restrict__ spare, int budget,
-                                                    const int* __restrict__ kept) {
-    constexpr int C8 = D / 8;
-    constexpr int PER = 64 * C8 / 256;
+// 64 kept tokens of a (sequence, head) into one spare page, K and V side by side so that their loads are under way
+// together. TAIL: some of them lie in the tail (a sequence's last page or two).
+template <int DT, int D, bool TAIL>
+__device__ __forceinline__ void gather_page(const KvArgs& kv, int h, size_t tbase, int page, const int* loc) {
+    constexpr int C8 = D / 8, PER = 64 * C8 / 256;
     __shared__ double red[8];
-    __shared__ int slots[kPage];
-    __shared__ int pages[kPage];
-    const int nb = budget / kPage;
-    long long unit = blockIdx.x;
-    const int which = (int) (unit & 1);
-    unit >>= 1;
-    const int blk = (int) (unit % nb);
-    unit /= nb;
-    const int h = (int) (unit % kv.heads), b = (int) (unit / kv.heads);
-    const int* mine = kept + ((size_t) b * kv.heads + h) * budget;
-    if (mine[0] < 0) return;
-    const int full = kv.lens[b] / kPage;
-    if (threadIdx.x < kPage) {
-        const int slot = mine[blk * kPage + threadIdx.x];
-        slots[threadIdx.x] = slot;
-        pages[threadIdx.x] = slot < full * kPage ? kv.table[(size_t) b * kv.width + slot / kPage] : -1;
+    __shared__ float scale[2][kPage], ratio[2][kPage];
+    if (threadIdx.x < 2 * kPage) {
+        const int which = threadIdx.x / kPage, at = loc[threadIdx.x % kPage];
+        scale[which][threadIdx.x % kPage] = at >= 0 ? (which ? kv.vs : kv.ks)[(size_t) (at / kPage) * kv.heads + h] : 1.0f;
     }
+    struct Chunk {
+        uint2 c;                       // a page's codes
+        Raw8<DT> t[1];                 // or, with TAIL, the tail's values
+    } raw[2][PER];
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * 256, d = c % C8 * 8, at = loc[c / C8];
+            if (!TAIL || at >= 0)
+                raw[which][i].c = *reinterpret_cast<const uint2*>(
+                    (which ? kv.v : kv.k) + (((size_t) (at / kPage) * kv.heads + h) * kPage + at % kPage) * D + d);
+            else if constexpr (TAIL)
+                raw[which][i].t[0] = raw8<DT>(which ? kv.tv : kv.tk, (tbase - 1 - at) * D + d, true);
+        }
+    auto values = [&](int which, int i, float (&x)[8]) {
+        if (!TAIL || loc[(threadIdx.x + i * 256) / C8] >= 0) {
+            const uint32_t w[2] = {raw[which][i].c.x ^ 0x80808080u, raw[which][i].c.y ^ 0x80808080u};
+            // code + 128 in the low bits of 2^23
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(__byte_perm(w[e / 4], 0x4b000000u, 0x7650 | (e % 4))) - 8388736.0f;
+        } else if constexpr (TAIL) {
+            floats8(raw[which][i].t[0], x);
+        }
+    };
     __syncthreads();
-    const int8_t* codes = which ? kv.v : kv.k;
-    const float* scales = which ? kv.vs : kv.ks;
-    const void* tail = which ? kv.tv : kv.tk;
-    const size_t tbase = ((size_t) b * kv.heads + h) * kPage;
-    float x[PER][8];                   // a page's codes, or the tail's values
-    float sc[PER];                     // their scale (1 for the tail)
-    double top = 0.0;
+    const size_t pb = (size_t) page * kv.heads + h;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int c = threadIdx.x + i * 256, r = c / C8, d = c % C8 * 8, page = pages[r], slot = slots[r];
-        if (page >= 0) {
-            const size_t pb = (size_t) page * kv.heads + h;
-            const uint2 u = *reinterpret_cast<const uint2*>(codes + (pb * kPage + slot % kPage) * D + d);
-            sc[i] = scales[pb];
+    for (int which = 0; which < 2; ++which) {
+        double top = 0.0;
+        bool odd = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[i][e] = (float) (int8_t) (u.x >> (8 * e));
-                x[i][4 + e] = (float) (int8_t) (u.y >> (8 * e));
+        for (int i = 0; i < PER; ++i) {
+            float x[8], m = 0.0f;
+            values(which, i, x);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (!TAIL || finite(x[u])) m = fmaxf(m, fabsf(x[u]));
+                else odd = true;
             }
-        } else {
-            ld8<DT>(tail, (tbase + slot - full * kPage) * D + d, true, x[i]);
-            sc[i] = 1.0f;
+            const double v = (double) m * (double) scale[which][(threadIdx.x + i * 256) / C8];   // exact: 24 bits times 24 at most
+            if (v > top) top = v;
         }
-        float m = 0.0f;
+        if (TAIL) odd = __syncthreads_or(odd);
+        top = block_max(top, red);
+        if (threadIdx.x == 0) (which ? kv.vs : kv.ks)[pb] = (float) (top / 127.0);
+        // where a float cannot hold 127 scale / top every code goes the long way
+        const bool far = top < 1e-30;
+        if (threadIdx.x < kPage) ratio[which][threadIdx.x] = far ? 0.0f : (float) ((double) scale[which][threadIdx.x] * 127.0 / top);
+        __syncthreads();
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (finite(x[i][u])) m = fmaxf(m, fabsf(x[i][u]));
-        const double v = (double) m * (double) sc[i];      // exact: 24 bits times 24 at most
-        if (v > top) top = v;
-    }
-    top = block_max(top, red);
-    const size_t pb = (size_t) spare[(size_t) b * nb + blk] * kv.heads + h;
-    if (threadIdx.x == 0) (which ? kv.vs : kv.ks)[pb] = (float) (top / 127.0);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int c = threadIdx.x + i * 256, r = c / C8, d = c % C8 * 8;
-        const double ratio = top > 0.0 ? (double) sc[i] * 127.0 / top : 0.0;
-        int q[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float y = x[i][u];
-            if (top == 0.0 || y != y) q[u] = 0;
-            else if (!finite(y)) q[u] = y > 0.0f ? 127 : -127;
-            else {
-                const double e = (double) y * ratio;
-                double n = rint(e);
-                if (fabs(fabs(e - n) - 0.5) < 1e-6) n = rint((double) y * (double) sc[i] * 127.0 / top);
-                q[u] = (int) fmin(fmax(n, -127.0), 127.0);
-            }
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * 256, r = c / C8, d = c % C8 * 8;
+            uint2 o = make_uint2(0, 0);
+            float x[8];
+            values(which, i, x);
+            if (top > 0.0) o = codes8(x, ratio[which][r], (double) scale[which][r], top, odd || far);
+            *reinterpret_cast<uint2*>((which ? kv.v : kv.k) + (pb * kPage + r) * D + d) = o;
         }
-        uint2 o;
-        o.x = pack4(q[0], q[1], q[2], q[3]);
-        o.y = pack4(q[4], q[5], q[6], q[7]);
-        *reinterpret_cast<uint2*>((which ? kv.v : kv.k) + (pb * kPage + r) * D + d) = o;
     }
-    if (which == 0 && threadIdx.x < kPage) {
-        const int slot = slots[threadIdx.x], page = pages[threadIdx.x];
-        kv.w[pb * kPage + threadIdx.x] =
-            page >= 0 ? kv.w[((size_t) page * kv.heads + h) * kPage + slot % kPage] : kv.tw[tbase + slot - full * kPage];
+    if (threadIdx.x < kPage) {
+        const int at = loc[threadIdx.x];
+        kv.w[pb * kPage + threadIdx.x] = at >= 0 ? kv.w[((size_t) (at / kPage) * kv.heads + h) * kPage + at % kPage] : kv.tw[tbase - 1 - at];
     }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256, 4) evict_gather(const __grid_constant__ KvArgs kv, const int* __restrict__ spare, int budget,
+                                                       const int* __restrict__ kept) {
+    __shared__ int loc[kPage];
+    const int nb = budget / kPage, blk = blockIdx.y;
+    const int b = (int) (blockIdx.x / kv.heads), h = (int) (blockIdx.x % kv.heads);
+    const int* mine = kept + (size_t) blockIdx.x * budget;
+    if (mine[0] == kLeftAlone) return;
+    const int page = spare[(size_t) b * nb + blk];
+    int at = 0;
+    if (threadIdx.x < kPage) loc[threadIdx.x] = at = mine[blk * kPage + threadIdx.x];
+    const size_t tbase = (size_t) blockIdx.x * kPage;
+    if (__syncthreads_or(at < 0)) gather_page<DT, D, true>(kv, h, tbase, page, loc);
+    else gather_page<DT, D, false>(kv, h, tbase, page, loc);
 }
 
 // the new pages take the old ones' place in the table, which take theirs among the spare ones
 __global__ void __launch_bounds__(256) evict_swap(const KvArgs kv, int* __restrict__ spare, int budget, const int* __restrict__ kept) {
     const int b = (int) blockIdx.x, nb = budget / kPage;
-    if (kept[(size_t) b * kv.heads * budget] < 0) return;
+    if (kept[(size_t) b * kv.heads * budget] == kLeftAlone) return;
     for (int i = threadIdx.x; i < nb; i += 256) {
         int* p = kv.table + (size_t) b * kv.width + i;
         int* q = spare + (size_t) b * nb + i;
@@ -1152,10 +1225,9 @@ __global__ void __launch_bounds__(256) evict_swap(const KvArgs kv, int* __restri
 template <int DT>
 cudaError_t append_dt(const KvArgs& kv, const void* k, const void* v, long long T, long long stride, const int* starts,
                       long long max_new, bool vec, cudaStream_t st) {
-    const long long J = std::max(1ll, (max_new + kPage - 1) / kPage);
-    const unsigned grid = (unsigned) (2 * J * kv.heads * kv.seqs);
-    if (kv.dim == 64) kv_append<DT, 64><<<grid, kAppThreads, 0, st>>>(kv, k, v, T, stride, starts, (int) J, vec);
-    else kv_append<DT, 128><<<grid, kAppThreads, 0, st>>>(kv, k, v, T, stride, starts, (int) J, vec);
+    const dim3 grid((unsigned) (kv.seqs * kv.heads), (unsigned) std::min(std::max(1ll, (max_new + kPage - 1) / kPage), 65535ll), 2);
+    if (kv.dim == 64) kv_append<DT, 64><<<grid, kAppThreads, 0, st>>>(kv, k, v, T, stride, starts, vec);
+    else kv_append<DT, 128><<<grid, kAppThreads, 0, st>>>(kv, k, v, T, stride, starts, vec);
     return cudaGetLastError();
 }
 
@@ -1230,22 +1302,26 @@ cudaError_t launch_attend(const AttendArgs& a, int n_sm, cudaStream_t st) {
 }
 
 template <int DT>
-cudaError_t evict_dt(const KvArgs& kv, const int* spare, int budget, const int* kept, unsigned grid, cudaStream_t st) {
+cudaError_t evict_dt(const KvArgs& kv, const int* spare, int budget, const int* kept, cudaStream_t st) {
+    const dim3 grid((unsigned) (kv.seqs * kv.heads), (unsigned) (budget / kPage));
     if (kv.dim == 64) evict_gather<DT, 64><<<grid, 256, 0, st>>>(kv, spare, budget, kept);
     else evict_gather<DT, 128><<<grid, 256, 0, st>>>(kv, spare, budget, kept);
     return cudaGetLastError();
 }
 
 cudaError_t launch_kv_evict(const KvArgs& kv, int* spare, int budget, int sinks, int recent, int* kept, cudaStream_t st) {
-    const unsigned units = (unsigned) (kv.seqs * kv.heads);
-    evict_select<<<units, kSelThreads, 0, st>>>(kv, spare, budget, sinks, recent, kept);
-    cudaError_t e = cudaGetLastError();
+    static std::atomic<uint64_t> ready{0};
+    cudaError_t e = allow_smem(ready, evict_select, kSelKeys * 4);
     if (e != cudaSuccess) return e;
-    const unsigned grid = units * (unsigned) (budget / kPage) * 2;
+    // room for the longest sequence that the table allows, as far as it goes
+    const int room = (int) std::min<long long>((long long) kv.width * kPage + kPage, kSelKeys);
+    evict_select<<<(unsigned) (kv.seqs * kv.heads), kSelThreads, (size_t) room * 4, st>>>(kv, spare, budget, sinks, recent, kept, room);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     switch (kv.dt) {
-        case F16: e = evict_dt<F16>(kv, spare, budget, kept, grid, st); break;
-        case BF16: e = evict_dt<BF16>(kv, spare, budget, kept, grid, st); break;
-        default: e = evict_dt<F32>(kv, spare, budget, kept, grid, st); break;
+        case F16: e = evict_dt<F16>(kv, spare, budget, kept, st); break;
+        case BF16: e = evict_dt<BF16>(kv, spare, budget, kept, st); break;
+        default: e = evict_dt<F32>(kv, spare, budget, kept, st); break;
     }
     if (e != cudaSuccess) return e;
     evict_swap<<<(unsigned) kv.seqs, 256, 0, st>>>(kv, spare, budget, kept);
