@@ -1197,11 +1197,11 @@ static AttendPlan attend_hints(const Ctx& c, const h3s_kv_cache* kv, int64_t T, 
     if (max_new <= 0 || max_new > T) max_new = T;
     const int64_t cap = kv->width * kPage + kPage - 1;
     if (max_len <= 0 || max_len > cap) max_len = cap;
-    return attend_plan(c.n_sm, kv->seqs, kv->heads, Hq / kv->heads, T, max_new, max_len);
+    return attend_plan(c.n_sm, kv->dt, kv->seqs, kv->heads, Hq / kv->heads, T, max_new, max_len);
 }
 static uint64_t attend_bytes(const AttendPlan& p, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate) {
     const uint64_t rows = (uint64_t) T * (uint64_t) Hq;
-    return (p.nz > 1 ? rows * p.nz * (kv->dim + 2) * 4 : 0) + (accumulate ? rows * 4 : 0);
+    return (p.nz > 1 ? rows * p.nz * (kv->dim + 2) * 4 : 0) + (accumulate ? (rows + 3) / 4 * 16 : 0);   // the partial results start on 16 bytes
 }
 static int check_attend(const char* who, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate, KvArgs& a) {
     if (check_kv(who, kv, accumulate != 0, a) != 0) return -1;
@@ -1240,10 +1240,11 @@ int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64
     a.starts = starts;
     a.out = out;
     a.lse = accumulate ? static_cast<float*>(work) : nullptr;
-    a.part = static_cast<float*>(work) + (accumulate ? T * Hq : 0);
+    a.part = static_cast<float*>(work) + (accumulate ? (T * Hq + 3) / 4 * 4 : 0);
     a.max_new = max_new;
     a.scale_log2 = (1.0f / std::sqrt((float) kv->dim)) * 1.4426950408889634f;
     a.q_vec = aligned16(q) && (qs * esize(kv->dt)) % 16 == 0;
+    a.out_vec = aligned16(out);
     a.wait_err = c.err;
     a.wait_ns = c.wait_ns;
     const cudaError_t e = launch_attend(a, c.n_sm, c.st);

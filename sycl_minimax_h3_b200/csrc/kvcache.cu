@@ -8,79 +8,10 @@
 
 #include "attn_common.cuh"
 #include "kvcache.cuh"
-#include "prepass.cuh"
+#include "kvcommon.cuh"
 
 namespace h3 {
 namespace {
-
-// ---- shared pieces -------------------------------------------------------------------------------------------------
-
-// Sequence b's new rows [s0, s0 + n) and its length L, checked against the call's rows and the table's width.
-struct Seq {
-    int s0, n, L;
-    bool ok;
-};
-__device__ __forceinline__ Seq load_seq(const KvArgs& kv, const int* starts, long long T, int b) {
-    Seq s;
-    s.s0 = starts[b];
-    const int s1 = starts[b + 1];
-    s.n = s1 - s.s0;
-    s.L = kv.lens[b];
-    s.ok = s.s0 >= 0 && s1 >= s.s0 && s1 <= T && s.L >= 0 && s.L / kPage <= kv.width;
-    return s;
-}
-__device__ __forceinline__ bool page_ok(const KvArgs& kv, int page) { return page >= 0 && page < kv.pages; }
-
-template <int DT>
-__device__ __forceinline__ void st1(void* p, size_t i, float x) {
-    if constexpr (DT == F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
-    else if constexpr (DT == BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-    else reinterpret_cast<float*>(p)[i] = x;
-}
-// 8 consecutive values at element i, with 16-byte loads where vec
-template <int DT>
-__device__ __forceinline__ void ld8(const void* p, size_t i, bool vec, float* x) {
-    if (vec) {
-        const char* c = reinterpret_cast<const char*>(p) + i * DtInfo<DT>::ES;
-        ld16<DT>(c, x);
-        if constexpr (DT == F32) ld16<DT>(c + 16, x + 4);
-    } else {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = ld1<DT>(p, i + u);
-    }
-}
-
-// 8 values as they lie in memory, and as floats
-template <int DT>
-struct Raw8 {
-    uint4 u[DT == F32 ? 2 : 1];
-};
-template <int DT>
-__device__ __forceinline__ Raw8<DT> raw8(const void* p, size_t i, bool vec) {
-    Raw8<DT> r;
-    const char* c = reinterpret_cast<const char*>(p) + i * DtInfo<DT>::ES;
-    if (vec) {
-        r.u[0] = *reinterpret_cast<const uint4*>(c);
-        if constexpr (DT == F32) r.u[1] = *reinterpret_cast<const uint4*>(c + 16);
-    } else {
-        uint32_t w[8] = {};
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            if constexpr (DT == F32) w[u] = reinterpret_cast<const uint32_t*>(c)[u];
-            else w[u / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(c)[u] << (16 * (u & 1));
-        }
-        r.u[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        if constexpr (DT == F32) r.u[1] = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-    return r;
-}
-template <int DT>
-__device__ __forceinline__ void floats8(const Raw8<DT>& r, float (&x)[8]) {
-    cvt16<DT>(r.u[0], x);
-    if constexpr (DT == F32) cvt16<DT>(r.u[1], x + 4);
-}
-
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // The codes of eight values x times sc in a block whose largest magnitude is top > 0: 127 x sc / top rounded to the nearest
 // whole number, half way to even, as if the ratio were exact. ratio = 127 sc / top as a float is off by 2^-23 of itself at
@@ -282,25 +213,6 @@ __device__ __forceinline__ uint32_t codes02(uint32_t x) {
 constexpr float kCodeUnit = 16777216.0f;                   // 2^24
 // keeps the compiler from loading shared memory ahead of this point, which would cost more registers than there are
 __device__ __forceinline__ void load_fence() { asm volatile("" ::: "memory"); }
-
-// The keys that a tile of query rows sees, and how they are divided: np whole pages in pieces of cz pages, and the tail
-// (when seen) as a piece of its own, or with the last piece where no split is left.
-struct Pieces {
-    int np, cz, nu, tail_at;           // nu pieces; the tail is read by piece tail_at (-1: not seen)
-};
-constexpr int kMinPages = 4;           // a split has at least a page per warp
-__device__ __forceinline__ Pieces pieces(int L, int last_pos, int nz) {
-    Pieces p;
-    const int seen = min(L, last_pos + 1), full = L / kPage;
-    if (seen <= 0) { p.np = 0; p.cz = 1; p.nu = 0; p.tail_at = -1; return p; }
-    p.np = min(full, (seen + kPage - 1) / kPage);
-    p.cz = max(kMinPages, (p.np + nz - 1) / nz);
-    const int nc = (p.np + p.cz - 1) / p.cz;
-    const bool tail = seen > full * kPage;
-    p.nu = tail ? min(nc + 1, nz) : nc;
-    p.tail_at = tail ? p.nu - 1 : -1;
-    return p;
-}
 
 constexpr int kAttWarps = 4;
 // p is 2^(s - m) with m the largest score less this, so at most 2^14: fp16 then keeps its 11 bits of every p down to
@@ -1240,14 +1152,17 @@ cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, lon
     }
 }
 
-AttendPlan attend_plan(int n_sm, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
+// Rows of a tile by how many rows a sequence brings. 256 rows on tcgen05 for 16-bit rows from kTcRows on.
+constexpr int64_t kTcRows = 128;
+AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
     AttendPlan p;
     const int64_t rows = std::min(max_new, T) * group;
-    p.rows = rows <= 8 ? 8 : 16;
+    p.rows = rows <= 8 ? 8 : dt != F32 && rows >= kTcRows ? 256 : 16;
     p.tiles = (int) std::min<int64_t>(std::max<int64_t>(1, (rows + p.rows - 1) / p.rows), 65535);
     const int64_t pages = (max_len + kPage - 1) / kPage, units = seqs * heads * p.tiles;
     const int64_t most = (pages + kMinPages - 1) / kMinPages;
-    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, (n_sm * 3 * (units > n_sm ? 4 : 1) + units - 1) / units, 512}));
+    const int64_t ctas = p.rows == 256 ? n_sm : n_sm * 3 * (units > n_sm ? 4 : 1);
+    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, p.rows == 256 ? ctas / units : (ctas + units - 1) / units, 512}));
     return p;
 }
 
@@ -1276,7 +1191,7 @@ cudaError_t attend_nb(const AttendArgs& a, cudaStream_t st) {
 template <int DT, int D>
 cudaError_t attend_dt(const AttendArgs& a, int n_sm, cudaStream_t st) {
     const KvArgs& kv = a.kv;
-    cudaError_t e = a.plan.rows == 8 ? attend_nb<DT, D, 1>(a, st) : attend_nb<DT, D, 2>(a, st);
+    cudaError_t e = a.plan.rows == 256 ? launch_attend_tc(a, st) : a.plan.rows == 8 ? attend_nb<DT, D, 1>(a, st) : attend_nb<DT, D, 2>(a, st);
     if (e != cudaSuccess) return e;
     if (a.plan.nz > 1) {
         const unsigned rows = (unsigned) std::min(a.max_new * a.Hq, 65535ll);

@@ -32,11 +32,11 @@ struct KvArgs {
 
 // How a call's queries and keys are divided (the same on the host and in every kernel of one call).
 struct AttendPlan {
-    int rows;                          // query rows of a tile: 8 or 16
+    int rows;                          // query rows of a tile: 8 or 16, or 256 on tcgen05
     int tiles;                         // tiles per (sequence, kv head); more are looped over
     int nz;                            // splits of the keys
 };
-AttendPlan attend_plan(int n_sm, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len);
+AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len);
 
 struct AttendArgs {
     KvArgs kv;
@@ -50,11 +50,13 @@ struct AttendArgs {
     AttendPlan plan;
     long long max_new;
     float scale_log2;                  // log2(e) / sqrt(dim)
-    int q_vec;                         // 16-byte loads of q's rows allowed
+    int q_vec, out_vec;                // 16-byte loads of q's rows and stores of out's allowed
     int* wait_err;                     // device error word of waits that gave up
     unsigned long long wait_ns;        // limit of every wait
 };
 cudaError_t launch_attend(const AttendArgs& a, int n_sm, cudaStream_t st);
+
+cudaError_t launch_attend_tc(const AttendArgs& a, cudaStream_t st);   // attendtc.cu
 
 cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, long long T, long long stride, const int* starts,
                              long long max_new, bool vec, cudaStream_t st);

@@ -90,7 +90,10 @@ def attention(c: ops.KVCache, q: torch.Tensor, heads_q: int, starts):
       (L / 16 + 64) 2^-23   the sums over L keys, of which a lane adds every sixteenth one after the other
     (in float32 also 2^-21 of |q k| for the scores: q enters as two terms). And sum_j |v_j| times 2^-38: p is held as fp16
     between 2^-24 and 2^14, the row's largest, so one of its smallest numbers is off by half of 2^-24, which is 2^-39 of the
-    largest p and of the sum of all p at most; twice that for the two terms. Then half a step of the output's type, of
+    largest p and of the sum of all p at most; twice that for the two terms. Where many rows come in a call, p times its
+    page's scale is what is rounded, its largest at least 2^6: 2^-31 of the row's largest p scale for every code |v| / scale,
+    twice that for the reference's own move (the tail's scale is the power of two that brings its largest into [2^13,
+    2^14)). Then half a step of the output's type, of
     what is rounded: the value and the errors before it."""
     heads, dim = c.k.shape[1], c.k.shape[3]
     starts = starts.tolist()
@@ -104,6 +107,10 @@ def attention(c: ops.KVCache, q: torch.Tensor, heads_q: int, starts):
         n, L = starts[b + 1] - starts[b], int(c.lens[b])
         k, v = sequence(c, b, "k"), sequence(c, b, "v")
         w = torch.zeros(heads, L, dtype=torch.float64)
+        full = L // PAGE
+        page = c.v_scale[c.table[b, :full].long()].double().cpu()
+        top = torch.where(c.tail_v[b].isfinite(), c.tail_v[b], 0).double().abs().amax((1, 2)).cpu() if L % PAGE else torch.ones(heads)
+        vscale = torch.cat((page.repeat_interleave(PAGE, 0), (2.0 ** (torch.floor(torch.log2(top)) - 13)).expand(L % PAGE, heads)))
         pos = torch.arange(L - n, L)
         hidden = torch.arange(L)[None] > pos[:, None]
         for h in range(heads_q):
@@ -117,6 +124,10 @@ def attention(c: ops.KVCache, q: torch.Tensor, heads_q: int, starts):
             ds = (mag.max(1).values if L else torch.zeros(n)) * ((dim + 8) * 2.0 ** -23 + (2.0 ** -21 if wide else 0.0))
             rel = 2 * ds + (2.0 ** -21 if wide else 2.0 ** -11) + 2.0 ** -22 + (L / 16 + 64) * 2.0 ** -23
             bound[starts[b]:starts[b + 1], h] = rel[:, None] * (p @ vh.abs()) + 2.0 ** -38 * ((~hidden).double() @ vh.abs())
+            if not wide and L:
+                vs = vscale[:, h // (heads_q // heads)]
+                code = torch.where(vs[:, None] > 0, vh.abs() / torch.where(vs > 0, vs, 1)[:, None], 0)
+                bound[starts[b]:starts[b + 1], h] += 2.0 ** -30 * (p * vs).max(1, keepdim=True).values * ((~hidden).double() @ code)
         weights.append(w)
     half = torch.finfo(c.tail_k.dtype).eps / 2
     bound = bound + half * (out.abs() + bound) + torch.finfo(c.tail_k.dtype).tiny

@@ -473,3 +473,85 @@ def test_bad_pages_and_lengths_are_reported(cuda):
             wait(cuda)
     wait(cuda)
     assert torch.equal(run_attention(cache, q, heads * per, starts, cuda)[0], good[0])
+
+
+# ---- many query rows (tcgen05 for 16-bit types) ----
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,per,lens,news", [
+    (1, 4, [64], [64]),                     # one page, one tile
+    (2, 4, [200], [200]),                   # a whole prompt: pages and a tail
+    (1, 1, [300], [256]),
+    (1, 3, [700, 130, 0, 64], [300, 7, 0, 60]),   # rows of a token over a tile's edge; short sequences beside a long one
+    (1, 8, [1000], [130]),                  # several tiles
+    (1, 16, [63], [63]),                    # the tail alone
+    (1, 2, [100, 5], [200, 90]),            # more rows than tokens: the first ones see nothing
+    (2, 2, [2500], [64]),                   # few tiles: the keys are split
+])
+def test_attention_of_many_rows(dtype, dim, heads, per, lens, news, cuda):
+    cache = _kv.random_cache(lens, heads, dim, dtype, cuda, seed=len(lens) + dim + 40)
+    q = make_rows(sum(news), heads * per * dim, dtype, cuda, 41)
+    starts = _kv.starts_of(news, cuda)
+    out = run_attention(cache, q, heads * per, starts, cuda)
+    check_attention(cache, q, starts, out, heads * per)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_with_few_tiles_in_the_grid(dtype, cuda):
+    """A hint of 128 new tokens for a sequence that brings 1,100: a CTA takes several tiles one after the other."""
+    cache = _kv.random_cache([1200, 600], 1, 64, dtype, cuda, seed=42)
+    q = make_rows(1100 + 130, 2 * 64, dtype, cuda, 43)
+    starts = _kv.starts_of([1100, 130], cuda)
+    out = run_attention(cache, q, 2, starts, cuda, max_new=128)
+    check_attention(cache, q, starts, out, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,news", [([150], [150]), ([900], [64])])
+def test_many_rows_value_scales_of_many_sizes(dtype, lens, news, cuda):
+    """Pages whose value scales differ by factors of 2^20, and some that are 0: every page counts by its own."""
+    cache = _kv.random_cache(lens, 1, 64, dtype, cuda, seed=44, weights=True)
+    pages = cache.table[0, :lens[0] // PAGE].long()
+    for i, p in enumerate(pages):
+        cache.v_scale[p] = 0.02 * 2.0 ** (-20 if i % 3 == 1 else 0)
+        if i % 3 == 2:
+            cache.v_scale[p] = 0
+            cache.v[p] = 0
+    q = make_rows(news[0], 4 * 64, dtype, cuda, 45)
+    starts = _kv.starts_of(news, cuda)
+    before = _kv.seq_weights(cache, 0).double()
+    out = run_attention(cache, q, 4, starts, cuda, accumulate=True)
+    weights = check_attention(cache, q, starts, out, 4)
+    got = _kv.seq_weights(cache, 0).double()
+    assert float(((got - before - weights[0]).abs() - 2.0 ** -12 * weights[0] - 2.0 ** -23 * (before + weights[0])).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_rows_hidden_slots_may_hold_anything(dtype, cuda):
+    """NaN and infinities behind the end, in later tokens, in other sequences' pages and in other rows of q."""
+    n, per, dim = 100, 2, 64
+    cache = _kv.random_cache([n], 1, dim, dtype, cuda, seed=46)
+    others = [p for p in range(cache.k.shape[0]) if p != int(cache.table[0, 0])]
+    cache.k_scale[others] = float("nan")
+    cache.v_scale[others] = float("inf")
+    cache.tail_k[0, :, n - PAGE:] = float("nan")
+    cache.tail_v[0, :, n - PAGE:] = float("inf")
+    q = make_rows(n, per * dim, dtype, cuda, 47)
+    starts = _kv.starts_of([n], cuda)
+    clean = run_attention(cache, q, per, starts, cuda)
+    check_attention(cache, q, starts, clean, per)
+    at = 90 - PAGE
+    cache.tail_v[0, 0, at, 5] = float("inf")
+    cache.tail_v[0, 0, at + 2, 6] = float("nan")
+    out = run_attention(cache, q, per, starts, cuda).view(n, per, dim)
+    was = clean.view(n, per, dim)
+    assert torch.equal(out[:90], was[:90]) and torch.equal(out[:, :, 7:], was[:, :, 7:])
+    assert bool((out[90:, :, 5] == float("inf")).all()) and bool(out[92:, :, 6].isnan().all())
+    assert torch.equal(out[90:92, :, 6], was[90:92, :, 6])
+    cache.tail_k[0, 0, at, 3] = float("nan")
+    q[7, 1], q[8, dim + 1] = float("nan"), float("inf")
+    out = run_attention(cache, q, per, starts, cuda).view(n, per, dim)
+    bad = torch.zeros(n, per, dtype=torch.bool, device=cuda)
+    bad[90:] = bad[7, 0] = bad[8, 1] = True
+    assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], was[~bad])
