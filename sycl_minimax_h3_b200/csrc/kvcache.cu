@@ -1160,6 +1160,8 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     p.rows = rows <= 8 ? 8 : dt != F32 && rows >= kTcRows ? 256 : 16;
     p.tiles = (int) std::min<int64_t>(std::max<int64_t>(1, (rows + p.rows - 1) / p.rows), 65535);
     const int64_t pages = (max_len + kPage - 1) / kPage, units = seqs * heads * p.tiles;
+    // on tcgen05 the tiles of all sequences lie one after the other: room for as many as there can be
+    if (p.rows == 256) p.tiles = (int) std::min<int64_t>(T * group / 256 + seqs, INT32_MAX / heads);
     const int64_t most = (pages + kMinPages - 1) / kMinPages;
     const int64_t ctas = p.rows == 256 ? n_sm : n_sm * 3 * (units > n_sm ? 4 : 1);
     p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, p.rows == 256 ? ctas / units : (ctas + units - 1) / units, 512}));

@@ -33,7 +33,7 @@ struct KvArgs {
 // How a call's queries and keys are divided (the same on the host and in every kernel of one call).
 struct AttendPlan {
     int rows;                          // query rows of a tile: 8 or 16, or 256 on tcgen05
-    int tiles;                         // tiles per (sequence, kv head); more are looped over
+    int tiles;                         // tiles per (sequence, kv head); more are looped over (256 rows: of all sequences)
     int nz;                            // splits of the keys
 };
 AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len);
