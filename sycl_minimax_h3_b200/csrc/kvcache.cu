@@ -322,6 +322,25 @@ __device__ __forceinline__ void page_scores(const QFrag<D, NB, TWO>& f, const in
 // warp: one or two are in flight while one is read.
 constexpr int kSlots = 2;
 
+// four neighbouring outputs, with one store where vec
+template <int DT>
+__device__ __forceinline__ void st4(void* p, size_t i, float x, float y, float z, float w, bool vec) {
+    if (!vec) {
+        st1<DT>(p, i, x);
+        st1<DT>(p, i + 1, y);
+        st1<DT>(p, i + 2, z);
+        st1<DT>(p, i + 3, w);
+    } else if constexpr (DT == F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(x, y, z, w);
+    } else if constexpr (DT == F16) {
+        *reinterpret_cast<uint2*>(static_cast<__half*>(p) + i) = make_uint2(pack_half2(x, y), pack_half2(z, w));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x, y), b = __floats2bfloat162_rn(z, w);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
 template <int D, int NB>
 struct AttSmem {
     union {
@@ -656,25 +675,27 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
             const int d = threadIdx.x % D, rb = threadIdx.x / D * TR;
 #pragma unroll
             for (int r = 0; r < TR; ++r) ot[r] = 0.0f;
-            if (sm.pos[0] >= s.L - 1) {                    // every row sees the whole tail
+            float odd = 0.0f;                              // NaN once a value is infinite or NaN
 #pragma unroll
-                for (int r = 0; r < TR; r += 4) {
-                    if (rb + r >= nrow) break;
+            for (int r = 0; r < TR; r += 4) {
+                if (rb + r >= nrow) break;
 #pragma unroll 8
-                    for (int key = 0; key < nkey; ++key) {
-                        const float x = ld1<DT>(sm.tail[1], (size_t) key * D + d);
-                        const float4 e = *reinterpret_cast<const float4*>(&sm.sc[key][rb + r]);
-                        ot[r] = fmaf(e.x, x, ot[r]);
-                        ot[r + 1] = fmaf(e.y, x, ot[r + 1]);
-                        ot[r + 2] = fmaf(e.z, x, ot[r + 2]);
-                        ot[r + 3] = fmaf(e.w, x, ot[r + 3]);
-                    }
+                for (int key = 0; key < nkey; ++key) {
+                    const float x = ld1<DT>(sm.tail[1], (size_t) key * D + d);
+                    const float4 e = *reinterpret_cast<const float4*>(&sm.sc[key][rb + r]);
+                    ot[r] = fmaf(e.x, x, ot[r]);
+                    ot[r + 1] = fmaf(e.y, x, ot[r + 1]);
+                    ot[r + 2] = fmaf(e.z, x, ot[r + 2]);
+                    ot[r + 3] = fmaf(e.w, x, ot[r + 3]);
+                    odd = fmaf(x, 0.0f, odd);
                 }
-            } else {
+            }
+            if (odd != 0.0f && sm.pos[0] < s.L - 1) {      // some rows see less: theirs again, without what they do not see
 #pragma unroll
                 for (int r = 0; r < TR; ++r) {
                     if (rb + r >= nrow) break;
                     const int see = min(nkey, sm.pos[rb + r] + 1 - full * kPage);
+                    ot[r] = 0.0f;
 #pragma unroll 4
                     for (int key = 0; key < see; ++key) ot[r] = fmaf(sm.sc[key][rb + r], ld1<DT>(sm.tail[1], (size_t) key * D + d), ot[r]);
                 }
@@ -692,26 +713,33 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                 for (int c = 0; c < 2; ++c)
                     *reinterpret_cast<float2*>(&sm.acc[warp][8 * nb + 2 * t + c][DG * g + 2 * i]) = make_float2(acc[i][nb][c], acc[i][nb][2 + c]);
         __syncthreads();
-        // the pieces of this CTA as one: rows straight out, or a partial result per split
+        // the pieces of this CTA as one: rows straight out, or a partial result per split; four features to a thread
         const int parts = kAttWarps + (tail ? 1 : 0);
-        for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32) {
-            const int r = i / D, d = i % D;
+        for (int i = threadIdx.x; i < nrow * (D / 4); i += kAttWarps * 32) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
             float mx = -INFINITY;
             for (int p = 0; p < parts; ++p) mx = fmaxf(mx, sm.m[p][r]);
             // NaN scores leave the maximum alone and come out of the sums
             const float mu = mx == -INFINITY ? 0.0f : mx;
-            float sum = 0.0f, o = 0.0f;
+            float sum = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int p = 0; p < parts; ++p) {
                 const float e = ex2(sm.m[p][r] - mu);
+                const float4 x = *reinterpret_cast<const float4*>(&sm.acc[p][r][d]);
                 sum = fmaf(e, sm.l[p][r], sum);
-                o = fmaf(e, sm.acc[p][r][d], o);
+                o.x = fmaf(e, x.x, o.x);
+                o.y = fmaf(e, x.y, o.y);
+                o.z = fmaf(e, x.z, o.z);
+                o.w = fmaf(e, x.w, o.w);
             }
             const size_t gr = (size_t) sm.row[r];
             if (pc.nu <= 1) {
-                st1<DT>(a.out, gr * D + d, sum == 0.0f ? 0.0f : o / sum);
-                if (a.lse && d == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);
+                const bool none = sum == 0.0f;
+                st4<DT>(a.out, gr * D + d, none ? 0.0f : o.x / sum, none ? 0.0f : o.y / sum, none ? 0.0f : o.z / sum,
+                        none ? 0.0f : o.w / sum, a.out_vec);
+                if (a.lse && d == 0) a.lse[gr] = none ? INFINITY : mu + log2f(sum);
             } else {
-                a.part[(gr * nz + z) * D + d] = o;
+                *reinterpret_cast<float4*>(a.part + (gr * nz + z) * D + d) = o;
                 if (d == 0) {
                     float* ml = a.part + (size_t) a.T * a.Hq * nz * D + (gr * nz + z) * 2;
                     ml[0] = mx;
@@ -1152,8 +1180,11 @@ cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, lon
     }
 }
 
-// Rows of a tile by how many rows a sequence brings. 256 rows on tcgen05 for 16-bit rows from kTcRows on.
-constexpr int64_t kTcRows = 128;
+// Rows of a tile by how many rows a sequence brings (new tokens times the heads of a group): up to 8, 16, and for 16-bit
+// types from kTcRows on 256, on tcgen05. Measured at 32 / 64 rows per kv head, tiles of 16 against tcgen05, us: one
+// sequence of 16,384 tokens 48 / 64 against 44 / 44, four of 2,048 39 / 45 against 29 / 33, sixteen of 300 66 / 108 against
+// 23 / 23, one of 131,072 170 / 302 against 224 / 226; 64-wide heads at 16,384 31 / 38 against 40 / 41.
+constexpr int64_t kTcRows = 48;
 AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
     AttendPlan p;
     const int64_t rows = std::min(max_new, T) * group;
@@ -1163,8 +1194,12 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     // on tcgen05 the tiles of all sequences lie one after the other: room for as many as there can be
     if (p.rows == 256) p.tiles = (int) std::min<int64_t>(T * group / 256 + seqs, INT32_MAX / heads);
     const int64_t most = (pages + kMinPages - 1) / kMinPages;
-    const int64_t ctas = p.rows == 256 ? n_sm : n_sm * 3 * (units > n_sm ? 4 : 1);
-    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, p.rows == 256 ? ctas / units : (ctas + units - 1) / units, 512}));
+    // tcgen05: a CTA per SM. Else three CTAs are resident on an SM; where there are more (sequence, head, tile) units than
+    // that takes, they are split only as far as unequal lengths want it
+    const int64_t room = p.rows == 256 ? n_sm : (int64_t) n_sm * 3;
+    static const double f = getenv("NZF") ? atof(getenv("NZF")) : 1.0;
+    const int64_t nz = p.rows == 256 ? room / units : units * 2 < room ? room / units : (int64_t) (f * room / units + 0.5);
+    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, nz, 512}));
     return p;
 }
 
