@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.Hq / kv.heads, nz = a.plan.nz;
     const int h = (int) (blockIdx.x % kv.heads), z = blockIdx.y;
+    let_next_launch();
     // which sequence's tile this is: the tiles of all sequences one after the other, a prefix sum over the sequences
     int* const found = reinterpret_cast<int*>(sm + C::OFF_MISC + 8);
     {
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
                 }
             }
             if (live && split) {
-                float* ml = a.part + (size_t) a.T * a.Hq * nz * HD + (gr * nz + z) * 2;
+                float* ml = a.part + (size_t) a.plan.entries * HD + (gr * nz + z) * 2;
                 ml[0] = m_run;
                 ml[1] = l_run;
             } else if (live && a.lse) {
@@ -601,7 +602,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     const cudaError_t e = allow(ready, attend_tc<DT, HD>, TcCfg<HD>::SMEM);
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned) (a.kv.heads * a.plan.tiles), (unsigned) a.plan.nz);
+    const dim3 grid((unsigned) (a.kv.heads * a.plan.grid), (unsigned) a.plan.nz);
     attend_tc<DT, HD><<<grid, TcCfg<HD>::THREADS, TcCfg<HD>::SMEM, st>>>(a);
     return cudaGetLastError();
 }

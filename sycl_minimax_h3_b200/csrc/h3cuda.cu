@@ -1201,7 +1201,7 @@ static AttendPlan attend_hints(const Ctx& c, const h3s_kv_cache* kv, int64_t T, 
 }
 static uint64_t attend_bytes(const AttendPlan& p, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate) {
     const uint64_t rows = (uint64_t) T * (uint64_t) Hq;
-    return (p.nz > 1 ? rows * p.nz * (kv->dim + 2) * 4 : 0) + (accumulate ? (rows + 3) / 4 * 16 : 0);   // the partial results start on 16 bytes
+    return (p.joined ? (uint64_t) p.entries * (kv->dim + 2) * 4 + (uint64_t) kv->seqs * 8 : 0) + (accumulate ? (rows + 3) / 4 * 16 : 0);   // the partial results start on 16 bytes
 }
 static int check_attend(const char* who, const h3s_kv_cache* kv, int64_t T, int64_t Hq, int accumulate, KvArgs& a) {
     if (check_kv(who, kv, accumulate != 0, a) != 0) return -1;

@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(kAppThreads, DT == F32 ? 3 : 4) kv_append(cons
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    // volatile: in the order written, which keeps four sums in flight and the operands' registers few
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -215,6 +216,126 @@ constexpr float kCodeUnit = 16777216.0f;                   // 2^24
 __device__ __forceinline__ void load_fence() { asm volatile("" ::: "memory"); }
 
 constexpr int kAttWarps = 4;
+
+// Which piece the flat-th of a call is. A sequence has tiles x heads units of `length` pages each (its whole pages, and the
+// tail as kTailPages more), cut into nz pieces; a piece has about as many pages as the sum over all units divided by
+// `room`, but kChunk at least: so unequal sequences give nearly equal pieces, and a short one is one piece. Up to 32
+// sequences are a warp's, a lane each, and every warp finds the piece for itself; more are the 128 threads' together.
+constexpr int kTailPages = 2, kChunk = 6;
+struct Piece {
+    int b, unit, z, nz;                // b < 0: there are no more
+    Seq s;
+};
+__device__ __forceinline__ int pieces_of_unit(int length, int chunk) { return max(1, (2 * length + chunk) / (2 * chunk)); }   // rounded
+template <int ROWS>
+__device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int group, int* scan) {
+    const KvArgs& kv = a.kv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto units_of = [&](int i, int& length) {
+        length = 0;
+        if (i >= kv.seqs) return 0;
+        const Seq s = load_seq(kv, a.starts, a.T, i);
+        if (!s.ok) {
+            atomicOr(kv.err, kErrLen);
+            return 0;
+        }
+        length = max(1, s.L / kPage + (s.L % kPage ? kTailPages : 0));
+        return (s.n * group + ROWS - 1) / ROWS * kv.heads;
+    };
+    if (kv.seqs <= 32) {
+        Seq s{0, 0, 0, false};
+        int units = 0, length = 0, nz = 1;
+        if (lane < kv.seqs) {
+            s = load_seq(kv, a.starts, a.T, lane);
+            length = max(1, s.L / kPage + (s.L % kPage ? kTailPages : 0));
+            if (s.ok) units = (s.n * group + ROWS - 1) / ROWS * kv.heads;
+            else atomicOr(kv.err, kErrLen);
+        }
+        if (a.plan.room > 0) {
+            float all = (float) units * (float) length;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            nz = pieces_of_unit(length, max(kChunk, (int) ceilf(all / (float) a.plan.room)));
+        }
+        int upto = units * nz;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const int from = upto - units * nz;
+        const uint32_t here = __ballot_sync(0xffffffffu, flat >= from && flat < upto);
+        Piece p{-1, 0, 0, 1, s};
+        if (here == 0) return p;
+        const int i = __ffs((int) here) - 1, at = flat - __shfl_sync(0xffffffffu, from, i);
+        p.nz = __shfl_sync(0xffffffffu, nz, i);
+        if (a.plan.joined && at == 0 && (int) threadIdx.x == i)
+            reinterpret_cast<int2*>(a.part + (size_t) a.plan.entries * (kv.dim + 2))[i] = make_int2(flat, nz);
+        p.b = i;
+        p.s.s0 = __shfl_sync(0xffffffffu, s.s0, i);
+        p.s.n = __shfl_sync(0xffffffffu, s.n, i);
+        p.s.L = __shfl_sync(0xffffffffu, s.L, i);
+        p.s.ok = true;
+        // the heads side by side: they lie side by side in a page, and are read at about the same time
+        const int zt = at / kv.heads;
+        p.unit = zt / p.nz * kv.heads + at % kv.heads;
+        p.z = zt % p.nz;
+        return p;
+    }
+    int length0 = 0, units0 = units_of((int) threadIdx.x, length0);      // the first 128 sequences' are kept
+    int chunk = 1 << 30;
+    if (a.plan.room > 0) {
+        float all = 0.0f;                                  // pages in all: a float is exact enough to divide them
+        for (int b0 = 0; b0 < kv.seqs; b0 += kAttWarps * 32) {
+            int length = length0;
+            const int units = b0 == 0 ? units0 : units_of(b0 + (int) threadIdx.x, length);
+            all += (float) units * (float) length;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (lane == 0) scan[warp] = __float_as_int(all);
+        __syncthreads();
+        all = __int_as_float(scan[0]) + __int_as_float(scan[1]) + __int_as_float(scan[2]) + __int_as_float(scan[3]);
+        chunk = max(kChunk, (int) ceilf(all / (float) a.plan.room));
+    }
+    int* found = scan + 2 * kAttWarps;
+    if (threadIdx.x == 0) found[0] = -1;
+    int before = 0;
+    for (int b0 = 0; b0 < kv.seqs; b0 += kAttWarps * 32) {
+        int length = length0;
+        const int units = b0 == 0 ? units0 : units_of(b0 + (int) threadIdx.x, length);
+        const int nz = pieces_of_unit(length, chunk), n = units * nz;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (b0 > 0) __syncthreads();                       // the sums of the sequences before have been read
+        if (lane == 31) scan[kAttWarps + warp] = upto;
+        __syncthreads();
+        int from = before + upto - n, sum = 0;
+#pragma unroll
+        for (int w = 0; w < kAttWarps; ++w) {
+            if (w < warp) from += scan[kAttWarps + w];
+            sum += scan[kAttWarps + w];
+        }
+        if (flat >= from && flat < from + n) {
+            found[0] = b0 + (int) threadIdx.x;
+            const int i = flat - from, h = i % kv.heads, zt = i / kv.heads;
+            found[1] = zt / nz * kv.heads + h;
+            found[2] = zt % nz;
+            found[3] = nz;
+            if (a.plan.joined && flat == from)
+                reinterpret_cast<int2*>(a.part + (size_t) a.plan.entries * (kv.dim + 2))[found[0]] = make_int2(from, nz);
+        }
+        before += sum;
+    }
+    __syncthreads();
+    Piece p{found[0], found[1], found[2], found[3], {0, 0, 0, false}};
+    if (p.b >= 0) p.s = load_seq(kv, a.starts, a.T, p.b);
+    return p;
+}
 // p is 2^(s - m) with m the largest score less this, so at most 2^14: fp16 then keeps its 11 bits of every p down to
 // 2^-28 of the row's largest (2^-14 without it), and 2^-39 of the largest is what it drops
 constexpr float kPTop = 14.0f;
@@ -356,6 +477,9 @@ struct AttSmem {
     long long qoff[8 * NB];                                // the query row's first element, or -1
     uint64_t full[kAttWarps][kSlots];
     uint64_t tail_full;
+    int scan[3 * kAttWarps + 4];
+    // what the epilogue needs again
+    int L, b, h, nrow, nu, tail_here;
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -400,6 +524,81 @@ __device__ __forceinline__ void tail_scores(const float (*qf)[D], const unsigned
         if (r0 + r < r1) sc[key][r0 + r] = acc[r] * scale;
 }
 
+// The tail of the piece at hand as one more partial result, sm.acc[kAttWarps]: on CUDA cores, in 32 bits, since it is in
+// its own type and has at most 63 keys. A function of its own, whose registers the loop over pages need not make room for.
+template <int DT, int D, int NB>
+__device__ __noinline__ void attend_tail(const AttendArgs& a) {
+    constexpr int ROWS = 8 * NB, TR = ROWS * D / (kAttWarps * 32);   // the rows in a thread, of one feature
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    AttSmem<D, NB>& sm = *reinterpret_cast<AttSmem<D, NB>*>(smem_raw);
+    const KvArgs& kv = a.kv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, L = sm.L, nrow = sm.nrow, b = sm.b, h = sm.h;
+    float ot[TR];
+    const int full = L / kPage, nkey = L - full * kPage;
+    __syncthreads();                               // the ring has been read
+    if (threadIdx.x == 0) {
+        const size_t tb = ((size_t) b * kv.heads + h) * kPage * D * DtInfo<DT>::ES;
+        const uint32_t bytes = (uint32_t) (nkey * D * DtInfo<DT>::ES);
+        mbar_expect_tx(&sm.tail_full, 2 * bytes);
+        bulk_load(sm.tail[0], static_cast<const char*>(kv.tk) + tb, bytes, &sm.tail_full);
+        bulk_load(sm.tail[1], static_cast<const char*>(kv.tv) + tb, bytes, &sm.tail_full);
+    }
+    for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32)
+        sm.q[i / D][i % D] = ld1<DT>(a.q, (size_t) sm.qoff[i / D] + i % D);
+    if (!mbar_wait(&sm.tail_full, 0, a.wait_ns, nullptr)) atomicOr(a.wait_err, kErrCache);
+    __syncthreads();
+    tail_scores<DT, D, ROWS>(sm.q, sm.tail[0], nrow, nkey, a.scale_log2, sm.sc);
+    __syncthreads();
+    for (int r = warp; r < nrow; r += kAttWarps) {
+        const int see = min(nkey, sm.pos[r] + 1 - full * kPage);
+        const float x0 = lane < see ? sm.sc[lane][r] : -INFINITY, x1 = lane + 32 < see ? sm.sc[lane + 32][r] : -INFINITY;
+        float mx = fmaxf(x0, x1);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        const float e0 = ex2(x0 - mu), e1 = ex2(x1 - mu);
+        float sum = e0 + e1;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sm.sc[lane][r] = e0;
+        sm.sc[lane + 32][r] = e1;
+        if (lane == 0) { sm.m[kAttWarps][r] = mx; sm.l[kAttWarps][r] = sum; }
+    }
+    __syncthreads();
+    // a thread has one feature and TR rows; a value that a row does not see is not multiplied by its p of 0
+    const int d = threadIdx.x % D, rb = threadIdx.x / D * TR;
+#pragma unroll
+    for (int r = 0; r < TR; ++r) ot[r] = 0.0f;
+    float odd = 0.0f;                              // NaN once a value is infinite or NaN
+#pragma unroll
+    for (int r = 0; r < TR; r += 4) {
+        if (rb + r >= nrow) break;
+#pragma unroll 8
+        for (int key = 0; key < nkey; ++key) {
+            const float x = ld1<DT>(sm.tail[1], (size_t) key * D + d);
+            const float4 e = *reinterpret_cast<const float4*>(&sm.sc[key][rb + r]);
+            ot[r] = fmaf(e.x, x, ot[r]);
+            ot[r + 1] = fmaf(e.y, x, ot[r + 1]);
+            ot[r + 2] = fmaf(e.z, x, ot[r + 2]);
+            ot[r + 3] = fmaf(e.w, x, ot[r + 3]);
+            odd = fmaf(x, 0.0f, odd);
+        }
+    }
+    if (odd != 0.0f && sm.pos[0] < L - 1) {      // some rows see less: theirs again, without what they do not see
+#pragma unroll
+        for (int r = 0; r < TR; ++r) {
+            if (rb + r >= nrow) break;
+            const int see = min(nkey, sm.pos[rb + r] + 1 - full * kPage);
+            ot[r] = 0.0f;
+#pragma unroll 4
+            for (int key = 0; key < see; ++key) ot[r] = fmaf(sm.sc[key][rb + r], ld1<DT>(sm.tail[1], (size_t) key * D + d), ot[r]);
+        }
+    }
+    __syncthreads();                                       // the tail has been read, its memory becomes accumulators
+#pragma unroll
+    for (int r = 0; r < TR; ++r) sm.acc[kAttWarps][threadIdx.x / D * TR + r][threadIdx.x % D] = ot[r];
+}
+
 template <int DT, int D, int NB>
 __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const __grid_constant__ AttendArgs a) {
     constexpr bool TWO = DT == F32;
@@ -409,27 +608,35 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
     AttSmem<D, NB>& sm = *reinterpret_cast<AttSmem<D, NB>*>(smem_raw);
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int group = a.Hq / kv.heads, nz = a.plan.nz;
-    const int b = (int) (blockIdx.x / kv.heads), h = (int) (blockIdx.x % kv.heads), z = blockIdx.y;
-    const Seq s = load_seq(kv, a.starts, a.T, b);
-    if (!s.ok) {
-        if (threadIdx.x == 0) atomicOr(kv.err, kErrLen);
-        return;
-    }
-    const int R = s.n * group;
+    const int group = a.Hq / kv.heads;
+    let_next_launch();
     if (threadIdx.x == 0) {
         for (int w = 0; w < kAttWarps; ++w)
             for (int i = 0; i < kSlots; ++i) mbar_init(&sm.full[w][i], 1);
         mbar_init(&sm.tail_full, 1);
         fence_barrier_init();
     }
-    uint32_t used = 0, issued = 0, tails = 0;              // tiles of this warp read and asked for; tails waited for
-    for (int tile = blockIdx.z; tile < (R + ROWS - 1) / ROWS; tile += gridDim.z) {
+    uint32_t used = 0, issued = 0;                         // tiles of this warp read and asked for
+    const int flat = (int) blockIdx.x;                     // the grid has room for every piece there can be
+    const Piece pcs = find_piece<ROWS>(a, flat, group, sm.scan);
+    if (pcs.b < 0) return;
+    {
+        const int b = pcs.b, nz = pcs.nz, z = pcs.z, h = pcs.unit % kv.heads, tile = pcs.unit / kv.heads;
+        const Seq s = pcs.s;
+        const int R = s.n * group;
         const int r0 = tile * ROWS, nrow = min(R - r0, ROWS);
         const int last_pos = s.L - s.n + (r0 + nrow - 1) / group;
         const Pieces pc = pieces(s.L, last_pos, nz);
-        if (z >= max(pc.nu, 1)) continue;
-        __syncthreads();                                   // the tile before has been written; the barriers are made
+        if (z >= max(pc.nu, 1)) return;
+        __syncthreads();                                   // the barriers are made
+        if (threadIdx.x == 0) {
+            sm.L = s.L;
+            sm.b = b;
+            sm.h = h;
+            sm.nrow = nrow;
+            sm.nu = pc.nu;
+            sm.tail_here = z == pc.tail_at;
+        }
         if (threadIdx.x < ROWS) {
             const int r = threadIdx.x;
             const bool in = r < nrow;
@@ -438,9 +645,52 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
             sm.row[r] = in ? (s.s0 + tok) * a.Hq + hq : -1;
             sm.qoff[r] = in ? (long long) (s.s0 + tok) * a.qs + hq * D : -1;
         }
-        fence_proxy_async_smem();                          // the ring was written as accumulators
         __syncthreads();
         float acc[DG / 2][NB][4], m[NB][2], l[NB][2];
+        const int p0 = z * pc.cz, p1 = min(pc.np, p0 + pc.cz);
+        // up to 32 pages of this warp at a time, from page `sub` on: lane i keeps the i-th one's id and scales. Their first
+        // tiles are asked for at once.
+        int sub = p0, id = -1;
+        float ks = 0.0f, vs = 0.0f;
+        uint32_t ask = 0, todo = 0;
+        bool ask_v = false;
+        auto next = [&]() {                                // the next tile into the slot that was freed last
+            if (ask == 0) return;
+            const int i = __ffs((int) ask) - 1, pid = __shfl_sync(0xffffffffu, id, i), slot = (int) (issued % kSlots);
+            if (lane == 0) {
+                mbar_expect_tx(&sm.full[warp][slot], TILE);
+                bulk_load(sm.ring[warp][slot], (ask_v ? kv.v : kv.k) + ((size_t) pid * kv.heads + h) * TILE, TILE, &sm.full[warp][slot]);
+            }
+            ++issued;
+            if (ask_v) ask &= ask - 1;
+            ask_v = !ask_v;
+        };
+        auto begin = [&]() {
+            const int mine = sub + warp + kAttWarps * lane;
+            id = -1;
+            if (mine < p1) {
+                id = kv.table[(size_t) b * kv.width + mine];
+                if (!page_ok(kv, id)) {
+                    atomicOr(kv.err, kErrPage);
+                    id = -1;
+                }
+            }
+            ask = todo = __ballot_sync(0xffffffffu, id >= 0);
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) next();
+            if (id >= 0) {
+                ks = kv.ks[(size_t) id * kv.heads + h];
+                vs = kv.vs[(size_t) id * kv.heads + h];
+            }
+        };
+        QFrag<D, NB, TWO> f;
+        if (p0 < p1) {
+            begin();
+            long long qrow[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) qrow[nb] = sm.qoff[8 * nb + g];
+            load_q<DT, D, NB, TWO>(f, a.q, qrow, a.q_vec, a.scale_log2);
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             m[nb][0] = m[nb][1] = -INFINITY;
@@ -450,9 +700,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
 #pragma unroll
                 for (int u = 0; u < 4; ++u) acc[i][nb][u] = 0.0f;
         }
-        const int p0 = z * pc.cz, p1 = min(pc.np, p0 + pc.cz);
         if (p0 < p1) {
-            QFrag<D, NB, TWO> f;
             int pos[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -460,46 +708,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                 pos[nb][1] = sm.pos[8 * nb + 2 * t + 1];
             }
             const int first_pos = sm.pos[0];
-            bool have_q = false;
-            for (int sub = p0; sub < p1; sub += 32 * kAttWarps) {
-                // up to 32 pages of this warp: lane i keeps the i-th one's id and scales
-                const int mine = sub + warp + kAttWarps * lane;
-                int id = -1;
-                float ks = 0.0f, vs = 0.0f;
-                if (mine < p1) {
-                    id = kv.table[(size_t) b * kv.width + mine];
-                    if (!page_ok(kv, id)) {
-                        atomicOr(kv.err, kErrPage);
-                        id = -1;
-                    }
-                }
-                uint32_t ask = __ballot_sync(0xffffffffu, id >= 0), todo = ask;
-                bool ask_v = false;
-                auto next = [&]() {                        // the next tile into the slot that was freed last
-                    if (ask == 0) return;
-                    const int i = __ffs((int) ask) - 1, pid = __shfl_sync(0xffffffffu, id, i), slot = (int) (issued % kSlots);
-                    if (lane == 0) {
-                        mbar_expect_tx(&sm.full[warp][slot], TILE);
-                        bulk_load(sm.ring[warp][slot], (ask_v ? kv.v : kv.k) + ((size_t) pid * kv.heads + h) * TILE, TILE,
-                                  &sm.full[warp][slot]);
-                    }
-                    ++issued;
-                    if (ask_v) ask &= ask - 1;
-                    ask_v = !ask_v;
-                };
-#pragma unroll
-                for (int i = 0; i < kSlots; ++i) next();
-                if (id >= 0) {
-                    ks = kv.ks[(size_t) id * kv.heads + h];
-                    vs = kv.vs[(size_t) id * kv.heads + h];
-                }
-                if (!have_q) {
-                    long long qrow[NB];
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) qrow[nb] = sm.qoff[8 * nb + g];
-                    load_q<DT, D, NB, TWO>(f, a.q, qrow, a.q_vec, a.scale_log2);
-                    have_q = true;
-                }
+            while (true) {
                 auto arrived = [&]() {
                     if (warp_wait(&sm.full[warp][used % kSlots], (used / kSlots) & 1, a.wait_ns, nullptr)) return true;
                     if (lane == 0) atomicOr(a.wait_err, kErrCache);
@@ -576,17 +785,19 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                                 w[mt][kk][0] = u.x;
                                 w[mt][kk][1] = u.y;
                             }
+                        float c[2][2][NB][4];
 #pragma unroll
-                        for (int wd = 0; wd < 2; ++wd) {
-                            float c[2][NB][4];
+                        for (int wd = 0; wd < 2; ++wd)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
 #pragma unroll
                                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) c[u][nb][e] = 0.0f;
+                                    for (int e = 0; e < 4; ++e) c[wd][u][nb][e] = 0.0f;
 #pragma unroll
-                            for (int mt = 0; mt < 4; ++mt) {
+                        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                            for (int wd = 0; wd < 2; ++wd) {
                                 uint32_t v[2][4];          // [keys 2t.. / 8 + 2t..][feature of the word]
 #pragma unroll
                                 for (int k2 = 0; k2 < 2; ++k2) {
@@ -600,11 +811,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                                     for (int nb = 0; nb < NB; ++nb) {
-                                        mma16816(c[u][nb], v[0][2 * u], v[0][2 * u + 1], v[1][2 * u], v[1][2 * u + 1], ph[mt][nb][0], ph[mt][nb][1]);
+                                        mma16816(c[wd][u][nb], v[0][2 * u], v[0][2 * u + 1], v[1][2 * u], v[1][2 * u + 1], ph[mt][nb][0], ph[mt][nb][1]);
                                         if constexpr (TWO)
-                                            mma16816(c[u][nb], v[0][2 * u], v[0][2 * u + 1], v[1][2 * u], v[1][2 * u + 1], pl[mt][nb][0], pl[mt][nb][1]);
+                                            mma16816(c[wd][u][nb], v[0][2 * u], v[0][2 * u + 1], v[1][2 * u], v[1][2 * u + 1], pl[mt][nb][0], pl[mt][nb][1]);
                                     }
                             }
+#pragma unroll
+                        for (int wd = 0; wd < 2; ++wd)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -612,14 +825,16 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
 #pragma unroll
                                     for (int e = 0; e < 4; ++e) {
                                         float& y = acc[hf * 4 + wd * 2 + u][nb][e];
-                                        y = fmaf(vscale, c[u][nb][e], y * al[nb][e & 1]);
+                                        y = fmaf(vscale, c[wd][u][nb][e], y * al[nb][e & 1]);
                                     }
-                        }
                     }
                     __syncwarp();
                     ++used;
                     next();
                 }
+                sub += 32 * kAttWarps;
+                if (sub >= p1) break;
+                begin();
             }
         }
 #pragma unroll
@@ -635,76 +850,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                     sm.l[warp][8 * nb + 2 * t + c] = x;
                 }
             }
-        const bool tail = z == pc.tail_at;
-        constexpr int TR = ROWS * D / (kAttWarps * 32);    // the tail's rows in a thread, of one feature
-        float ot[TR];
-        if (tail) {                                        // CUDA cores: the tail is in its own type, at most 63 keys
-            const int full = s.L / kPage, nkey = s.L - full * kPage;
-            __syncthreads();                               // the ring has been read
-            if (threadIdx.x == 0) {
-                const size_t tb = ((size_t) b * kv.heads + h) * kPage * D * DtInfo<DT>::ES;
-                const uint32_t bytes = (uint32_t) (nkey * D * DtInfo<DT>::ES);
-                mbar_expect_tx(&sm.tail_full, 2 * bytes);
-                bulk_load(sm.tail[0], static_cast<const char*>(kv.tk) + tb, bytes, &sm.tail_full);
-                bulk_load(sm.tail[1], static_cast<const char*>(kv.tv) + tb, bytes, &sm.tail_full);
-            }
-            for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32)
-                sm.q[i / D][i % D] = ld1<DT>(a.q, (size_t) sm.qoff[i / D] + i % D);
-            if (!mbar_wait(&sm.tail_full, tails & 1, a.wait_ns, nullptr)) atomicOr(a.wait_err, kErrCache);
-            ++tails;
-            __syncthreads();
-            tail_scores<DT, D, ROWS>(sm.q, sm.tail[0], nrow, nkey, a.scale_log2, sm.sc);
-            __syncthreads();
-            for (int r = warp; r < nrow; r += kAttWarps) {
-                const int see = min(nkey, sm.pos[r] + 1 - full * kPage);
-                const float x0 = lane < see ? sm.sc[lane][r] : -INFINITY, x1 = lane + 32 < see ? sm.sc[lane + 32][r] : -INFINITY;
-                float mx = fmaxf(x0, x1);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float mu = mx == -INFINITY ? 0.0f : mx;
-                const float e0 = ex2(x0 - mu), e1 = ex2(x1 - mu);
-                float sum = e0 + e1;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                sm.sc[lane][r] = e0;
-                sm.sc[lane + 32][r] = e1;
-                if (lane == 0) { sm.m[kAttWarps][r] = mx; sm.l[kAttWarps][r] = sum; }
-            }
-            __syncthreads();
-            // a thread has one feature and TR rows; a value that a row does not see is not multiplied by its p of 0
-            const int d = threadIdx.x % D, rb = threadIdx.x / D * TR;
-#pragma unroll
-            for (int r = 0; r < TR; ++r) ot[r] = 0.0f;
-            float odd = 0.0f;                              // NaN once a value is infinite or NaN
-#pragma unroll
-            for (int r = 0; r < TR; r += 4) {
-                if (rb + r >= nrow) break;
-#pragma unroll 8
-                for (int key = 0; key < nkey; ++key) {
-                    const float x = ld1<DT>(sm.tail[1], (size_t) key * D + d);
-                    const float4 e = *reinterpret_cast<const float4*>(&sm.sc[key][rb + r]);
-                    ot[r] = fmaf(e.x, x, ot[r]);
-                    ot[r + 1] = fmaf(e.y, x, ot[r + 1]);
-                    ot[r + 2] = fmaf(e.z, x, ot[r + 2]);
-                    ot[r + 3] = fmaf(e.w, x, ot[r + 3]);
-                    odd = fmaf(x, 0.0f, odd);
-                }
-            }
-            if (odd != 0.0f && sm.pos[0] < s.L - 1) {      // some rows see less: theirs again, without what they do not see
-#pragma unroll
-                for (int r = 0; r < TR; ++r) {
-                    if (rb + r >= nrow) break;
-                    const int see = min(nkey, sm.pos[rb + r] + 1 - full * kPage);
-                    ot[r] = 0.0f;
-#pragma unroll 4
-                    for (int key = 0; key < see; ++key) ot[r] = fmaf(sm.sc[key][rb + r], ld1<DT>(sm.tail[1], (size_t) key * D + d), ot[r]);
-                }
-            }
-        }
-        __syncthreads();                                   // ring and tail have been read: they become accumulators
-        if (tail)
-#pragma unroll
-            for (int r = 0; r < TR; ++r) sm.acc[kAttWarps][threadIdx.x / D * TR + r][threadIdx.x % D] = ot[r];
+        const bool tail = sm.tail_here != 0;
+        if (tail) attend_tail<DT, D, NB>(a);
+        else __syncthreads();                              // the ring has been read: it becomes accumulators
 #pragma unroll
         for (int i = 0; i < DG / 2; ++i)
 #pragma unroll
@@ -715,7 +863,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
         __syncthreads();
         // the pieces of this CTA as one: rows straight out, or a partial result per split; four features to a thread
         const int parts = kAttWarps + (tail ? 1 : 0);
-        for (int i = threadIdx.x; i < nrow * (D / 4); i += kAttWarps * 32) {
+        const int n_rows = sm.nrow;
+        const bool whole = sm.nu <= 1;
+        for (int i = threadIdx.x; i < n_rows * (D / 4); i += kAttWarps * 32) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             float mx = -INFINITY;
             for (int p = 0; p < parts; ++p) mx = fmaxf(mx, sm.m[p][r]);
@@ -733,15 +883,16 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                 o.w = fmaf(e, x.w, o.w);
             }
             const size_t gr = (size_t) sm.row[r];
-            if (pc.nu <= 1) {
+            if (whole) {
                 const bool none = sum == 0.0f;
                 st4<DT>(a.out, gr * D + d, none ? 0.0f : o.x / sum, none ? 0.0f : o.y / sum, none ? 0.0f : o.z / sum,
                         none ? 0.0f : o.w / sum, a.out_vec);
                 if (a.lse && d == 0) a.lse[gr] = none ? INFINITY : mu + log2f(sum);
             } else {
-                *reinterpret_cast<float4*>(a.part + (gr * nz + z) * D + d) = o;
+                const size_t at = (size_t) blockIdx.x * ROWS + r;
+                *reinterpret_cast<float4*>(a.part + at * D + d) = o;
                 if (d == 0) {
-                    float* ml = a.part + (size_t) a.T * a.Hq * nz * D + (gr * nz + z) * 2;
+                    float* ml = a.part + (size_t) a.plan.entries * D + at * 2;
                     ml[0] = mx;
                     ml[1] = sum;
                 }
@@ -751,47 +902,84 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
 }
 
 // The splits' partial results of a row as one: a CTA per row, whose warps take the splits in turn and then meet.
+constexpr int kJoinWarps = 8;
 template <int DT, int D>
-__global__ void __launch_bounds__(128) attend_join(const __grid_constant__ AttendArgs a) {
-    __shared__ float so[4][D], sl[4];
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_constant__ AttendArgs a) {
+    __shared__ float so[kJoinWarps][D], sl[kJoinWarps], sx[kJoinWarps];
     const KvArgs& kv = a.kv;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nz = a.plan.nz, group = a.Hq / kv.heads, rows = a.plan.rows;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.Hq / kv.heads, rows = a.plan.rows;
     const int b = blockIdx.x;
     const Seq s = load_seq(kv, a.starts, a.T, b);
-    if (!s.ok) return;
-    const float* mls = a.part + (size_t) a.T * a.Hq * nz * D;
+    let_next_launch();
+    wait_for_previous();
+    if (!s.ok || s.n == 0) return;
+    const float* mls = a.part + (size_t) a.plan.entries * D;
+    int2 pieces_of = make_int2(0, a.plan.nz);              // this sequence's first piece, the pieces of a unit
+    if (rows != 256) pieces_of = reinterpret_cast<const int2*>(mls + (size_t) a.plan.entries * 2)[b];
+    if (pieces_of.y <= 1) return;
     for (int i = blockIdx.y; i < s.n * a.Hq; i += gridDim.y) {
         const int tok = i / a.Hq, hq = i % a.Hq;
-        const int R = s.n * group, r0 = (tok * group + hq % group) / rows * rows;
+        const int R = s.n * group, row = tok * group + hq % group, tile = row / rows, r0 = tile * rows;
         const int last_pos = s.L - s.n + (min(R, r0 + rows) - 1) / group;
-        const Pieces pc = pieces(s.L, last_pos, nz);
+        const Pieces pc = pieces(s.L, last_pos, pieces_of.y);
         if (pc.nu <= 1) continue;
         const size_t gr = (size_t) (s.s0 + tok) * a.Hq + hq;
-        const float* ml = mls + gr * nz * 2;
-        float mx = -INFINITY;
-        for (int z = lane; z < pc.nu; z += 32) mx = fmaxf(mx, ml[2 * z]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float mu = mx == -INFINITY ? 0.0f : mx;
-        float sum = 0.0f, o[D / 32];
+        // the row's partial results: entries at, at + step, ...
+        const size_t step = rows == 256 ? 1 : (size_t) kv.heads * rows;
+        const size_t at = rows == 256 ? gr * a.plan.nz
+                                      : (size_t) (pieces_of.x + tile * pieces_of.y * kv.heads + hq / group) * rows + (row - r0);
+        // each warp its own splits, up to 8 at a time under way
+        float m = -INFINITY, sum = 0.0f, o[D / 32];
 #pragma unroll
         for (int u = 0; u < D / 32; ++u) o[u] = 0.0f;
-#pragma unroll 4
-        for (int z = warp; z < pc.nu; z += 4) {
-            const float e = ex2(ml[2 * z] - mu);
-            sum = fmaf(e, ml[2 * z + 1], sum);
+        for (int z0 = warp; z0 < pc.nu; z0 += 8 * kJoinWarps) {
+            float2 ml[8];
+            float x[8][D / 32];
 #pragma unroll
-            for (int u = 0; u < D / 32; ++u) o[u] = fmaf(e, a.part[(gr * nz + z) * D + lane + 32 * u], o[u]);
+            for (int i = 0; i < 8; ++i) {
+                const int z = z0 + i * kJoinWarps;
+                const size_t w = at + (size_t) min(z, pc.nu - 1) * step;
+                ml[i] = *reinterpret_cast<const float2*>(mls + w * 2);
+                if (z >= pc.nu) ml[i] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int u = 0; u < D / 32; ++u) x[i][u] = z < pc.nu ? a.part[w * D + lane + 32 * u] : 0.0f;
+            }
+            float mn = m;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+            const float mu = mn == -INFINITY ? 0.0f : mn, al = ex2(m - mu);
+            sum *= al;
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) o[u] *= al;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float e = ex2(ml[i].x - mu);
+                sum = fmaf(e, ml[i].y, sum);
+#pragma unroll
+                for (int u = 0; u < D / 32; ++u) o[u] = fmaf(e, x[i][u], o[u]);
+            }
+            m = mn;
         }
         __syncthreads();                                   // the row before has been written
-        if (lane == 0) sl[warp] = sum;
+        if (lane == 0) {
+            sl[warp] = sum;
+            sx[warp] = m;
+        }
 #pragma unroll
         for (int u = 0; u < D / 32; ++u) so[warp][lane + 32 * u] = o[u];
         __syncthreads();
-        sum = sl[0] + sl[1] + sl[2] + sl[3];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) mx = fmaxf(mx, sx[w]);
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) sum = fmaf(ex2(sx[w] - mu), sl[w], sum);
         if (threadIdx.x < D) {
             const int d = threadIdx.x;
-            const float y = so[0][d] + so[1][d] + so[2][d] + so[3][d];
+            float y = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) y = fmaf(ex2(sx[w] - mu), so[w][d], y);
             st1<DT>(a.out, gr * D + d, sum == 0.0f ? 0.0f : y / sum);
         }
         if (a.lse && threadIdx.x == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);
@@ -812,6 +1000,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_co
     const int group = a.Hq / kv.heads;
     const int z = (int) (blockIdx.x % nzw), h = (int) (blockIdx.x / nzw % kv.heads), b = (int) (blockIdx.x / nzw / kv.heads);
     const Seq s = load_seq(kv, a.starts, a.T, b);
+    wait_for_previous();
     if (!s.ok || s.n == 0) return;
     const int R = s.n * group;
     const int full = s.L / kPage;
@@ -928,6 +1117,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
     const int h = (int) (blockIdx.x % kv.heads), b = (int) (blockIdx.x / kv.heads);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int L = kv.lens[b];
+    let_next_launch();
     int* out = kept + (size_t) blockIdx.x * budget;
     const int* table = kv.table + (size_t) b * kv.width;
     const int full = L / kPage;
@@ -1135,6 +1325,8 @@ __global__ void __launch_bounds__(256, 4) evict_gather(const __grid_constant__ K
     const int nb = budget / kPage, blk = blockIdx.y;
     const int b = (int) (blockIdx.x / kv.heads), h = (int) (blockIdx.x % kv.heads);
     const int* mine = kept + (size_t) blockIdx.x * budget;
+    let_next_launch();
+    wait_for_previous();
     if (mine[0] == kLeftAlone) return;
     const int page = spare[(size_t) b * nb + blk];
     int at = 0;
@@ -1147,6 +1339,7 @@ __global__ void __launch_bounds__(256, 4) evict_gather(const __grid_constant__ K
 // the new pages take the old ones' place in the table, which take theirs among the spare ones
 __global__ void __launch_bounds__(256) evict_swap(const KvArgs kv, int* __restrict__ spare, int budget, const int* __restrict__ kept) {
     const int b = (int) blockIdx.x, nb = budget / kPage;
+    wait_for_previous();
     if (kept[(size_t) b * kv.heads * budget] == kLeftAlone) return;
     for (int i = threadIdx.x; i < nb; i += 256) {
         int* p = kv.table + (size_t) b * kv.width + i;
@@ -1186,20 +1379,26 @@ cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, lon
 // 23 / 23, one of 131,072 170 / 302 against 224 / 226; 64-wide heads at 16,384 31 / 38 against 40 / 41.
 constexpr int64_t kTcRows = 48;
 AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
-    AttendPlan p;
-    const int64_t rows = std::min(max_new, T) * group;
+    AttendPlan p{};
+    const int64_t rows = std::min(max_new, T) * group, pages = (max_len + kPage - 1) / kPage;
     p.rows = rows <= 8 ? 8 : dt != F32 && rows >= kTcRows ? 256 : 16;
-    p.tiles = (int) std::min<int64_t>(std::max<int64_t>(1, (rows + p.rows - 1) / p.rows), 65535);
-    const int64_t pages = (max_len + kPage - 1) / kPage, units = seqs * heads * p.tiles;
-    // on tcgen05 the tiles of all sequences lie one after the other: room for as many as there can be
-    if (p.rows == 256) p.tiles = (int) std::min<int64_t>(T * group / 256 + seqs, INT32_MAX / heads);
-    const int64_t most = (pages + kMinPages - 1) / kMinPages;
-    // tcgen05: a CTA per SM. Else three CTAs are resident on an SM; where there are more (sequence, head, tile) units than
-    // that takes, they are split only as far as unequal lengths want it
-    const int64_t room = p.rows == 256 ? n_sm : (int64_t) n_sm * 3;
-    static const double f = getenv("NZF") ? atof(getenv("NZF")) : 1.0;
-    const int64_t nz = p.rows == 256 ? room / units : units * 2 < room ? room / units : (int64_t) (f * room / units + 0.5);
-    p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({most, nz, 512}));
+    // as many tiles as there can be, of all sequences together
+    const int64_t tiles = T * group / p.rows + seqs;
+    if (p.rows == 256) {
+        p.grid = (int) std::min<int64_t>(tiles, INT32_MAX / heads);
+        const int64_t units = seqs * heads * std::max<int64_t>(1, (rows + 255) / 256);
+        p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({(pages + kMinPages - 1) / kMinPages, n_sm / units, 512}));
+        p.joined = p.nz > 1;
+        p.entries = p.joined ? T * heads * group * p.nz : 0;
+        return p;
+    }
+    // two or three CTAs are resident on an SM. Units that are many, or as short as a piece may be, stay whole.
+    const int64_t room = (int64_t) n_sm * (p.rows == 8 ? 3 : 2), units = tiles * heads;
+    p.nz = 1;
+    p.joined = units <= 8 * room && 2 * (pages + kTailPages) >= 3 * kChunk;
+    p.room = p.joined ? (int) room : 0;
+    p.grid = (int) std::min<int64_t>(units + p.room, 1 << 30);
+    p.entries = p.joined ? (units + room) * p.rows : 0;
     return p;
 }
 
@@ -1220,8 +1419,7 @@ cudaError_t attend_nb(const AttendArgs& a, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
     const cudaError_t e = allow_smem(ready, attend<DT, D, NB>, sizeof(AttSmem<D, NB>));
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned) (a.kv.seqs * a.kv.heads), (unsigned) a.plan.nz, (unsigned) a.plan.tiles);
-    attend<DT, D, NB><<<grid, kAttWarps * 32, sizeof(AttSmem<D, NB>), st>>>(a);
+    attend<DT, D, NB><<<(unsigned) a.plan.grid, kAttWarps * 32, sizeof(AttSmem<D, NB>), st>>>(a);
     return cudaGetLastError();
 }
 
@@ -1230,16 +1428,14 @@ cudaError_t attend_dt(const AttendArgs& a, int n_sm, cudaStream_t st) {
     const KvArgs& kv = a.kv;
     cudaError_t e = a.plan.rows == 256 ? launch_attend_tc(a, st) : a.plan.rows == 8 ? attend_nb<DT, D, 1>(a, st) : attend_nb<DT, D, 2>(a, st);
     if (e != cudaSuccess) return e;
-    if (a.plan.nz > 1) {
-        const unsigned rows = (unsigned) std::min(a.max_new * a.Hq, 65535ll);
-        attend_join<DT, D><<<dim3((unsigned) kv.seqs, rows), 128, 0, st>>>(a);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (a.plan.joined) {
+        const dim3 grid((unsigned) kv.seqs, (unsigned) std::min(a.max_new * a.Hq, 65535ll));
+        if ((e = launch_after(attend_join<DT, D>, grid, kJoinWarps * 32, 0, st, a)) != cudaSuccess) return e;
     }
     if (a.lse) {
         const long long units = (long long) kv.seqs * kv.heads;
         const int nzw = (int) std::max(1ll, std::min<long long>((kv.width + kAttWarps - 1) / kAttWarps, (n_sm * 4 + units - 1) / units));
-        attend_weights<DT, D><<<(unsigned) (units * nzw), kAttWarps * 32, (kPage - 1) * D * DtInfo<DT>::ES, st>>>(a, nzw);
-        e = cudaGetLastError();
+        e = launch_after(attend_weights<DT, D>, dim3((unsigned) (units * nzw)), kAttWarps * 32, (kPage - 1) * D * DtInfo<DT>::ES, st, a, nzw);
     }
     return e;
 }
@@ -1256,9 +1452,8 @@ cudaError_t launch_attend(const AttendArgs& a, int n_sm, cudaStream_t st) {
 template <int DT>
 cudaError_t evict_dt(const KvArgs& kv, const int* spare, int budget, const int* kept, cudaStream_t st) {
     const dim3 grid((unsigned) (kv.seqs * kv.heads), (unsigned) (budget / kPage));
-    if (kv.dim == 64) evict_gather<DT, 64><<<grid, 256, 0, st>>>(kv, spare, budget, kept);
-    else evict_gather<DT, 128><<<grid, 256, 0, st>>>(kv, spare, budget, kept);
-    return cudaGetLastError();
+    if (kv.dim == 64) return launch_after(evict_gather<DT, 64>, grid, 256, 0, st, kv, spare, budget, kept);
+    return launch_after(evict_gather<DT, 128>, grid, 256, 0, st, kv, spare, budget, kept);
 }
 
 cudaError_t launch_kv_evict(const KvArgs& kv, int* spare, int budget, int sinks, int recent, int* kept, cudaStream_t st) {
@@ -1276,8 +1471,7 @@ cudaError_t launch_kv_evict(const KvArgs& kv, int* spare, int budget, int sinks,
         default: e = evict_dt<F32>(kv, spare, budget, kept, st); break;
     }
     if (e != cudaSuccess) return e;
-    evict_swap<<<(unsigned) kv.seqs, 256, 0, st>>>(kv, spare, budget, kept);
-    return cudaGetLastError();
+    return launch_after(evict_swap, dim3((unsigned) kv.seqs), 256, 0, st, kv, spare, budget, kept);
 }
 
 }  // namespace h3

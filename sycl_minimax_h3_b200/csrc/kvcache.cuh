@@ -33,8 +33,12 @@ struct KvArgs {
 // How a call's queries and keys are divided (the same on the host and in every kernel of one call).
 struct AttendPlan {
     int rows;                          // query rows of a tile: 8 or 16, or 256 on tcgen05
-    int tiles;                         // tiles per (sequence, kv head); more are looped over (256 rows: of all sequences)
-    int nz;                            // splits of the keys
+    // 8 or 16 rows: `grid` CTAs take the pieces of all (sequence, tile, head) units one after the other, the pieces of
+    // about as many pages as make `room` of them (0: every unit is one piece). 256: `grid` tiles (of all sequences) x
+    // heads x nz splits of the keys.
+    int grid, room, nz;
+    bool joined;                       // partial results may be left, which attend_join brings together
+    long long entries;                 // of partial rows
 };
 AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len);
 
@@ -45,7 +49,8 @@ struct AttendArgs {
     int Hq;
     const int* starts;                 // [seqs + 1]
     void* out;                         // [T, Hq * dim]
-    float* part;                       // [T * Hq, nz, dim] accumulators and, behind them, [T * Hq, nz, 2] (max, sum); nz > 1
+    float* part;                       // [entries, dim] accumulators, [entries, 2] (max, sum), and an int2 per sequence: its
+                                       // first piece and the pieces of one of its units
     float* lse;                        // [T * Hq] or NULL: log2 of the softmax's sum, for the weights
     AttendPlan plan;
     long long max_new;
