@@ -348,24 +348,39 @@ struct QFrag {
     float s0[NB][2];                   //   and where their sums start
 };
 
-// rows 8 nb + g of a tile as B fragments; qrow: element offsets, or -1 for a row of zeros
+// rows 8 nb + g of a tile as they lie in memory: features 64 c + 16 t .. + 15; qrow: element offsets, or -1 for zeros. Apart
+// from what makes fragments of them, so that other loads can be made while these are under way.
+template <int DT, int D, int NB>
+struct QRows {
+    Raw8<DT> x[NB][D / 32];
+};
+template <int DT, int D, int NB>
+__device__ __forceinline__ void load_q(QRows<DT, D, NB>& r, const void* q, const long long (&qrow)[NB], bool vec) {
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            if (qrow[nb] >= 0) r.x[nb][i] = raw8<DT>(q, (size_t) qrow[nb] + (i >> 1) * 64 + t * 16 + (i & 1) * 8, vec);
+            else
+#pragma unroll
+                for (int u = 0; u < (DT == F32 ? 2 : 1); ++u) r.x[nb][i].u[u] = make_uint4(0, 0, 0, 0);
+        }
+}
+// ... as B fragments
 template <int DT, int D, int NB, bool TWO>
-__device__ __forceinline__ void load_q(QFrag<D, NB, TWO>& f, const void* q, const long long (&qrow)[NB], bool vec, float scale) {
+__device__ __forceinline__ void make_q(QFrag<D, NB, TWO>& f, const QRows<DT, D, NB>& r, float scale) {
     const int t = threadIdx.x & 3;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        float x[D / 4];                // features 64 c + 16 t .. + 15
-        float top = 0.0f;
+        float x[D / 4], top = 0.0f;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
+        for (int i = 0; i < D / 32; ++i) {
+            float y[8];
+            floats8(r.x[nb][i], y);
 #pragma unroll
-            for (int u = 0; u < 16; u += 8) {
-                float* y = &x[c * 16 + u];
-                if (qrow[nb] >= 0) ld8<DT>(q, (size_t) qrow[nb] + c * 64 + t * 16 + u, vec, y);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = 0.0f;
-            }
+            for (int u = 0; u < 8; ++u) x[i * 8 + u] = y[u];
+        }
 #pragma unroll
         for (int i = 0; i < D / 4; ++i)
             if (finite(x[i])) top = fmaxf(top, fabsf(x[i]));
@@ -482,9 +497,16 @@ struct AttSmem {
     int L, b, h, nrow, nu, tail_here;
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar))
+// The codes leave L2 first: a step reads them once, and what every CTA waits for at its start (lengths, tables, scales,
+// queries) should not make room for them.
+__device__ __forceinline__ uint64_t leave_first() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(dst)),
+                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
                  : "memory");
 }
 
@@ -540,8 +562,8 @@ __device__ __noinline__ void attend_tail(const AttendArgs& a) {
         const size_t tb = ((size_t) b * kv.heads + h) * kPage * D * DtInfo<DT>::ES;
         const uint32_t bytes = (uint32_t) (nkey * D * DtInfo<DT>::ES);
         mbar_expect_tx(&sm.tail_full, 2 * bytes);
-        bulk_load(sm.tail[0], static_cast<const char*>(kv.tk) + tb, bytes, &sm.tail_full);
-        bulk_load(sm.tail[1], static_cast<const char*>(kv.tv) + tb, bytes, &sm.tail_full);
+        bulk_load(sm.tail[0], static_cast<const char*>(kv.tk) + tb, bytes, &sm.tail_full, leave_first());
+        bulk_load(sm.tail[1], static_cast<const char*>(kv.tv) + tb, bytes, &sm.tail_full, leave_first());
     }
     for (int i = threadIdx.x; i < nrow * D; i += kAttWarps * 32)
         sm.q[i / D][i % D] = ld1<DT>(a.q, (size_t) sm.qoff[i / D] + i % D);
@@ -659,7 +681,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
             const int i = __ffs((int) ask) - 1, pid = __shfl_sync(0xffffffffu, id, i), slot = (int) (issued % kSlots);
             if (lane == 0) {
                 mbar_expect_tx(&sm.full[warp][slot], TILE);
-                bulk_load(sm.ring[warp][slot], (ask_v ? kv.v : kv.k) + ((size_t) pid * kv.heads + h) * TILE, TILE, &sm.full[warp][slot]);
+                bulk_load(sm.ring[warp][slot], (ask_v ? kv.v : kv.k) + ((size_t) pid * kv.heads + h) * TILE, TILE, &sm.full[warp][slot], leave_first());
             }
             ++issued;
             if (ask_v) ask &= ask - 1;
@@ -685,11 +707,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
         };
         QFrag<D, NB, TWO> f;
         if (p0 < p1) {
-            begin();
+            QRows<DT, D, NB> rows;
             long long qrow[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) qrow[nb] = sm.qoff[8 * nb + g];
-            load_q<DT, D, NB, TWO>(f, a.q, qrow, a.q_vec, a.scale_log2);
+            load_q(rows, a.q, qrow, a.q_vec);
+            begin();
+            make_q(f, rows, a.scale_log2);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -1033,8 +1057,10 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_co
                 pos2[c] = __shfl_sync(0xffffffffu, pos, 8 * t + 4 * c);
                 lse2[c] = __shfl_sync(0xffffffffu, lse, 8 * t + 4 * c);
             }
+            QRows<DT, D, NB> rows;
             QFrag<D, NB, TWO> f;
-            load_q<DT, D, NB, TWO>(f, a.q, off, a.q_vec, a.scale_log2);
+            load_q(rows, a.q, off, a.q_vec);
+            make_q(f, rows, a.scale_log2);
             float x[4][NB][4];
             page_scores<D, NB, TWO>(f, kv.k + pb * kPage * D, x);
 #pragma unroll
