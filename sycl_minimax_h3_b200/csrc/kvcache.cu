@@ -340,78 +340,76 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
 // 2^-28 of the row's largest (2^-14 without it), and 2^-39 of the largest is what it drops
 constexpr float kPTop = 14.0f;
 
+// The query rows of a tile as B fragments in shared memory, which a CTA's warps share: step ks of rows 8 nb + g is two words
+// of lane (g, t), hi[nb][ks][lane]; TWO: and the second terms. rs: what a row's scores are multiplied by, with a page's scale; s0:
+// where its sums start.
 template <int D, int NB, bool TWO>
 struct QFrag {
-    uint32_t hi[NB][D / 16][2];
-    uint32_t lo[TWO ? NB : 1][TWO ? D / 16 : 1][2];
-    float rs[NB][2];                   // queries 8 nb + 2 t and + 1: what their scores are multiplied by, with a page's scale
-    float s0[NB][2];                   //   and where their sums start
+    uint2 hi[NB][D / 16][32];
+    uint2 lo[TWO ? NB : 1][TWO ? D / 16 : 1][32];
+    float rs[8 * NB], s0[8 * NB];
 };
-
-// rows 8 nb + g of a tile as they lie in memory: features 64 c + 16 t .. + 15; qrow: element offsets, or -1 for zeros. Apart
-// from what makes fragments of them, so that other loads can be made while these are under way.
-template <int DT, int D, int NB>
+// D / 8 threads to a row, 8 features to a thread; T threads. The loads apart from what makes fragments of them, so that
+// others can be made while these are under way. qoff: the rows' element offsets, or -1 for a row of zeros.
+template <int DT, int D, int NB, int T>
 struct QRows {
-    Raw8<DT> x[NB][D / 32];
+    static constexpr int PER = (8 * NB * D / 8 + T - 1) / T;
+    Raw8<DT> x[PER];
 };
-template <int DT, int D, int NB>
-__device__ __forceinline__ void load_q(QRows<DT, D, NB>& r, const void* q, const long long (&qrow)[NB], bool vec) {
-    const int t = threadIdx.x & 3;
+template <int DT, int D, int NB, int T>
+__device__ __forceinline__ void load_q(QRows<DT, D, NB, T>& r, const void* q, const long long* qoff, bool vec) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int j = 0; j < QRows<DT, D, NB, T>::PER; ++j) {
+        const int i = (int) threadIdx.x % T + j * T, row = i / (D / 8);
+        const long long at = row < 8 * NB ? qoff[row] : -1;
+        if (at >= 0) r.x[j] = raw8<DT>(q, (size_t) at + i % (D / 8) * 8, vec);
+        else
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            if (qrow[nb] >= 0) r.x[nb][i] = raw8<DT>(q, (size_t) qrow[nb] + (i >> 1) * 64 + t * 16 + (i & 1) * 8, vec);
-            else
-#pragma unroll
-                for (int u = 0; u < (DT == F32 ? 2 : 1); ++u) r.x[nb][i].u[u] = make_uint4(0, 0, 0, 0);
-        }
+            for (int u = 0; u < (DT == F32 ? 2 : 1); ++u) r.x[j].u[u] = make_uint4(0, 0, 0, 0);
+    }
 }
-// ... as B fragments
-template <int DT, int D, int NB, bool TWO>
-__device__ __forceinline__ void make_q(QFrag<D, NB, TWO>& f, const QRows<DT, D, NB>& r, float scale) {
-    const int t = threadIdx.x & 3;
+template <int DT, int D, int NB, bool TWO, int T>
+__device__ __forceinline__ void make_q(QFrag<D, NB, TWO>& f, const QRows<DT, D, NB, T>& r, float scale) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        float x[D / 4], top = 0.0f;
+    for (int j = 0; j < QRows<DT, D, NB, T>::PER; ++j) {
+        const int i = (int) threadIdx.x % T + j * T, row = i / (D / 8), d = i % (D / 8) * 8;
+        float x[8], top = 0.0f;
+        floats8(r.x[j], x);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            float y[8];
-            floats8(r.x[nb][i], y);
+        for (int u = 0; u < 8; ++u)
+            if (finite(x[u])) top = fmaxf(top, fabsf(x[u]));
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[i * 8 + u] = y[u];
-        }
-#pragma unroll
-        for (int i = 0; i < D / 4; ++i)
-            if (finite(x[i])) top = fmaxf(top, fabsf(x[i]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         // 2^e in two factors: each is a normal float, whatever the row's size (e from -162 to 114)
         int e = 0;
         if (top > 0.0f) e = ilogbf(top) - 13;
         const int e1 = e / 2, e2 = e - e1;
         const float m1 = __int_as_float((127 - e1) << 23), m2 = __int_as_float((127 - e2) << 23);
-        float rs = scale * (TWO ? 1.0f : kCodeUnit) * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
         float sum = 0.0f;
+        // features d .. d + 7 are two steps (four each) of lane (row % 8, d % 64 / 16); 0 and 2, 1 and 3 of four, as codes02
+        const int ks = d / 64 * 4 + d % 16 / 4, lane = row % 8 * 4 + d % 64 / 16;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
+        for (int k = 0; k < 2; ++k) {
+            uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {                  // features 0 and 2, 1 and 3 of four, as codes02 has them
-                const float y0 = x[ks * 4 + u] * m1 * m2, y1 = x[ks * 4 + u + 2] * m1 * m2;
+            for (int u = 0; u < 2; ++u) {
+                const float y0 = x[k * 4 + u] * m1 * m2, y1 = x[k * 4 + u + 2] * m1 * m2;
                 const __half2 h = __floats2half2_rn(y0, y1);
                 const float2 back = __half22float2(h);
-                f.hi[nb][ks][u] = half2_bits(h);
-                if constexpr (TWO)
-                    f.lo[nb][ks][u] = half2_bits(__floats2half2_rn(finite(y0) ? y0 - back.x : 0.0f, finite(y1) ? y1 - back.y : 0.0f));
+                hi[u] = half2_bits(h);
+                if constexpr (TWO) lo[u] = half2_bits(__floats2half2_rn(finite(y0) ? y0 - back.x : 0.0f, finite(y1) ? y1 - back.y : 0.0f));
                 else sum += back.x + back.y;
             }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= -128.0f / kCodeUnit;
+            if (row < 8 * NB) {
+                f.hi[row / 8][ks + k][lane] = make_uint2(hi[0], hi[1]);
+                if constexpr (TWO) f.lo[row / 8][ks + k][lane] = make_uint2(lo[0], lo[1]);
+            }
+        }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f.rs[nb][u] = __shfl_sync(0xffffffffu, rs, 8 * t + 4 * u);
-            f.s0[nb][u] = TWO ? 0.0f : __shfl_sync(0xffffffffu, sum, 8 * t + 4 * u);
+        for (int o = 1; o < D / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (d == 0 && row < 8 * NB) {
+            f.rs[row] = scale * (TWO ? 1.0f : kCodeUnit) * __int_as_float((127 + e1) << 23) * __int_as_float((127 + e2) << 23);
+            f.s0[row] = TWO ? 0.0f : sum * (-128.0f / kCodeUnit);
         }
     }
 }
@@ -425,7 +423,7 @@ __device__ __forceinline__ void page_scores(const QFrag<D, NB, TWO>& f, const in
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[mt][nb][i] = f.s0[nb][i & 1];
+            for (int i = 0; i < 4; ++i) s[mt][nb][i] = f.s0[8 * nb + 2 * t + (i & 1)];
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
         load_fence();
@@ -439,18 +437,25 @@ __device__ __forceinline__ void page_scores(const QFrag<D, NB, TWO>& f, const in
             }
         // the key tiles' products side by side: sums that do not wait for one another
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            const int ks = c * 4 + i, lane = threadIdx.x & 31;
+            uint2 q[NB], q2[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                q[nb] = f.hi[nb][ks][lane];
+                if constexpr (TWO) q2[nb] = f.lo[nb][ks][lane];
+            }
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
                 const uint32_t a0 = codes02<!TWO>(w[mt][0][i]), a2 = codes02<!TWO>(w[mt][0][i] >> 8);
                 const uint32_t a1 = codes02<!TWO>(w[mt][1][i]), a3 = codes02<!TWO>(w[mt][1][i] >> 8);
-                const int ks = c * 4 + i;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    mma16816(s[mt][nb], a0, a1, a2, a3, f.hi[nb][ks][0], f.hi[nb][ks][1]);
-                    if constexpr (TWO) mma16816(s[mt][nb], a0, a1, a2, a3, f.lo[nb][ks][0], f.lo[nb][ks][1]);
+                    mma16816(s[mt][nb], a0, a1, a2, a3, q[nb].x, q[nb].y);
+                    if constexpr (TWO) mma16816(s[mt][nb], a0, a1, a2, a3, q2[nb].x, q2[nb].y);
                 }
             }
+        }
     }
 }
 
@@ -477,13 +482,14 @@ __device__ __forceinline__ void st4(void* p, size_t i, float x, float y, float z
     }
 }
 
-template <int D, int NB>
+template <int D, int NB, bool TWO>
 struct AttSmem {
     union {
         int8_t ring[kAttWarps][kSlots][kPage * D];
         float acc[kAttWarps + 1][8 * NB][D];               // the warps' accumulators, then the tail's
         unsigned char tail[2][(kPage - 1) * D * 4];        // the tail's keys and values
     };
+    QFrag<D, NB, TWO> f;
     float q[8 * NB][D];
     float sc[kPage][8 * NB];                               // the tail's scores, then its p: [key][row]
     float m[kAttWarps + 1][8 * NB], l[kAttWarps + 1][8 * NB];
@@ -552,7 +558,7 @@ template <int DT, int D, int NB>
 __device__ __noinline__ void attend_tail(const AttendArgs& a) {
     constexpr int ROWS = 8 * NB, TR = ROWS * D / (kAttWarps * 32);   // the rows in a thread, of one feature
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    AttSmem<D, NB>& sm = *reinterpret_cast<AttSmem<D, NB>*>(smem_raw);
+    AttSmem<D, NB, DT == F32>& sm = *reinterpret_cast<AttSmem<D, NB, DT == F32>*>(smem_raw);
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, L = sm.L, nrow = sm.nrow, b = sm.b, h = sm.h;
     float ot[TR];
@@ -627,7 +633,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
     constexpr int DG = D / 8, ROWS = 8 * NB;
     constexpr uint32_t TILE = kPage * D;
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    AttSmem<D, NB>& sm = *reinterpret_cast<AttSmem<D, NB>*>(smem_raw);
+    AttSmem<D, NB, DT == F32>& sm = *reinterpret_cast<AttSmem<D, NB, DT == F32>*>(smem_raw);
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.Hq / kv.heads;
@@ -705,16 +711,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                 vs = kv.vs[(size_t) id * kv.heads + h];
             }
         };
-        QFrag<D, NB, TWO> f;
         if (p0 < p1) {
-            QRows<DT, D, NB> rows;
-            long long qrow[NB];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) qrow[nb] = sm.qoff[8 * nb + g];
-            load_q(rows, a.q, qrow, a.q_vec);
+            QRows<DT, D, NB, kAttWarps * 32> rows;
+            load_q(rows, a.q, sm.qoff, a.q_vec);
             begin();
-            make_q(f, rows, a.scale_log2);
+            make_q(sm.f, rows, a.scale_log2);
         }
+        __syncthreads();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             m[nb][0] = m[nb][1] = -INFINITY;
@@ -726,11 +729,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
         }
         if (p0 < p1) {
             int pos[NB][2];
+            float rs[NB][2];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                pos[nb][0] = sm.pos[8 * nb + 2 * t];
-                pos[nb][1] = sm.pos[8 * nb + 2 * t + 1];
-            }
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    pos[nb][c] = sm.pos[8 * nb + 2 * t + c];
+                    rs[nb][c] = sm.f.rs[8 * nb + 2 * t + c];
+                }
             const int first_pos = sm.pos[0];
             while (true) {
                 auto arrived = [&]() {
@@ -747,7 +753,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                     const float kscale = __shfl_sync(0xffffffffu, ks, i), vscale = __shfl_sync(0xffffffffu, vs, i);
                     if (!arrived()) { used = issued; break; }
                     float sc[4][NB][4];
-                    page_scores<D, NB, TWO>(f, sm.ring[warp][used % kSlots], sc);
+                    page_scores<D, NB, TWO>(sm.f, sm.ring[warp][used % kSlots], sc);
                     __syncwarp();
                     ++used;
                     next();
@@ -759,7 +765,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                         float mu[2];
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float fs = kscale * f.rs[nb][c];
+                            const float fs = kscale * rs[nb][c];
                             float mx = -INFINITY;
 #pragma unroll
                             for (int mt = 0; mt < 4; ++mt)
@@ -1018,6 +1024,8 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_co
     constexpr int NB = 1, ROWS = 8;
     __shared__ __align__(16) float qs[ROWS][D];
     __shared__ __align__(16) float sc[kPage][ROWS];
+    __shared__ QFrag<D, NB, TWO> fr[kAttWarps];
+    __shared__ long long qoff[kAttWarps][ROWS];
     extern __shared__ __align__(16) unsigned char kt[];
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -1049,25 +1057,29 @@ __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_co
         // from the first row that sees slot 64 p on
         for (int r0 = max(0, p * kPage - (s.L - s.n)) * group / ROWS * ROWS; r0 < R; r0 += ROWS) {
             int pos, pos2[2];
-            long long off[1];
+            long long off;
             float lse, lse2[2];
-            place(r0 + g, pos, off[0], lse);
+            place(r0 + g, pos, off, lse);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 pos2[c] = __shfl_sync(0xffffffffu, pos, 8 * t + 4 * c);
                 lse2[c] = __shfl_sync(0xffffffffu, lse, 8 * t + 4 * c);
             }
-            QRows<DT, D, NB> rows;
-            QFrag<D, NB, TWO> f;
-            load_q(rows, a.q, off, a.q_vec);
+            __syncwarp();                                  // the rows before have been read
+            if (t == 0) qoff[warp][g] = off;
+            __syncwarp();
+            QRows<DT, D, NB, 32> rows;
+            load_q(rows, a.q, qoff[warp], a.q_vec);
+            QFrag<D, NB, TWO>& f = fr[warp];
             make_q(f, rows, a.scale_log2);
+            __syncwarp();
             float x[4][NB][4];
             page_scores<D, NB, TWO>(f, kv.k + pb * kPage * D, x);
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = ex2(x[mt][0][i] * (ks * f.rs[0][i & 1]) - lse2[i & 1]);
+                    const float e = ex2(x[mt][0][i] * (ks * f.rs[2 * t + (i & 1)]) - lse2[i & 1]);
                     if (p * kPage + mt * 16 + (i >> 1) * 8 + g <= pos2[i & 1]) sum[mt][i >> 1] += e;
                 }
         }
@@ -1443,9 +1455,9 @@ cudaError_t allow_smem(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {
 template <int DT, int D, int NB>
 cudaError_t attend_nb(const AttendArgs& a, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
-    const cudaError_t e = allow_smem(ready, attend<DT, D, NB>, sizeof(AttSmem<D, NB>));
+    const cudaError_t e = allow_smem(ready, attend<DT, D, NB>, sizeof(AttSmem<D, NB, DT == F32>));
     if (e != cudaSuccess) return e;
-    attend<DT, D, NB><<<(unsigned) a.plan.grid, kAttWarps * 32, sizeof(AttSmem<D, NB>), st>>>(a);
+    attend<DT, D, NB><<<(unsigned) a.plan.grid, kAttWarps * 32, sizeof(AttSmem<D, NB, DT == F32>), st>>>(a);
     return cudaGetLastError();
 }
 
@@ -1461,7 +1473,10 @@ cudaError_t attend_dt(const AttendArgs& a, int n_sm, cudaStream_t st) {
     if (a.lse) {
         const long long units = (long long) kv.seqs * kv.heads;
         const int nzw = (int) std::max(1ll, std::min<long long>((kv.width + kAttWarps - 1) / kAttWarps, (n_sm * 4 + units - 1) / units));
-        e = launch_after(attend_weights<DT, D>, dim3((unsigned) (units * nzw)), kAttWarps * 32, (kPage - 1) * D * DtInfo<DT>::ES, st, a, nzw);
+        constexpr size_t tail = (kPage - 1) * D * DtInfo<DT>::ES;
+        static std::atomic<uint64_t> ready{0};
+        if ((e = allow_smem(ready, attend_weights<DT, D>, tail)) != cudaSuccess) return e;
+        e = launch_after(attend_weights<DT, D>, dim3((unsigned) (units * nzw)), kAttWarps * 32, tail, st, a, nzw);
     }
     return e;
 }

@@ -196,6 +196,24 @@ def test_attention(dtype, dim, heads, per, lens, news, cuda):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seqs", [1, 5, 40, 300])
+@pytest.mark.parametrize("heads,per", [(1, 4), (5, 2), (1, 9)])
+def test_attention_shares_of_many_sequences(dtype, seqs, heads, per, cuda):
+    """Sequences of all lengths in one call, several to a lane and to a CTA's share, some with nothing new, and one that is
+    much longer than the others."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 400, (seqs,), generator=g).tolist()
+    lens[seqs // 2] = 6000 if seqs <= 40 else 20000
+    news = [1 if b % 7 != 3 else 0 for b in range(seqs)]
+    news[seqs // 2] = 1
+    cache = _kv.random_cache(lens, heads, 64, dtype, cuda, seed=seqs + heads)
+    q = make_rows(sum(news), heads * per * 64, dtype, cuda, 48)
+    starts = _kv.starts_of(news, cuda)
+    out = run_attention(cache, q, heads * per, starts, cuda, max_new=1)
+    check_attention(cache, q, starts, out, heads * per)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("max_new,max_len", [(1, 1), (1, 100000), (40, 64), (1000, 1 << 40)])
 def test_attention_hints_only_divide_the_work(dtype, max_new, max_len, cuda):
     lens, news, heads, per, dim = [900, 333, 70], [40, 1, 70], 2, 3, 128
@@ -287,9 +305,10 @@ def test_attention_nan_and_infinite_queries_stay_in_their_rows(cuda):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("lens,news", [([1], [1]), ([64, 65, 0, 300], [1, 1, 0, 1]), ([200, 90], [50, 90])])
-def test_attention_weights(dtype, lens, news, cuda):
-    heads, per, dim = 2, 3, 64
+def test_attention_weights(dtype, dim, lens, news, cuda):
+    heads, per = 2, 3
     cache = _kv.random_cache(lens, heads, dim, dtype, cuda, seed=21, weights=True)
     q = make_rows(sum(news), heads * per * dim, dtype, cuda, 22)
     starts = _kv.starts_of(news, cuda)
