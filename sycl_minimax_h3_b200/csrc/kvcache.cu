@@ -1434,7 +1434,9 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     const int64_t room = (int64_t) n_sm * (p.rows == 8 ? 3 : 2), units = tiles * heads;
     p.nz = 1;
     p.joined = units <= 8 * room && 2 * (pages + kTailPages) >= 3 * kChunk;
-    p.room = p.joined ? (int) room : 0;
+    // five sixths of that: pieces are rounded up to whole ones, and those that then find no room run after all the others
+    // (48 sequences of 200 to 8,191 tokens: 88 us, all of it 94; one of 131,037: 51 and 53)
+    p.room = p.joined ? (int) (room * 5 / 6) : 0;
     p.grid = (int) std::min<int64_t>(units + p.room, 1 << 30);
     p.entries = p.joined ? (units + room) * p.rows : 0;
     return p;

@@ -15,17 +15,22 @@ import torch
 from .native import Context, H3Error, KVCacheStruct, dt_code
 
 _ctx: dict[tuple[int, int], Context] = {}
+# the handle of a device's current stream, without a stream object for every call where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def context(device=None) -> Context:
     """The h3s context of a device around PyTorch's current stream on it (made once per (device, stream))."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
-    s = torch.cuda.current_stream(index)
-    key = (index, int(s.cuda_stream))
-    if key not in _ctx:
+    if device is None:
+        index = torch.cuda.current_device()
+    else:
+        index = (device if isinstance(device, torch.device) else torch.device(device)).index or 0
+    key = (index, _raw_stream(index))
+    ctx = _ctx.get(key)
+    if ctx is None:
         with torch.cuda.device(index):
-            _ctx[key] = Context(s)
-    return _ctx[key]
+            ctx = _ctx[key] = Context(torch.cuda.current_stream())
+    return ctx
 
 
 @dataclass(frozen=True)
@@ -184,7 +189,7 @@ PAGE = 64  # tokens of a page
 
 def _part(t: torch.Tensor, what: str, dtype: torch.dtype, shape, device) -> int:
     """The address of a contiguous tensor of this type, shape and device."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise H3Error(f"{what}: contiguous {dtype} {list(shape)} on {device} expected, got {t.dtype} {list(t.shape)} on "
                       f"{t.device}")
     return t.data_ptr()
@@ -238,6 +243,8 @@ class KVCache:
             None if self.tail_weight is None else _part(self.tail_weight, "KVCache: tail_weight", f32, (seqs, heads, PAGE), dev),
             _part(self.table, "KVCache: table", i32, (seqs, width), dev), _part(self.lens, "KVCache: lens", i32, (seqs,), dev),
             pages, seqs, width, heads, dim, dt_code(dt))
+        object.__setattr__(self, "_sizes", (pages, heads, dim, seqs, width))
+        object.__setattr__(self, "_device", dev)
         object.__setattr__(self, "_struct", s)
         object.__setattr__(self, "_ptr", ctypes.addressof(s))
         object.__setattr__(self, "_work", {})
@@ -258,13 +265,13 @@ class KVCache:
                        torch.zeros(seqs, heads, PAGE, dtype=f32, **kw) if weights else None)
 
     def _rows(self, what: str, x: Rows) -> int:
-        if x.dim != self.k.shape[3] or x.t.dtype != self.tail_k.dtype or x.t.device != self.k.device:
+        if x.dim != self._sizes[2] or x.t.dtype != self.tail_k.dtype or x.t.device != self._device:
             raise H3Error(f"{what}: {x.t.dtype} rows with heads of {x.dim} on {x.t.device}, but the cache has {self.tail_k.dtype} "
                           f"and {self.k.shape[3]} on {self.k.device}")
         return x.ptr()
 
     def _starts(self, what: str, starts: torch.Tensor) -> int:
-        return _part(starts, f"{what}: starts", torch.int32, (self.table.shape[0] + 1,), self.k.device)
+        return _part(starts, what, torch.int32, (self._sizes[3] + 1,), self._device)
 
 
 def kv_append(cache: KVCache, k: Rows, v: Rows, starts: torch.Tensor, max_new: int | None = None) -> None:
@@ -273,11 +280,11 @@ def kv_append(cache: KVCache, k: Rows, v: Rows, starts: torch.Tensor, max_new: i
     stay in the tail as they are. ``max_new`` (about the most that one sequence gets) only divides the work."""
     if k.layout() != v.layout():
         raise H3Error("kv_append: k and v must have the same layout")
-    if k.heads != cache.k.shape[1]:
-        raise H3Error(f"kv_append: {k.heads} heads for a cache of {cache.k.shape[1]}")
-    kp, vp, sp = cache._rows("kv_append", k), cache._rows("kv_append", v), cache._starts("kv_append", starts)
-    _on_gpu(cache.k.device, "kv_append")
-    context(cache.k.device).kv_append(cache._ptr, kp, vp, k.tokens, k.stride, sp, max_new or 0)
+    if k.heads != cache._sizes[1]:
+        raise H3Error(f"kv_append: {k.heads} heads for a cache of {cache._sizes[1]}")
+    kp, vp, sp = cache._rows("kv_append", k), cache._rows("kv_append", v), cache._starts("kv_append: starts", starts)
+    _on_gpu(cache._device, "kv_append")
+    context(cache._device).kv_append(cache._ptr, kp, vp, k.tokens, k.stride, sp, max_new or 0)
 
 
 def attention_cached(q: Rows, cache: KVCache, starts: torch.Tensor, out: torch.Tensor, max_new: int | None = None,
@@ -287,7 +294,7 @@ def attention_cached(q: Rows, cache: KVCache, starts: torch.Tensor, out: torch.T
     nothing is 0; rows behind the last sequence are left as they were. ``accumulate`` adds the weight that every token
     receives to ``cache.weight``. ``max_new`` and ``max_len`` (about the most new tokens, and the longest sequence) only
     divide the work."""
-    heads, dim = cache.k.shape[1], cache.k.shape[3]
+    heads, dim = cache._sizes[1:3]
     if q.heads == 0 or q.heads % heads != 0:
         raise H3Error(f"attention_cached: {q.heads} query heads over {heads} key/value heads")
     if accumulate and cache.weight is None:
@@ -295,16 +302,16 @@ def attention_cached(q: Rows, cache: KVCache, starts: torch.Tensor, out: torch.T
     if out.dtype != q.t.dtype or out.numel() != q.tokens * q.heads * dim or not out.is_contiguous() or out.device != q.t.device:
         raise H3Error(f"attention_cached: out {list(out.shape)} {out.dtype} for {q.tokens} tokens of {q.heads} x {dim} in "
                       f"{q.t.dtype}")
-    qp, sp = cache._rows("attention_cached", q), cache._starts("attention_cached", starts)
-    _on_gpu(cache.k.device, "attention_cached")
-    ctx = context(cache.k.device)
+    qp, sp = cache._rows("attention_cached", q), cache._starts("attention_cached: starts", starts)
+    _on_gpu(cache._device, "attention_cached")
+    ctx = context(cache._device)
     key = (q.tokens, q.heads, max_new, max_len, accumulate)
     nbytes = cache._work.get(key)
     if nbytes is None:
         if len(cache._work) >= 256:
             cache._work.clear()
         nbytes = cache._work[key] = ctx.attention_cached_work(cache._ptr, q.tokens, q.heads, max_new or 0, max_len or 0, accumulate)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=cache.k.device) if nbytes else None
+    work = torch.empty(nbytes, dtype=torch.uint8, device=cache._device) if nbytes else None
     ctx.attention_cached(cache._ptr, qp, q.tokens, q.heads, q.stride, sp, max_new or 0, max_len or 0, out.data_ptr(),
                          int(accumulate), work.data_ptr() if nbytes else 0, nbytes)
 
