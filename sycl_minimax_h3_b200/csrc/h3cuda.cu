@@ -1281,7 +1281,7 @@ int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, co
     if (!check_dt(x_dt) || !check_dt(s_dt) || !check_dt(out_dt)) return kv_fail(who, "unknown element type");
     if (!x || !tiles || !scale || !out) return kv_fail(who, "a null pointer");
     if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
-    if (N > INT32_MAX - 16 || K > (1 << 30) || M > 65535ll * 64) return kv_fail(who, "too large");
+    if (N > INT32_MAX - 16 || K > (1 << 30) || M > 65535ll * 32) return kv_fail(who, "too large");
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     Int4Args a{};
@@ -1299,6 +1299,8 @@ int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, co
     a.s_dt = s_dt;
     a.out_dt = out_dt;
     a.x_vec = aligned16(x) && (K * esize(x_dt)) % 16 == 0;
+    a.err = c.err;
+    a.wait_ns = c.wait_ns;
     const cudaError_t e = launch_int4_linear(a, c.n_sm, c.st);
     return e == cudaSuccess ? 0 : cuda_fail(who, e);
 }

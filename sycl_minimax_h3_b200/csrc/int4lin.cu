@@ -25,6 +25,7 @@ namespace h3 {
 namespace {
 
 constexpr int kI4Warps = 8;
+constexpr int kErrInt4 = 128;          // a wait of the 4-bit layer's kernel gave up
 
 template <int XT>
 __device__ __forceinline__ void mma_x(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, DT == F32 ? 2 : 3) int4_few(con
     }
 }
 
-// ---- more rows -------------------------------------------------------------------------------------------------------
+// ---- 9 to 16 rows, and any number of rows of float32 -------------------------------------------------------------------------------------------------------
 // 128 outputs x up to 64 rows per CTA: a warp has 16 outputs and every row, so that a tile is unpacked once for all of
 // them; x comes through a ring in shared memory, 128 inputs at a time, of which warps 0-7 take the first 64 and warps
 // 8-15 the others. A cluster of `split` CTAs divides the inputs. The sums meet in shared memory, always in one order.
@@ -473,6 +474,8 @@ __global__ void __launch_bounds__(kRowsThreads) int4_rows(const __grid_constant_
     }
 }
 
+#include "int4tc.cuh"
+
 // codes [N, K / 2], two to a byte, the even input in the low four bits -> tiles
 __global__ void int4_pack(const uint8_t* __restrict__ codes, long long N, long long K, uint32_t* __restrict__ tiles) {
     const long long KT = (K + 63) / 64, words = (N + 15) / 16 * KT * 128;
@@ -496,28 +499,24 @@ __global__ void int4_pack(const uint8_t* __restrict__ codes, long long N, long l
 
 }  // namespace
 
-template <int DT, bool ZERO, bool G32, int MT>
-cudaError_t rows_mt(const Int4Args& a, int n_sm, cudaStream_t st) {
-    constexpr int TERMS = DT == F32 ? 3 : 1;
-    static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
+template <typename F>
+cudaError_t allow(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {   // a bit per device: the attribute belongs to a device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (!(ready.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(int4_rows<DT, ZERO, G32, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) sizeof(RowsSmem<TERMS>));
-        if (e != cudaSuccess) return e;
-        ready.fetch_or(bit, std::memory_order_relaxed);
-    }
-    const int blocks = (a.N + kRowsN - 1) / kRowsN, KP = (a.K + 127) / 128;
-    const long long chunks = (a.M + 8 * MT - 1) / (8 * MT);
-    // as many CTAs as there are SMs, or half again as many; a part of the inputs has at least two stages
-    int split = 1;
-    while (split < 8 && blocks * chunks * split * 2 <= n_sm + n_sm / 2 && KP / (split * 2) >= 2) split *= 2;
+    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+template <typename... A>
+cudaError_t in_clusters(void (*kernel)(A..., int), int blocks, long long chunks, int split, int threads, size_t smem,
+                        cudaStream_t st, const A&... a) {
     cudaLaunchConfig_t c{};
     c.gridDim = dim3((unsigned) (blocks * split), (unsigned) chunks);
-    c.blockDim = dim3(kRowsThreads);
-    c.dynamicSmemBytes = sizeof(RowsSmem<TERMS>);
+    c.blockDim = dim3((unsigned) threads);
+    c.dynamicSmemBytes = smem;
     c.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -525,7 +524,46 @@ cudaError_t rows_mt(const Int4Args& a, int n_sm, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, int4_rows<DT, ZERO, G32, MT>, a, split);
+    return cudaLaunchKernelEx(&c, kernel, a..., split);
+}
+
+template <int DT, bool ZERO, bool G32, int MT>
+cudaError_t rows_mt(const Int4Args& a, int n_sm, cudaStream_t st) {
+    constexpr int TERMS = DT == F32 ? 3 : 1;
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = allow(ready, int4_rows<DT, ZERO, G32, MT>, sizeof(RowsSmem<TERMS>));
+    if (e != cudaSuccess) return e;
+    const int blocks = (a.N + kRowsN - 1) / kRowsN, KP = (a.K + 127) / 128;
+    const long long chunks = (a.M + 8 * MT - 1) / (8 * MT);
+    // as many CTAs as there are SMs, or half again as many; a part of the inputs has at least two stages
+    int split = 1;
+    while (split < 8 && blocks * chunks * split * 2 <= n_sm + n_sm / 2 && KP / (split * 2) >= 2) split *= 2;
+    return in_clusters<Int4Args>(int4_rows<DT, ZERO, G32, MT>, blocks, chunks, split, kRowsThreads, sizeof(RowsSmem<TERMS>), st, a);
+}
+
+template <int DT, bool ZERO, int US, int NC>
+cudaError_t tc_nc(const Int4Args& a, int n_sm, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    constexpr size_t bytes = sizeof(TcSmem) + 1024;
+    const cudaError_t e = allow(ready, int4_tc<DT, ZERO, US, NC>, bytes);
+    if (e != cudaSuccess) return e;
+    const int blocks = (a.N + 127) / 128, KT = (a.K + 63) / 64;
+    const long long chunks = (a.M + 32 * NC - 1) / (32 * NC);
+    // a CTA per SM, as far as a part of the inputs has at least four stages
+    int split = 1;
+    while (split < 8 && blocks * chunks * split * 2 <= n_sm && KT / (split * 2) >= 4) split *= 2;
+    CUtensorMap tx{};
+    if (a.x_vec) {                                         // x as [M, K]: boxes of 64 inputs x ROWS rows, 128-byte swizzle
+        auto enc = tensor_map_encoder();
+        if (!enc) return cudaErrorNotSupported;
+        const cuuint64_t dims[2] = {(cuuint64_t) a.K, (cuuint64_t) a.M}, strides[1] = {(cuuint64_t) a.K * 2};
+        const cuuint32_t box[2] = {64, 32 * NC}, steps[2] = {1, 1};
+        if (enc(&tx, DT == F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.x), dims, strides,
+                box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
+    return in_clusters<Int4Args, CUtensorMap>(int4_tc<DT, ZERO, US, NC>, blocks, chunks, split, kTcThreads, bytes, st, a, tx);
 }
 
 template <int DT, int SDT, bool ZERO, bool G32>
@@ -545,10 +583,19 @@ cudaError_t int4_dt(const Int4Args& a, int n_sm, cudaStream_t st) {
             default: return few_s<DT, F32, ZERO, G32>(a, n_sm, st);
         }
     }
+    // up to 16 rows of a 16-bit type mma.sync is the quicker, its stages being shorter: 4096 outputs of 4096 inputs 9.6 us
+    // against 11.6 (12288 of 4096: 28.4 against 26.2); at 17 rows 11.8 against 11.7, at 32 of 12288 34.6 against 26.6
     if (a.M <= 16) return rows_mt<DT, ZERO, G32, 2>(a, n_sm, st);
-    if (a.M <= 32) return rows_mt<DT, ZERO, G32, 4>(a, n_sm, st);
-    if (a.M <= 48) return rows_mt<DT, ZERO, G32, 6>(a, n_sm, st);
-    return rows_mt<DT, ZERO, G32, 8>(a, n_sm, st);
+    if constexpr (DT == F32) {
+        if (a.M <= 32) return rows_mt<DT, ZERO, G32, 4>(a, n_sm, st);
+        if (a.M <= 48) return rows_mt<DT, ZERO, G32, 6>(a, n_sm, st);
+        return rows_mt<DT, ZERO, G32, 8>(a, n_sm, st);
+    } else {
+        // 4, 2 or 1 units in a stage
+        if constexpr (G32) return a.M <= 32 ? tc_nc<DT, ZERO, 2, 1>(a, n_sm, st) : tc_nc<DT, ZERO, 2, 2>(a, n_sm, st);
+        else if (a.group_shift == 6) return a.M <= 32 ? tc_nc<DT, ZERO, 1, 1>(a, n_sm, st) : tc_nc<DT, ZERO, 1, 2>(a, n_sm, st);
+        else return a.M <= 32 ? tc_nc<DT, ZERO, 0, 1>(a, n_sm, st) : tc_nc<DT, ZERO, 0, 2>(a, n_sm, st);
+    }
 }
 
 template <int DT>

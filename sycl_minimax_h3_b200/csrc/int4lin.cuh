@@ -20,6 +20,8 @@ struct Int4Args {
     int N, K, group_shift;             // groups of 2^group_shift inputs: 5 to 7, or 30 (one scale for each output)
     int x_dt, s_dt, out_dt;
     int x_vec;                         // 16-byte loads of x's rows allowed
+    int* err;                          // device error word of waits that gave up
+    unsigned long long wait_ns;        // limit of every wait
 };
 cudaError_t launch_int4_linear(const Int4Args& a, int n_sm, cudaStream_t st);
 cudaError_t launch_int4_pack(const uint8_t* codes, long long N, long long K, void* tiles, int n_sm, cudaStream_t st);

@@ -133,3 +133,30 @@ def test_refusals(cuda):
     assert call(M=0) == 0 and call(N=0) == 0 and call(K=0) == 0
     for kw, why in (({"group": 16}, "groups"), ({"x_dt": 3}, "type"), ({"t": 8}, "16 bytes"), ({"s": 0}, "null")):
         assert call(**kw) == -1 and why in native.last_error()
+
+
+@pytest.mark.parametrize("x_dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("group,zero", [(0, True), (32, True), (64, True), (128, True), (32, False), (128, False)])
+@pytest.mark.parametrize("M,N,K,shift", [(17, 130, 14336, 0), (40, 130, 1344, 0), (65, 257, 2112, 0), (129, 16, 62, 0), (64, 128, 1026, 0), (33, 140, 4096, 1)])
+def test_many_rows(x_dt, group, zero, M, N, K, shift, cuda):
+    """More stages than the rings have, parts that end inside a stage, rows past 32 and 64, x that cannot be copied by 16 bytes"""
+    codes, scale, z, b, x, lin = make(M, N, K, group, x_dt, torch.float32, zero, True, cuda, seed=M + K)
+    buf = torch.empty(M * K + shift, dtype=x_dt, device=cuda)
+    buf[shift:] = x.reshape(-1).to(cuda)
+    out = torch.full((M + 1, N), 7.0, dtype=torch.float32, device=cuda)
+    lin.forward(buf[shift:].view(M, K), out[:M])
+    ops.context(cuda).wait()
+    check(codes, scale, z, b, x, group, out[:M])
+    assert (out[M] == 7.0).all()
+
+
+def test_nan_and_infinity_stay_in_their_row_of_many(cuda):
+    codes, scale, z, b, x, lin = make(40, 150, 1024, 128, torch.bfloat16, torch.bfloat16, False, False, cuda, seed=5)
+    x[1, 7], x[33, 900] = float("nan"), float("inf")
+    out = torch.empty(40, 150, dtype=torch.float32, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    bad = ~torch.isfinite(out).all(1).cpu()
+    assert bad.nonzero().flatten().tolist() == [1, 33]
+    keep = [m for m in range(40) if m not in (1, 33)]
+    check(codes, scale, z, b, x[keep], 128, out[keep])
