@@ -218,8 +218,9 @@ int h3s_attention_sage_static(void* stream, const void* q, const void* k, const 
  * share through `table`; the tokens of a sequence that do not fill a page yet are in its tail, in the rows' own type dt.
  * Token (slot) s of sequence b, head h: s < 64 * (lens[b] / 64): page table[b, s / 64], value code * scale, in float;
  * else tail row s % 64. Which pages are free is the caller's to keep. A page id outside the pool, or lens / starts out
- * of range, is found by the kernels: that page counts as unseen (attention) or that sequence is left alone (the others),
- * and the next h3s_wait returns -1. All arrays are contiguous; k, v, tail_k and tail_v start on 16 bytes. */
+ * of range, is found by the kernels: that page counts as unseen (attention) or is not written (append), that sequence is
+ * left alone (eviction; lens and starts in all of them), and the next h3s_wait returns -1. Starts that run backwards may
+ * leave any row of out as it was. All arrays are contiguous; k, v, tail_k and tail_v start on 16 bytes. */
 typedef struct h3s_kv_cache {
     int8_t *k, *v;             /* [pages, heads, 64, dim] codes */
     float *k_scale, *v_scale;  /* [pages, heads] */
@@ -260,7 +261,8 @@ uint64_t h3s_attention_cached_work(void* ctx, const h3s_kv_cache* kv, int64_t T,
  * their order. They are quantised again, as h3s_kv_append does, into the pages spare [seqs, budget / 64], weights with
  * them; then the first budget / 64 entries of the sequence's table and of its row of spare change places, and lens[b] =
  * budget: the old pages are the next eviction's spare ones. Sequences up to the budget keep everything, spare included.
- * A spare page belongs to no sequence and is named once. work: 4 * seqs * heads * budget bytes. */
+ * A spare page belongs to no sequence and is named once, and so must an evicted sequence's old pages be: one that another
+ * table names too (a common prefix) would be written over by the next eviction. work: 4 * seqs * heads * budget bytes. */
 int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budget, int64_t sinks, int64_t recent,
                  void* work, uint64_t work_bytes);
 

@@ -1207,6 +1207,7 @@ static int check_attend(const char* who, const h3s_kv_cache* kv, int64_t T, int6
     if (check_kv(who, kv, accumulate != 0, a) != 0) return -1;
     if (Hq < 1 || Hq % kv->heads != 0) return kv_fail(who, "the query heads must be a multiple of the cache's heads");
     if (Hq > INT32_MAX - 16 || (T > 0 && T > (INT32_MAX - 16) / Hq)) return kv_fail(who, "too many rows");
+    if (T * Hq / 8 + kv->seqs * kv->heads > 1 << 30) return kv_fail(who, "too many sequences");   // tiles of a launch
     return 0;
 }
 

@@ -947,6 +947,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
     int2 pieces_of = make_int2(0, a.plan.nz);              // this sequence's first piece, the pieces of a unit
     if (rows != 256) pieces_of = reinterpret_cast<const int2*>(mls + (size_t) a.plan.entries * 2)[b];
     if (pieces_of.y <= 1) return;
+    // row starts that run backwards can stand for more pieces than the call has rows: the call has reported them, and what
+    // was not written is not followed
+    const long long units = (long long) ((s.n * group + rows - 1) / rows) * kv.heads;
+    if (rows != 256 && (pieces_of.x < 0 || pieces_of.x + units * pieces_of.y > a.plan.grid)) return;
     for (int i = blockIdx.y; i < s.n * a.Hq; i += gridDim.y) {
         const int tok = i / a.Hq, hq = i % a.Hq;
         const int R = s.n * group, row = tok * group + hq % group, tile = row / rows, r0 = tile * rows;
@@ -1423,7 +1427,7 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     // as many tiles as there can be, of all sequences together
     const int64_t tiles = T * group / p.rows + seqs;
     if (p.rows == 256) {
-        p.grid = (int) std::min<int64_t>(tiles, INT32_MAX / heads);
+        p.grid = (int) tiles;
         const int64_t units = seqs * heads * std::max<int64_t>(1, (rows + 255) / 256);
         p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({(pages + kMinPages - 1) / kMinPages, n_sm / units, 512}));
         p.joined = p.nz > 1;
@@ -1437,7 +1441,7 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     // five sixths of that: pieces are rounded up to whole ones, and those that then find no room run after all the others
     // (48 sequences of 200 to 8,191 tokens: 88 us, all of it 94; one of 131,037: 51 and 53)
     p.room = p.joined ? (int) (room * 5 / 6) : 0;
-    p.grid = (int) std::min<int64_t>(units + p.room, 1 << 30);
+    p.grid = (int) (units + p.room);                       // (the caller has seen to it that it is one)
     p.entries = p.joined ? (units + room) * p.rows : 0;
     return p;
 }

@@ -147,6 +147,14 @@ def test_c_refusals():
         assert L.h3s_int4_linear(None, 16, 0, M, K, 16, N, 16, None, 0, 32, None, 16, 0) == 0
 
 
+def test_c_refuses_more_tiles_than_a_launch_has():
+    L = native.lib()
+    keep, s = struct(seqs=1 << 28, heads=5)
+    p = ctypes.addressof(s)
+    assert L.h3s_attention_cached(None, p, 16, 4, 5, 5 * 64, 16, 0, 0, 16, 0, None, 0) == -1 and "too many sequences" in native.last_error()
+    assert L.h3s_attention_cached_work(None, p, 4, 5, 0, 0, 0) == 0
+
+
 def test_the_definitions_of_the_tests():
     """quantised(): ties to even, infinities saturate, NaN is 0; a cache reads back what was put into its tail."""
     codes, scale = _kv.quantised(torch.tensor([[127.0, 0.5, 1.5, -2.5, float("inf"), float("nan")]]))
