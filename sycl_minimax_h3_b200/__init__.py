@@ -8,7 +8,8 @@ The product is two C-ABI libraries built from ``csrc/`` into ``lib/``:
 
 This package is the Python host side over that ABI: ``native`` (ctypes bindings, fails loudly when the libraries are
 missing), ``ops`` (``Rows`` / ``attention`` / ``attention_batch``, the reference engine's operator interface from
-``engine/h3-core/src/ops.rs``) and ``ulysses`` (the sequence-parallel all-to-all over NCCL).
+``engine/h3-core/src/ops.rs``; beside it the text model's ``KVCache`` / ``kv_append`` / ``attention_cached`` / ``kv_evict``
+and ``Int4Linear``) and ``ulysses`` (the sequence-parallel all-to-all over NCCL).
 """
 from .native import H3Error, Context, lib, sage_lib, LIB_DIR  # noqa: F401
 

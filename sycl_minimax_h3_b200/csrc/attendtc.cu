@@ -17,6 +17,10 @@
 // the two halves of the key tiles, 14 and 15 those of the value tiles (16 codes per lane and load; the next half's loads
 // are under way while a half is unpacked). The 128 registers a thread that 512 threads start with are dealt out again: 168 to
 // the softmax warps, 120 to the unpacking ones, 56 to warps 0-3 (128 x (56 + 2 x 168 + 120) = 65,536).
+//
+// Measured: 1,999 tokens behind 15,002 cached ones, 32 heads of 128 over 8, fp16: 654 us, 524 GFLOP at 802 TFLOP/s (0.48 of the
+// measured dense rate). The tensor pipe is active 43 % of the time: 256 CTAs on 148 SMs are two rounds where 1.73 would do,
+// and within a CTA the softmax (an exponential per score, 16 a clock and SM) takes about as long as the products.
 #include <algorithm>
 #include <atomic>
 

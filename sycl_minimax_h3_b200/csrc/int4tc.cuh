@@ -8,14 +8,15 @@
 // in registers. Zero points enter as scale * (8 - zero) * the sum of x over the unit, which warps 9-11 take from the rows.
 // A stage's fence stands before the next loads: behind them it waits for their data (x by cp.async and fences: 40 us for
 // 48 rows, 4096 outputs of 14336 inputs; by tensor copies 27).
-// Measured: 48 x 14336 -> 4096 27 us (29 MB of codes, 209 TFLOP/s; mma.sync 35.5), 64 x 14336 -> 16384 81 us (117 MB, 370
-// TFLOP/s; mma.sync 146). What bounds it is the unpacking, seven logic and four floating-point instructions for eight codes
-// in eight warps that share their schedulers with the other roles, and the fixed 5 us of clusters, barriers and sums.
+// Measured, bf16, groups of 128: 48 x 14336 -> 4096 27 us (29 MB of codes, 209 TFLOP/s; mma.sync 35.5), groups of 64 29, of
+// 32 43; 64 x 14336 -> 16384 81 us (117 MB, 370 TFLOP/s; mma.sync 146). The roles wait for one another: the tensor pipe is
+// active 13 % and the schedulers issue 35 % of the time; unpacking eight codes is seven logic and four floating-point
+// instructions in eight warps, a wait that suspends resumes some hundred cycles late, and clusters, barriers and the sums at
+// the end are 5 us of every call.
 #pragma once
 
 constexpr int kTcThreads = 512, kTcStages = 4, kTcBufs = 4, kTcCols = 64;
-constexpr int kTcAhead = 3, kTcSums = 2 * kTcStages;       // x's stages in flight; stages whose sums of x are kept
-constexpr int kTcSpin = 0;                                // probes before a wait that suspends
+constexpr int kTcAhead = 3, kTcSums = 2 * kTcStages;       // stages from x's copy to its sums; stages whose sums are kept
 
 struct TcSmem {
     uint8_t a[kTcStages][2][128 * 128];                    // two blocks of 64 inputs
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) int4_tc(const __grid_constant__
     const uint32_t tmem = sm.tmem;
     static_assert(kTcBufs == kTcStages, "with a unit to a stage the unit's barrier frees the stage too");
     uint64_t* empty = US > 0 ? sm.empty : sm.d_full;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, a.wait_ns, abort, kTcSpin); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, a.wait_ns, abort); };
     bool ok = true;
     float acc[ROWS];
     if (warp < 8) {
@@ -122,29 +123,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) int4_tc(const __grid_constant__
     } else if (warp == 8) {
         // ---------------- products ----------------
         const uint64_t da = sdesc(smem_u32(sm.a[0][0]), 16, 1024), db = sdesc(smem_u32(sm.b[0][0]), 16, 1024);
-        for (int base = 0; base < n_it && ok; base += kTcStages) {
-            const uint32_t ph = (uint32_t) (base / kTcStages) & 1, first = base == 0;
+        uint32_t unit = 0;
+        for (int it = 0; it < n_it && ok; ++it) {
+            const int st = it % kTcStages;
+            const uint32_t ph = (uint32_t) (it / kTcStages) & 1;
+            ok = wait(sm.a_full + st, ph) && wait(sm.b_full + st, ph);
+            const uint64_t sa = da + (uint32_t) (st * 2048), sb = db + (uint32_t) (st * 1024);   // (they count in 16 bytes)
 #pragma unroll
-            for (int st = 0; st < kTcStages; ++st) {
-                if (base + st >= n_it || !ok) break;
-                ok = wait(sm.a_full + st, ph) && wait(sm.b_full + st, ph);
+            for (int u = 0; u < UNITS; ++u, ++unit) {
+                const uint32_t buf = unit % kTcBufs;
+                if (ok && unit >= kTcBufs) ok = wait(sm.d_empty + buf, ((unit / kTcBufs) & 1) ^ 1);
+                if (!ok) break;
+                tc_fence_after();
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
-                    constexpr int TURNS = UNITS * kTcStages / kTcBufs;      // a buffer's uses in kTcStages stages
-                    const int buf = (st * UNITS + u) % kTcBufs, turn = (st * UNITS + u) / kTcBufs;
-                    if (ok && !(first && turn == 0)) ok = wait(sm.d_empty + buf, (TURNS & 1 ? ph : 0) ^ (turn & 1) ^ 1);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int i = 0; i < STEPS; ++i) {      // 16 inputs of 2 bytes; descriptors count in 16 bytes
-                        const int kk = u * STEPS + i;
-                        mma_ss_w<false>(tmem + buf * kTcCols, da + (uint32_t) ((st * 2 + (kk >> 2)) * 1024 + (kk & 3) * 2),
-                                        db + (uint32_t) ((st * 2 + (kk >> 2)) * 512 + (kk & 3) * 2), IDESC, i > 0 ? 1u : 0u);
-                    }
-                    mma_commit_w(sm.d_full + buf);
+                for (int i = 0; i < STEPS; ++i) {          // 16 inputs of 2 bytes
+                    const int kk = u * STEPS + i;
+                    mma_ss_w<false>(tmem + buf * kTcCols, sa + (uint32_t) ((kk >> 2) * 1024 + (kk & 3) * 2),
+                                    sb + (uint32_t) ((kk >> 2) * 512 + (kk & 3) * 2), IDESC, i > 0 ? 1u : 0u);
                 }
-                if (US > 0 && ok) mma_commit_w(sm.empty + st);
+                mma_commit_w(sm.d_full + buf);
             }
+            if (US > 0 && ok) mma_commit_w(sm.empty + st);
         }
         mma_commit_w(&sm.done);                            // products in flight, also where a wait gave up
         warp_wait(&sm.done, 0, a.wait_ns, nullptr);

@@ -72,6 +72,10 @@ __device__ __forceinline__ T block_max(T x, T* red) {     // over 256 threads; e
 // neither counts for a.
 // One CTA per (sequence, head), block, and K or V. The CTA of the sequence's first block reads the old tail and, after
 // that, writes the new one: the two share slots.
+// A block's rows are read once, into registers (16 KB a CTA of 256 threads, four to an SM), since the maximum comes before
+// the codes; what bounds a prompt is the issue of the conversions (maximum, product, rounding check, packing), about as much
+// as the loads: three prompts of 700 to 4,133 tokens, 8 heads of 128 in fp16, 58 MB, 27 us (2.2 TB/s; the bytes alone 9). A
+// step of 48 single tokens is 8 us: one launch and three loads that follow from one another (start, length, page).
 constexpr int kAppThreads = 256;
 
 template <int DT, int D>
@@ -182,6 +186,12 @@ __global__ void __launch_bounds__(kAppThreads, DT == F32 ? 3 : 4) kv_append(cons
 // Nothing is ordered inside a row's features: lane (g, t) of a warp reads 16-byte pieces of K (key g, features 16 t..),
 // and the query's fragment uses the same order. For P.V it reads features D/8 g.. of four keys, and accumulators
 // [i][..][e] of a lane are feature D/8 g + 2 i + e / 2 of query 2 t + e % 2.
+//
+// Four warps per CTA take the pages of a piece in turn, each with a ring of two 8 KB tiles of its own that bulk copies fill:
+// no warp waits for another before the end. What bounds it, by lengths (bf16, 8 heads of 128, 4 queries each): 48 sequences
+// of 2,048 tokens 41 us (4.9 TB/s of codes; the bytes alone 31), of 200 to 8,191 88 us (4.9 TB/s; 66: pieces are whole pages and
+// their ends leave SMs idle), one of 131,037 51 us (5.3 TB/s; 41); one of 64 to 4,096 tokens 6 to 10 us, which are the
+// loads that follow from one another: start and length, page id, codes, scale, and the joining launch.
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -931,7 +941,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
     }
 }
 
-// The splits' partial results of a row as one: a CTA per row, whose warps take the splits in turn and then meet.
+// The splits' partial results of a row as one: a CTA per row, whose warps take the splits in turn and then meet. The
+// partial results lie in L2; a launch that is ready when the pieces end makes it 2 to 3 us.
 constexpr int kJoinWarps = 8;
 template <int DT, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_constant__ AttendArgs a) {
@@ -1022,6 +1033,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
 
 // weight[slot] += the sum over the group's query rows of p = 2^(s - lse): the scores once more, against the finished
 // sums. One CTA per (sequence, kv head, piece of the pages), the last piece also the tail; a page's sums stay in one warp.
+// Reading the keys again costs less than keeping every score of the first pass would. 16 sequences of 100 to 4,500 tokens,
+// 2 heads of 64 with 8 queries each in float32: 13 us beside the attention's 14 and 6, all three bound by their first loads.
 template <int DT, int D>
 __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_constant__ AttendArgs a, int nzw) {
     constexpr bool TWO = DT == F32;
@@ -1148,7 +1161,8 @@ constexpr int kSelKeys = 48 * 1024;    // keys that fit shared memory; those of 
 // kept[..][0] = kLeftAlone where the sequence is left alone. One CTA per
 // (sequence, head). The weights' keys are read once into shared memory; the key of the last kept one is found by four
 // passes over 8 bits of them each; then every thread counts the kept ones in a run of slots of its own, one scan over
-// the threads gives the places, and the runs are written down.
+// the threads gives the places, and the runs are written down. Few CTAs with scans in a row bound it: 18 us for 12 sequences
+// of 3,500 to 8,111 tokens and 8 heads.
 __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ KvArgs kv, const int* __restrict__ spare,
                                                             int budget, int sinks, int recent, int* __restrict__ kept, int room) {
     extern __shared__ uint32_t keys[];
@@ -1285,6 +1299,9 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
 
 // 64 kept tokens of a (sequence, head) into one spare page, K and V side by side so that their loads are under way
 // together. TAIL: some of them lie in the tail (a sequence's last page or two).
+// A kept token's row is 128 bytes anywhere in the old pages: loads of that size, and the two passes over them in registers
+// (values and maximum, then codes), bound it: 12 sequences cut to 4,096 tokens, 8 heads of 128, 188 MB in 89 us (2.1 TB/s; the
+// bytes alone 29). Both passes take the codes exactly, code x scale in 64 bits where 32 are not sure of the rounding.
 template <int DT, int D, bool TAIL>
 __device__ __forceinline__ void gather_page(const KvArgs& kv, int h, size_t tbase, int page, const int* loc) {
     constexpr int C8 = D / 8, PER = 64 * C8 / 256;

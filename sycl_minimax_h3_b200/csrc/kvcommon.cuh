@@ -101,7 +101,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466
 struct Pieces {
     int np, cz, nu, tail_at;           // nu pieces; the tail is read by piece tail_at (-1: not seen)
 };
-constexpr int kMinPages = 4;           // a split has at least a page per warp
+constexpr int kMinPages = 4;           // a piece has at least a page for each of attend's warps, two key tiles of attend_tc's
 __device__ __forceinline__ Pieces pieces(int L, int last_pos, int nz) {
     Pieces p;
     const int seen = min(L, last_pos + 1), full = L / kPage;
