@@ -1238,6 +1238,9 @@ int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64
     a.T = T;
     a.qs = qs;
     a.Hq = (int) Hq;
+    auto shift = [](int64_t x) { int n = 0; while ((1ll << n) < x) ++n; return (1ll << n) == x ? n : -1; };
+    a.group_shift = shift(Hq / kv->heads);
+    a.head_shift = shift(kv->heads);
     a.starts = starts;
     a.out = out;
     a.lse = accumulate ? static_cast<float*>(work) : nullptr;

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "kvcache.cuh"
@@ -190,8 +191,8 @@ __global__ void __launch_bounds__(kAppThreads, DT == F32 ? 3 : 4) kv_append(cons
 // Four warps per CTA take the pages of a piece in turn, each with a ring of two 8 KB tiles of its own that bulk copies fill:
 // no warp waits for another before the end. What bounds it, by lengths (bf16, 8 heads of 128, 4 queries each): 48 sequences
 // of 2,048 tokens 41 us (4.9 TB/s of codes; the bytes alone 31), of 200 to 8,191 88 us (4.9 TB/s; 66: pieces are whole pages and
-// their ends leave SMs idle), one of 131,037 51 us (5.3 TB/s; 41); one of 64 to 4,096 tokens 6 to 10 us, which are the
-// loads that follow from one another: start and length, page id, codes, scale, and the joining launch.
+// their ends leave SMs idle), one of 131,037 51 us (5.3 TB/s; 41); one of 64 to 4,096 tokens 6 to 10 us (77: 8.1), which
+// are the loads that follow from one another, start and length, page id, codes and scale, tail, and the joining launch.
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -233,7 +234,7 @@ constexpr int kAttWarps = 4;
 // sequences are a warp's, a lane each, and every warp finds the piece for itself; more are the 128 threads' together.
 constexpr int kTailPages = 2, kChunk = 6;
 struct Piece {
-    int b, unit, z, nz;                // b < 0: there are no more
+    int b, tile, h, z, nz;             // b < 0: there are no more
     Seq s;
 };
 __device__ __forceinline__ int pieces_of_unit(int length, int chunk) { return max(1, (2 * length + chunk) / (2 * chunk)); }   // rounded
@@ -275,7 +276,7 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
         }
         const int from = upto - units * nz;
         const uint32_t here = __ballot_sync(0xffffffffu, flat >= from && flat < upto);
-        Piece p{-1, 0, 0, 1, s};
+        Piece p{-1, 0, 0, 0, 1, s};
         if (here == 0) return p;
         const int i = __ffs((int) here) - 1, at = flat - __shfl_sync(0xffffffffu, from, i);
         p.nz = __shfl_sync(0xffffffffu, nz, i);
@@ -287,9 +288,10 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
         p.s.L = __shfl_sync(0xffffffffu, s.L, i);
         p.s.ok = true;
         // the heads side by side: they lie side by side in a page, and are read at about the same time
-        const int zt = at / kv.heads;
-        p.unit = zt / p.nz * kv.heads + at % kv.heads;
-        p.z = zt % p.nz;
+        const int zt = quotient(at, kv.heads, a.head_shift);
+        p.h = at - zt * kv.heads;
+        p.tile = p.nz == 1 ? zt : zt / p.nz;
+        p.z = zt - p.tile * p.nz;
         return p;
     }
     int length0 = 0, units0 = units_of((int) threadIdx.x, length0);      // the first 128 sequences' are kept
@@ -333,16 +335,17 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
         if (flat >= from && flat < from + n) {
             found[0] = b0 + (int) threadIdx.x;
             const int i = flat - from, h = i % kv.heads, zt = i / kv.heads;
-            found[1] = zt / nz * kv.heads + h;
+            found[1] = zt / nz;
             found[2] = zt % nz;
             found[3] = nz;
+            found[4] = h;
             if (a.plan.joined && flat == from)
                 reinterpret_cast<int2*>(a.part + (size_t) a.plan.entries * (kv.dim + 2))[found[0]] = make_int2(from, nz);
         }
         before += sum;
     }
     __syncthreads();
-    Piece p{found[0], found[1], found[2], found[3], {0, 0, 0, false}};
+    Piece p{found[0], found[1], found[4], found[2], found[3], {0, 0, 0, false}};
     if (p.b >= 0) p.s = load_seq(kv, a.starts, a.T, p.b);
     return p;
 }
@@ -529,6 +532,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // Scores of the tail's keys in plain 32-bit arithmetic, sc[key][row] in log2 units: qf [rows][D] as floats, kt the tail's
 // rows in dt (shared memory). 128 threads, each a key and half of the rows; a thread starts at the 16-byte piece that its
 // key's number names, so that neighbouring keys, whose rows start in the same banks, read different ones.
+// No branch per row: with one, every load was waited for, and 13 keys of 4 rows took 1.8 us, now 0.7.
 template <int DT, int D, int ROWS>
 __device__ __forceinline__ void tail_scores(const float (*qf)[D], const unsigned char* kt, int nrow, int nkey, float scale,
                                             float (*sc)[ROWS]) {
@@ -536,30 +540,34 @@ __device__ __forceinline__ void tail_scores(const float (*qf)[D], const unsigned
     const int key = threadIdx.x & 63, half = threadIdx.x >> 6, per = (nrow + 1) / 2;
     const int r0 = half * per, r1 = min(nrow, r0 + per);
     if (key >= nkey) return;
-    float acc[ROWS / 2];
+    // rows past the last are computed from what lies there, and not stored
+    auto rows = [&](auto count) {
+        constexpr int R = decltype(count)::value;
+        float acc[R];
 #pragma unroll
-    for (int r = 0; r < ROWS / 2; ++r) acc[r] = 0.0f;
+        for (int r = 0; r < R; ++r) acc[r] = 0.0f;
 #pragma unroll 4
-    for (int i = 0; i < N; ++i) {
-        const int d = (i + key) % N * E;
-        float x[E];
-        cvt16<DT>(*reinterpret_cast<const uint4*>(kt + (key * D + d) * DtInfo<DT>::ES), x);
+        for (int i = 0; i < N; ++i) {
+            const int d = (i + key) % N * E;
+            float x[E];
+            cvt16<DT>(*reinterpret_cast<const uint4*>(kt + (key * D + d) * DtInfo<DT>::ES), x);
 #pragma unroll
-        for (int r = 0; r < ROWS / 2; ++r) {
-            if (r0 + r >= r1) break;
+            for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int u = 0; u < E; u += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(&qf[r0 + r][d + u]);
-                acc[r] = fmaf(y.x, x[u], acc[r]);
-                acc[r] = fmaf(y.y, x[u + 1], acc[r]);
-                acc[r] = fmaf(y.z, x[u + 2], acc[r]);
-                acc[r] = fmaf(y.w, x[u + 3], acc[r]);
-            }
+                for (int u = 0; u < E; u += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(&qf[r0 + r][d + u]);
+                    acc[r] = fmaf(y.x, x[u], acc[r]);
+                    acc[r] = fmaf(y.y, x[u + 1], acc[r]);
+                    acc[r] = fmaf(y.z, x[u + 2], acc[r]);
+                    acc[r] = fmaf(y.w, x[u + 3], acc[r]);
+                }
         }
-    }
 #pragma unroll
-    for (int r = 0; r < ROWS / 2; ++r)
-        if (r0 + r < r1) sc[key][r0 + r] = acc[r] * scale;
+        for (int r = 0; r < R; ++r)
+            if (r0 + r < r1) sc[key][r0 + r] = acc[r] * scale;
+    };
+    if (per <= 2) rows(std::integral_constant<int, 2>{});
+    else rows(std::integral_constant<int, ROWS / 2>{});
 }
 
 // The tail of the piece at hand as one more partial result, sm.acc[kAttWarps]: on CUDA cores, in 32 bits, since it is in
@@ -646,7 +654,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
     AttSmem<D, NB, DT == F32>& sm = *reinterpret_cast<AttSmem<D, NB, DT == F32>*>(smem_raw);
     const KvArgs& kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int group = a.Hq / kv.heads;
+    const int group = quotient(a.Hq, kv.heads, a.head_shift);
     let_next_launch();
     if (threadIdx.x == 0) {
         for (int w = 0; w < kAttWarps; ++w)
@@ -659,11 +667,11 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
     const Piece pcs = find_piece<ROWS>(a, flat, group, sm.scan);
     if (pcs.b < 0) return;
     {
-        const int b = pcs.b, nz = pcs.nz, z = pcs.z, h = pcs.unit % kv.heads, tile = pcs.unit / kv.heads;
+        const int b = pcs.b, nz = pcs.nz, z = pcs.z, h = pcs.h, tile = pcs.tile;
         const Seq s = pcs.s;
         const int R = s.n * group;
         const int r0 = tile * ROWS, nrow = min(R - r0, ROWS);
-        const int last_pos = s.L - s.n + (r0 + nrow - 1) / group;
+        const int last_pos = s.L - s.n + quotient(r0 + nrow - 1, group, a.group_shift);
         const Pieces pc = pieces(s.L, last_pos, nz);
         if (z >= max(pc.nu, 1)) return;
         __syncthreads();                                   // the barriers are made
@@ -678,7 +686,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
         if (threadIdx.x < ROWS) {
             const int r = threadIdx.x;
             const bool in = r < nrow;
-            const int tok = (r0 + r) / group, hq = h * group + (r0 + r) % group;
+            const int tok = quotient(r0 + r, group, a.group_shift), hq = h * group + r0 + r - tok * group;
             sm.pos[r] = in ? s.L - s.n + tok : -1;
             sm.row[r] = in ? (s.s0 + tok) * a.Hq + hq : -1;
             sm.qoff[r] = in ? (long long) (s.s0 + tok) * a.qs + hq * D : -1;
@@ -925,8 +933,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
             const size_t gr = (size_t) sm.row[r];
             if (whole) {
                 const bool none = sum == 0.0f;
-                st4<DT>(a.out, gr * D + d, none ? 0.0f : o.x / sum, none ? 0.0f : o.y / sum, none ? 0.0f : o.z / sum,
-                        none ? 0.0f : o.w / sum, a.out_vec);
+                const float inv = none ? 0.0f : 1.0f / sum;
+                st4<DT>(a.out, gr * D + d, none ? 0.0f : o.x * inv, none ? 0.0f : o.y * inv, none ? 0.0f : o.z * inv,
+                        none ? 0.0f : o.w * inv, a.out_vec);
                 if (a.lse && d == 0) a.lse[gr] = none ? INFINITY : mu + log2f(sum);
             } else {
                 const size_t at = (size_t) blockIdx.x * ROWS + r;

@@ -47,6 +47,7 @@ struct AttendArgs {
     const void* q;
     long long T, qs;                   // query rows, their stride (elements)
     int Hq;
+    int group_shift, head_shift;       // log2 of Hq / heads and of heads, or -1: a division is 100 cycles of a short step's start
     const int* starts;                 // [seqs + 1]
     void* out;                         // [T, Hq * dim]
     float* part;                       // [entries, dim] accumulators, [entries, 2] (max, sum), and an int2 per sequence: its

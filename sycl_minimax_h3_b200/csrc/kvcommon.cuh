@@ -43,6 +43,7 @@ __device__ __forceinline__ Seq load_seq(const KvArgs& kv, const int* starts, lon
     s.ok = s.s0 >= 0 && s1 >= s.s0 && s1 <= T && s.L >= 0 && s.L / kPage <= kv.width;
     return s;
 }
+__device__ __forceinline__ int quotient(int x, int d, int shift) { return shift >= 0 ? x >> shift : x / d; }   // x >= 0
 __device__ __forceinline__ bool page_ok(const KvArgs& kv, int page) { return page >= 0 && page < kv.pages; }
 
 template <int DT>
@@ -107,8 +108,8 @@ __device__ __forceinline__ Pieces pieces(int L, int last_pos, int nz) {
     const int seen = min(L, last_pos + 1), full = L / kPage;
     if (seen <= 0) { p.np = 0; p.cz = 1; p.nu = 0; p.tail_at = -1; return p; }
     p.np = min(full, (seen + kPage - 1) / kPage);
-    p.cz = max(kMinPages, (p.np + nz - 1) / nz);
-    const int nc = (p.np + p.cz - 1) / p.cz;
+    p.cz = max(kMinPages, nz == 1 ? p.np : (p.np + nz - 1) / nz);
+    const int nc = nz == 1 ? (p.np > 0) : (p.np + p.cz - 1) / p.cz;
     const bool tail = seen > full * kPage;
     p.nu = tail ? min(nc + 1, nz) : nc;
     p.tail_at = tail ? p.nu - 1 : -1;
