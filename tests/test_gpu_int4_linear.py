@@ -160,3 +160,32 @@ def test_nan_and_infinity_stay_in_their_row_of_many(cuda):
     assert bad.nonzero().flatten().tolist() == [1, 33]
     keep = [m for m in range(40) if m not in (1, 33)]
     check(codes, scale, z, b, x[keep], 128, out[keep])
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 1, 8), (64, 128, 56), (40, 20, 72), (200, 33, 200)])
+def test_many_rows_of_few_inputs(M, N, K, cuda):
+    """Fewer inputs than a box of x has"""
+    codes, scale, z, b, x, lin = make(M, N, K, 32, torch.float16, torch.float16, True, True, cuda, seed=M + K)
+    out = torch.empty(M, N, dtype=torch.float32, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    check(codes, scale, z, b, x, 32, out)
+
+
+@pytest.mark.parametrize("M", [4, 12, 40])
+def test_captured_calls_read_what_x_holds_at_the_replay(M, cuda):
+    codes, scale, z, b, x, lin = make(M, 300, 1024, 64, torch.bfloat16, torch.float32, True, True, cuda, seed=7)
+    held, out = torch.zeros(M, 1024, dtype=torch.bfloat16, device=cuda), torch.empty(M, 300, device=cuda)
+    stream, graph = torch.cuda.Stream(cuda), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        lin.forward(held, out)
+    for i in range(3):
+        xi = x.roll(i, 1)
+        held.copy_(xi)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(codes, scale, z, b, xi, 64, out)
+    eager = torch.empty_like(out)
+    lin.forward(held, eager)
+    ops.context(cuda).wait()
+    assert torch.equal(eager, out)
