@@ -17,6 +17,7 @@
 
 constexpr int kTcThreads = 512, kTcStages = 4, kTcBufs = 4, kTcCols = 64;
 constexpr int kTcAhead = 3, kTcSums = 2 * kTcStages;       // stages from x's copy to its sums; stages whose sums are kept
+static_assert(kTcAhead < kTcStages, "a stage's sums are taken before its refill waits for them");
 
 struct TcSmem {
     uint8_t a[kTcStages][2][128 * 128];                    // two blocks of 64 inputs
@@ -181,7 +182,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) int4_tc(const __grid_constant__
         int issued = 0;
         for (int nx = 0; nx < n_it + (ZERO ? kTcAhead : 0); ++nx) {
             if (nx < n_it) {
-                if (nx >= kTcStages && !wait(empty + nx % kTcStages, ((nx / kTcStages) & 1) ^ 1)) { ok = false; break; }
+                // A stage is free once its products are complete and its sums have been taken. A thread that stores x takes
+                // the sums of what it stored, earlier in this loop; one thread's copies write what all three warps read:
+                // that one waits for the sums of the stage that leaves (sx_full cannot run ahead of this warp, which is
+                // one of those that complete it). The other two follow by b_full alone, a phase of which waits for them.
+                const int leaves = nx - kTcStages;
+                if (leaves >= 0 && !(ZERO && a.x_vec && warp != 9)) {
+                    ok = wait(empty + nx % kTcStages, ((nx / kTcStages) & 1) ^ 1);
+                    if (ZERO && a.x_vec && ok) ok = wait(sm.sx_full + leaves % kTcSums, (leaves / kTcSums) & 1);
+                    if (!ok) break;
+                }
                 load(nx);
                 issued = nx + 1;
             }
