@@ -179,8 +179,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) int4_tc(const __grid_constant__
             fence_proxy_async_smem();
             mbar_arrive(bar);
         };
+        // Two warps have nothing to do where one thread's copies bring x and there are no sums to take: phases that nothing
+        // holds for them could pass unseen, and a wait for one of them would then last to its limit.
+        const int rounds = a.x_vec && !ZERO && warp != 9 ? 0 : n_it + (ZERO ? kTcAhead : 0);
         int issued = 0;
-        for (int nx = 0; nx < n_it + (ZERO ? kTcAhead : 0); ++nx) {
+        for (int nx = 0; nx < rounds; ++nx) {
             if (nx < n_it) {
                 // A stage is free once its products are complete and its sums have been taken. A thread that stores x takes
                 // the sums of what it stored, earlier in this loop; one thread's copies write what all three warps read:

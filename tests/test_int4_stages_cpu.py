@@ -1,7 +1,8 @@
 """The stages of the 4-bit layer's tcgen05 kernel (csrc/int4tc.cuh) as a model on the CPU: its roles, barriers and waits by
 parity, run in orders that no GPU promises to avoid: a role may be held back for as long as any other can go on. What is
 checked: nobody reads a stage of x, or the sums taken of it, that holds another stage's, and every wait ends. The model's
-earlier form (a refill that waits for the products alone) has to fail, or the model would see nothing."""
+earlier form (a refill that waits for the products alone, warps that wait for phases which nothing holds for them) has to
+fail, or the model would see nothing."""
 import random
 
 import pytest
@@ -151,7 +152,7 @@ def simulate(seed, units, zero, copies, n_it, gated=True, idle_leave=True):
     return True
 
 
-FORMS = [(units, zero, copies) for units in (1, 2, 4) for zero, copies in ((True, True), (True, False), (False, False))]
+FORMS = [(units, zero, copies) for units in (1, 2, 4) for zero in (False, True) for copies in (False, True)]
 
 
 @pytest.mark.parametrize("units,zero,copies", FORMS)
@@ -169,3 +170,8 @@ def test_the_model_sees_a_refill_that_does_not_wait_for_the_sums(units):
         except Wrong:
             stale += 1
     assert stale > 0
+
+
+@pytest.mark.parametrize("units", [1, 2, 4])
+def test_the_model_sees_waits_for_phases_that_nothing_holds(units):
+    assert not all(simulate(seed, units, False, True, 24, idle_leave=False) for seed in range(150))
