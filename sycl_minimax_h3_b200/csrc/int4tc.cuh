@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) int4_tc(const __grid_constant__
                 if (lane == 0) mbar_arrive(sm.sx_full + it % kTcSums);
             }
         }
-        if (a.x_vec)                                       // copies in flight
+        if (a.x_vec && warp == 9)                          // copies in flight, of the warp that made them
             for (int it = max(0, issued - kTcStages); it < issued; ++it) warp_wait(sm.b_full + it % kTcStages, (it / kTcStages) & 1, a.wait_ns, nullptr);
     } else {
         // ---------------- sums: output n of this thread, every row ----------------
