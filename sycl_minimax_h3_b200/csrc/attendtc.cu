@@ -534,42 +534,44 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
 #pragma unroll
             for (int c4 = 0; c4 < HD / 32; ++c4) {
                 uint32_t o[32];
+                __syncwarp();                          // the loads are the whole warp's; what follows is each row's own
                 tmem_ld32(t_lane + colO + c4 * 32, o);
                 tmem_wait_ld();
-                if (!live) continue;
-                float y[32];
+                if (live) {
+                    float y[32];
 #pragma unroll
-                for (int u = 0; u < 32; ++u) y[u] = l_run == 0.0f ? 0.0f : __uint_as_float(o[u]) * f;
-                if (added) {                           // the tail's infinities and NaN, where this row sees them
-                    for (int k = 0; k < min(nkey, pos + 1 - full * kPage); ++k)
+                    for (int u = 0; u < 32; ++u) y[u] = l_run == 0.0f ? 0.0f : __uint_as_float(o[u]) * f;
+                    if (added) {                           // the tail's infinities and NaN, where this row sees them
+                        for (int k = 0; k < min(nkey, pos + 1 - full * kPage); ++k)
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) {
-                            const float v = ld1<DT>(kv.tv, tbase + (size_t) k * HD + c4 * 32 + u);
-                            if (!finite(v)) y[u] += v;
-                        }
-                }
-                if (split) {
-                    float4* to = reinterpret_cast<float4*>(a.part + (gr * nz + z) * HD + c4 * 32);
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) to[u] = make_float4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
-                } else if (a.out_vec) {
-                    uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + (gr * HD + c4 * 32) * 2);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if constexpr (DT == F16) w[e] = pack_half2(y[8 * u + 2 * e], y[8 * u + 2 * e + 1]);
-                            else {
-                                const __nv_bfloat162 v = __floats2bfloat162_rn(y[8 * u + 2 * e], y[8 * u + 2 * e + 1]);
-                                w[e] = *reinterpret_cast<const uint32_t*>(&v);
+                            for (int u = 0; u < 32; ++u) {
+                                const float v = ld1<DT>(kv.tv, tbase + (size_t) k * HD + c4 * 32 + u);
+                                if (!finite(v)) y[u] += v;
                             }
-                        }
-                        to[u] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                } else {
+                    if (split) {
+                        float4* to = reinterpret_cast<float4*>(a.part + (gr * nz + z) * HD + c4 * 32);
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) st1<DT>(a.out, gr * HD + c4 * 32 + u, y[u]);
+                        for (int u = 0; u < 8; ++u) to[u] = make_float4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
+                    } else if (a.out_vec) {
+                        uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + (gr * HD + c4 * 32) * 2);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if constexpr (DT == F16) w[e] = pack_half2(y[8 * u + 2 * e], y[8 * u + 2 * e + 1]);
+                                else {
+                                    const __nv_bfloat162 v = __floats2bfloat162_rn(y[8 * u + 2 * e], y[8 * u + 2 * e + 1]);
+                                    w[e] = *reinterpret_cast<const uint32_t*>(&v);
+                                }
+                            }
+                            to[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) st1<DT>(a.out, gr * HD + c4 * 32 + u, y[u]);
+                    }
                 }
             }
             if (live && split) {

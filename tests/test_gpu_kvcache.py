@@ -574,3 +574,34 @@ def test_many_rows_hidden_slots_may_hold_anything(dtype, cuda):
     bad = torch.zeros(n, per, dtype=torch.bool, device=cuda)
     bad[90:] = bad[7, 0] = bad[8, 1] = True
     assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], was[~bad])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,per,L", [(75, 1, 75), (50, 3, 1500)])
+def test_many_rows_of_a_warp_that_see_unlike_tails(dtype, dim, n, per, L, cuda):
+    """A tile that ends inside a warp, and infinities in every 32 features of the tail that some rows of a warp see and others
+    do not: every feature of every row comes out as if it were alone. Once in one piece, once with the keys split."""
+    cache = _kv.random_cache([L], 1, dim, dtype, cuda, seed=49)
+    q = make_rows(n, per * dim, dtype, cuda, 50)
+    starts = _kv.starts_of([n], cuda)
+    clean = run_attention(cache, q, per, starts, cuda)
+    check_attention(cache, q, starts, clean, per)
+    tail = L % PAGE
+    want = clean.view(n, per, dim).clone()
+    for i in range(min(tail, n)):                  # tail row tail - 1 - i is seen by the last i + 1 tokens
+        if i % 3 == 0:
+            feature = (7 * i + 32 * (i // 3)) % dim
+            sign = float("inf") if i % 2 else -float("inf")
+            if cache.tail_v[0, 0, :tail, feature].isfinite().all():
+                cache.tail_v[0, 0, tail - 1 - i, feature] = sign
+                want[n - 1 - i:, :, feature] = sign
+    out = run_attention(cache, q, per, starts, cuda)
+    # what is finite: the tail's power of two may have moved with the values that became infinite
+    infinite = ~want.isfinite()
+    out = out.view(n, per, dim)
+    assert torch.equal(out[infinite], want[infinite])
+    cache.tail_v[0, 0, :tail][~cache.tail_v[0, 0, :tail].isfinite()] = 0
+    exact, _, bound = _kv.attention(cache, q, per, starts)
+    off = ((out.double().cpu() - exact.view(n, per, dim)).abs() - bound.view(n, per, dim))[~infinite.cpu()]
+    assert float(off.max()) <= 0, f"off by {float(off.max()):.3g} more than the roundings"
