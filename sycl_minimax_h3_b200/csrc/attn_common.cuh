@@ -124,13 +124,15 @@ __device__ __forceinline__ void store_out_cols(const AttnArgs& a, int b, int h, 
     for (int c4 = 0; c4 < 4; ++c4) {
         if (c4 >= chunks || col0 + c4 * 32 >= a.D) break;
         uint32_t o[32];
+        __syncwarp();                                  // the load is the whole warp's, also where rows past S store nothing
         tmem_ld32(o_taddr + c4 * 32, o);
         tmem_wait_ld();
-        if (!live) continue;
-        float v[32];
+        if (live) {
+            float v[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
-        store_out32(a, out, base + c4 * 32, v, min(32, a.D - col0 - c4 * 32));
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
+            store_out32(a, out, base + c4 * 32, v, min(32, a.D - col0 - c4 * 32));
+        }
     }
 }
 __device__ __forceinline__ void store_out_row(const AttnArgs& a, int b, int h, int qrow, uint32_t o_taddr, float inv, bool live) {

@@ -258,3 +258,24 @@ def test_other_head_sizes(D, dtype, cuda):
         qkv = make_qkv(S, H, D, seed=S + D, dtype=dtype)
         out = run_attention(qkv.to(cuda), H, D, min_s=min_s)
         check_attention(qkv, out, H, D, sage=False)
+
+
+@pytest.mark.parametrize("S", [190, 333])
+@pytest.mark.parametrize("min_s", [0, 1 << 30])
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+def test_output_rows_off_16_bytes(S, min_s, out_dtype, cuda, monkeypatch):
+    """An output that starts off 16 bytes, whose last query tile ends inside a warp: the same values as an aligned one, and
+    nothing beside it is written."""
+    H, D = 2, 128
+    qkv = make_qkv(S, H, D, seed=70).to(cuda)
+    monkeypatch.setenv("H3S_SAGE_MIN_S", str(min_s))
+    ops._ctx.clear()
+    rows = ops.Rows.qkv(qkv, H, D)
+    want = torch.empty(S, H * D, dtype=out_dtype, device=cuda)
+    room = torch.full((S * H * D + 9,), 7.0, dtype=out_dtype, device=cuda)
+    ops.attention(*rows, want)
+    ops.attention(*rows, room[1:1 + S * H * D].view(S, H * D))
+    ops.context(cuda).wait()
+    ops._ctx.clear()
+    assert torch.equal(room[1:1 + S * H * D].view(S, H * D), want)
+    assert room[0] == 7 and bool((room[1 + S * H * D:] == 7).all())
