@@ -514,6 +514,7 @@ __device__ __forceinline__ void lin_epilogue(const LinArgs& a, uint32_t taddr, i
         const int n0 = n_base + cc * 32;
         if (n0 >= a.N) break;    // the same for the whole warp
         uint32_t r[32];
+        __syncwarp();            // the load is the whole warp's, the rows' stores before it each row's own
         tmem_ld32(taddr + cc * 32, r);
         tmem_wait_ld();
         float y[32];
