@@ -237,7 +237,12 @@ struct Piece {
     int b, tile, h, z, nz;             // b < 0: there are no more
     Seq s;
 };
-__device__ __forceinline__ int pieces_of_unit(int length, int chunk) { return max(1, (2 * length + chunk) / (2 * chunk)); }   // rounded
+constexpr int kWhole = 0;              // no chunk: every unit is one piece
+__device__ __forceinline__ int pieces_of_unit(int length, int chunk) {   // rounded
+    return chunk == kWhole ? 1 : max(1, (2 * length + chunk) / (2 * chunk));
+}
+// (starts that run backwards can stand for any number of pages: the chunk stays where twice of it is an int)
+__device__ __forceinline__ int chunk_pages(float all, int room) { return max(kChunk, (int) fminf(ceilf(all / (float) room), 1 << 28)); }
 template <int ROWS>
 __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int group, int* scan) {
     const KvArgs& kv = a.kv;
@@ -266,7 +271,7 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
             float all = (float) units * (float) length;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-            nz = pieces_of_unit(length, max(kChunk, (int) ceilf(all / (float) a.plan.room)));
+            nz = pieces_of_unit(length, chunk_pages(all, a.plan.room));
         }
         int upto = units * nz;
 #pragma unroll
@@ -295,7 +300,7 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
         return p;
     }
     int length0 = 0, units0 = units_of((int) threadIdx.x, length0);      // the first 128 sequences' are kept
-    int chunk = 1 << 30;
+    int chunk = kWhole;
     if (a.plan.room > 0) {
         float all = 0.0f;                                  // pages in all: a float is exact enough to divide them
         for (int b0 = 0; b0 < kv.seqs; b0 += kAttWarps * 32) {
@@ -308,7 +313,7 @@ __device__ __forceinline__ Piece find_piece(const AttendArgs& a, int flat, int g
         if (lane == 0) scan[warp] = __float_as_int(all);
         __syncthreads();
         all = __int_as_float(scan[0]) + __int_as_float(scan[1]) + __int_as_float(scan[2]) + __int_as_float(scan[3]);
-        chunk = max(kChunk, (int) ceilf(all / (float) a.plan.room));
+        chunk = chunk_pages(all, a.plan.room);
     }
     int* found = scan + 2 * kAttWarps;
     if (threadIdx.x == 0) found[0] = -1;

@@ -605,3 +605,17 @@ def test_many_rows_of_a_warp_that_see_unlike_tails(dtype, dim, n, per, L, cuda):
     exact, _, bound = _kv.attention(cache, q, per, starts)
     off = ((out.double().cpu() - exact.view(n, per, dim)).abs() - bound.view(n, per, dim))[~infinite.cpu()]
     assert float(off.max()) <= 0, f"off by {float(off.max()):.3g} more than the roundings"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("seqs,heads,max_len", [(40, 2, 64), (33, 1, 1), (700, 8, None)])
+def test_attention_of_many_sequences_in_whole_pieces(dtype, seqs, heads, max_len, cuda):
+    """More sequences than a warp has lanes, and no unit cut: by a hint of short lengths, or because there are many units."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 300, (seqs,), generator=g).tolist()
+    news = [0 if b % 9 == 4 else 1 for b in range(seqs)]
+    cache = _kv.random_cache(lens, heads, 64, dtype, cuda, seed=seqs)
+    q = make_rows(sum(news), heads * 2 * 64, dtype, cuda, 51)
+    starts = _kv.starts_of(news, cuda)
+    out = run_attention(cache, q, heads * 2, starts, cuda, max_new=1, max_len=max_len)
+    check_attention(cache, q, starts, out, heads * 2)
