@@ -270,8 +270,9 @@ int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budg
  *   W[n, k] = scale[k / group, n] * (code[n, k] - zero[k / group, n])      code 0..15, zero NULL: 8
  * x [M, K] in x_dt; scale and zero [ceil(K / group), N] in s_dt; bias float [N] or NULL; out [M, N] in out_dt, rounded
  * once from float. group 32, 64, 128 or 0 (one scale per output). tiles: the codes as h3s_int4_pack lays them out, 16 *
- * ceil(N / 16) * 64 * ceil(K / 64) / 2 bytes on 16 bytes. Any M is right; from some hundred rows on a matrix product on
- * unpacked weights is faster. M, K or N <= 0: nothing to do, returns 0. */
+ * ceil(N / 16) * 64 * ceil(K / 64) / 2 bytes on 16 bytes. Any M is right (from some hundred rows on a matrix product on
+ * unpacked weights is faster) up to 2,097,120; N up to 2^29 - 128, K up to 2^30; more is refused. M, K or N <= 0: nothing
+ * to do, returns 0. */
 int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, const void* tiles, int64_t N,
                     const void* scale, const void* zero, int s_dt, int group, const float* bias, void* out, int out_dt);
 /* codes uint8 [N, K / 2] (K even), input 2 i in the low four bits of byte i -> tiles, once per layer. */

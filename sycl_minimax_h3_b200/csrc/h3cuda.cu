@@ -1276,6 +1276,9 @@ int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budg
     return e == cudaSuccess ? 0 : cuda_fail(who, e);
 }
 
+// The kernels count outputs, up to the end of the last block of 128, and the bytes of a group's scales in an int.
+constexpr int64_t kInt4Outputs = (1ll << 29) - 128;
+
 // ---- 4-bit linear layers (int4lin.cu) --------------------------------------------------------------------------------
 int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, const void* tiles, int64_t N,
                     const void* scale, const void* zero, int s_dt, int group, const float* bias, void* out, int out_dt) {
@@ -1285,7 +1288,7 @@ int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, co
     if (!check_dt(x_dt) || !check_dt(s_dt) || !check_dt(out_dt)) return kv_fail(who, "unknown element type");
     if (!x || !tiles || !scale || !out) return kv_fail(who, "a null pointer");
     if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
-    if (N > INT32_MAX - 16 || K > (1 << 30) || M > 65535ll * 32) return kv_fail(who, "too large");
+    if (N > kInt4Outputs || K > (1 << 30) || M > 65535ll * 32) return kv_fail(who, "too large");
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     Int4Args a{};
@@ -1315,7 +1318,7 @@ int h3s_int4_pack(void* ctx, const uint8_t* codes, int64_t N, int64_t K, void* t
     if (K % 2 != 0) return kv_fail(who, "the inputs must be even in number: two codes to a byte");
     if (!codes || !tiles) return kv_fail(who, "a null pointer");
     if (!aligned16(tiles)) return kv_fail(who, "the tiles must start on 16 bytes");
-    if (N > INT32_MAX - 16 || K > (1 << 30)) return kv_fail(who, "too large");
+    if (N > kInt4Outputs || K > (1 << 30)) return kv_fail(who, "too large");
     auto& c = *static_cast<Ctx*>(ctx);
     DeviceGuard g(c.device);
     const cudaError_t e = launch_int4_pack(codes, N, K, tiles, c.n_sm, c.st);

@@ -164,3 +164,12 @@ def test_the_definitions_of_the_tests():
     assert torch.equal(_kv.sequence(c, 1, "v")[2, 1], c.tail_v[1, 1, 2].double())
     page = int(c.table[0, 0])
     assert torch.equal(_kv.sequence(c, 0, "k")[5, 1], c.k[page, 1, 5].double() * c.k_scale[page, 1].double())
+
+
+@pytest.mark.parametrize("N", [(1 << 29) - 127, 1 << 29, (1 << 31) - 143, (1 << 31) - 17])
+def test_c_refuses_outputs_that_an_int_cannot_count(N):
+    """Up to the end of the last block of 128 outputs, and in bytes of float32 scales"""
+    L = native.lib()
+    for M in (1, 12, 40):
+        assert L.h3s_int4_linear(None, 16, 0, M, 64, 16, N, 16, None, 0, 32, None, 16, 0) == -1 and "too large" in native.last_error()
+    assert L.h3s_int4_pack(None, 16, N, 64, 16) == -1 and "too large" in native.last_error()
