@@ -189,3 +189,35 @@ def test_captured_calls_read_what_x_holds_at_the_replay(M, cuda):
     lin.forward(held, eager)
     ops.context(cuda).wait()
     assert torch.equal(eager, out)
+
+
+@pytest.mark.parametrize("x_dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("group", [0, 32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(40, 9600, 14336), (17, 9600, 1280), (64, 200, 14336)])
+def test_zero_points_over_many_stages(x_dt, group, M, N, K, cuda):
+    """Codes that are all 8, so that the output is the zero points' part alone: scale (8 - zero) times the sum of x over a
+    group. More stages than the rings have, in CTAs that take all of a layer's inputs and in parts of them; every call gives
+    the same bits."""
+    g = torch.Generator().manual_seed(M + K + group)
+    groups = -(-K // group) if group else 1
+    packed = torch.full((N, K // 2), 0x88, dtype=torch.uint8, device=cuda)
+    s = (0.01 + 0.05 * torch.rand(groups, N, generator=g)).to(cuda)
+    z = (5 + 6 * torch.rand(groups, N, generator=g)).to(cuda)
+    # the stages' rows are unlike: another size for every 128 inputs
+    size = 2.0 ** torch.randint(-3, 4, (1, K // 128), generator=g).repeat_interleave(128, 1)
+    x = (torch.randn(M, K, generator=g) * size).to(x_dt).to(cuda)
+    lin = ops.Int4Linear.pack(packed, s, group, z)
+    out = torch.empty(M, N, device=cuda)
+    lin.forward(x, out)
+    ops.context(cuda).wait()
+    part = s.double() * (8 - z.double())
+    sums = x.double().view(M, groups, K // groups)
+    want = sums.sum(2) @ part
+    bound = (K / 64 + 64) * 2.0 ** -22 * (sums.abs().sum(2) @ part.abs())
+    bound = bound + want.abs() * 2.0 ** -23 + torch.finfo(torch.float32).tiny
+    assert float(((out.double() - want).abs() - bound).max()) <= 0
+    again = torch.empty_like(out)
+    for _ in range(20):
+        lin.forward(x, again)
+        ops.context(cuda).wait()
+        assert torch.equal(again, out)
