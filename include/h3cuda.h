@@ -269,7 +269,9 @@ int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budg
 /* A linear layer with 4-bit weights for a few rows of x, out = x . W^T + bias:
  *   W[n, k] = scale[k / group, n] * (code[n, k] - zero[k / group, n])      code 0..15, zero NULL: 8
  * x [M, K] in x_dt; scale and zero [ceil(K / group), N] in s_dt; bias float [N] or NULL; out [M, N] in out_dt, rounded
- * once from float. group 32, 64, 128 or 0 (one scale per output). tiles: the codes as h3s_int4_pack lays them out, 16 *
+ * once from float. Sums are taken in float as sum x (code - 8) + (8 - zero) sum x and scaled per group; one that is not finite
+ * is taken again, term by term in 64 bits, so that infinities and NaN come out as the definition has them and a sum that
+ * passes float's largest only on its way comes out as it is. group 32, 64, 128 or 0 (one scale per output). tiles: the codes as h3s_int4_pack lays them out, 16 *
  * ceil(N / 16) * 64 * ceil(K / 64) / 2 bytes on 16 bytes. Any M is right (from some hundred rows on a matrix product on
  * unpacked weights is faster) up to 2,097,120; N up to 2^29 - 128, K up to 2^30; more is refused. M, K or N <= 0: nothing
  * to do, returns 0. */

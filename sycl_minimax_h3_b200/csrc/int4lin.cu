@@ -135,6 +135,34 @@ __device__ __forceinline__ void st_dt(void* p, size_t i, float x, int dt) {
     else reinterpret_cast<float*>(p)[i] = x;
 }
 
+// Output n of row m without its bias, term by term as the layer is defined and in 64 bits, for sums that are not finite in
+// the kernels. These form sum x (code - 8) and (8 - zero) sum x apart, and multiply by the scale last: an infinite x is then
+// 0 times infinity for the code 8, or infinity less infinity, where the definition has an infinity, and a large x passes
+// float's largest where scale (code - zero) x does not. One thread reads a whole row for it (some milliseconds for 14,336
+// inputs); a finite sum never comes here, and what is not finite on the way to a sum stays not finite.
+__device__ __noinline__ float int4_exact(const Int4Args& a, long long m, int n) {
+    const long long KT = (a.K + 63) / 64;
+    const uint2* tile = reinterpret_cast<const uint2*>(a.tiles + (n / 16) * KT * 32 + (n & 7) * 4);
+    const int up = 4 * ((n >> 3) & 1);                     // outputs 8-15 of a strip: the odd nibbles
+    double y = 0.0;
+    for (int k0 = 0; k0 < a.K; k0 += 8) {                  // 8 inputs: a pair of a lane's words, within one group
+        const uint2 u = tile[(k0 / 64) * 64 + (k0 / 8 % 4) * 2 + k0 / 32 % 2];
+        const size_t at = (size_t) (k0 >> a.group_shift) * a.N + n;
+        const double s = bits_value(ld_bits(a.scale, at, a.s_dt), a.s_dt);
+        const double z = a.zero ? bits_value(ld_bits(a.zero, at, a.s_dt), a.s_dt) : 8.0f;
+        const int count = min(8, a.K - k0);
+        for (int i = 0; i < count; ++i) {
+            const uint32_t word = i < 4 ? u.x : u.y;
+            const int code = (word >> (8 * (i / 2 % 2) + up + 16 * (i & 1))) & 15;
+            const double x = bits_value(ld_bits(a.x, (size_t) m * a.K + k0 + i, a.x_dt), a.x_dt);
+            y += s * (((double) code - z) * x);
+        }
+        if (y != y) break;
+    }
+    return (float) y;
+}
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
 // Scales and zero points of two outputs for the halves of a 64-input tile (one for both where a group has more than 32
 // inputs), as bits. An output past the last reads the last one's: its sums are not stored.
 template <bool ZERO, bool G32>
@@ -296,6 +324,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, DT == F32 ? 2 : 3) int4_few(con
             float y = 0.0f;
 #pragma unroll
             for (int w = 0; w < kI4Warps; ++w) y += red[w][c][m];
+            if (!is_finite(y)) y = int4_exact(a, m, n);
             if (a.bias) y += a.bias[n];
             st_dt(a.out, (size_t) m * a.N + n, y, a.out_dt);
         }
@@ -475,6 +504,7 @@ __global__ void __launch_bounds__(kRowsThreads) int4_rows(const __grid_constant_
         if (n >= a.N || m >= a.M) continue;
         float y = 0.0f;
         for (int p = 0; p < 2 * split; ++p) y += sm.part[(p * rows + r) * kRowsN + c];
+        if (!is_finite(y)) y = int4_exact(a, m, n);
         if (a.bias) y += a.bias[n];
         st_dt(a.out, (size_t) m * a.N + n, y, a.out_dt);
     }

@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) int4_tc(const __grid_constant__
         if (n >= a.N || m >= a.M) continue;
         float y = 0.0f;
         for (int p = 0; p < split; ++p) y += sums[(p * rows + r) * 128 + c];
+        if (!is_finite(y)) y = int4_exact(a, m, n);
         if (a.bias) y += a.bias[n];
         st_dt(a.out, (size_t) m * a.N + n, y, a.out_dt);
     }

@@ -221,3 +221,90 @@ def test_zero_points_over_many_stages(x_dt, group, M, N, K, cuda):
         lin.forward(x, again)
         ops.context(cuda).wait()
         assert torch.equal(again, out)
+
+
+def by_definition(codes, scale, z, b, x, group):
+    """The layer in 64 bits, term by term: infinities, NaN and 0 times infinity as they come."""
+    K = codes.shape[1]
+    at = torch.arange(K) // (group or K)
+    s = scale.double().t()[:, at]
+    w = codes.double() - (8.0 if z is None else z.double().t()[:, at])
+    y = torch.stack([(s * (w * row)).sum(1) for row in x.double()])
+    return y if b is None else y + b.double()
+
+
+def check_with_infinities(codes, scale, z, b, x, group, out):
+    """NaN and infinities where the definition rounded to the output's type has them; the rest within ``check``'s bound."""
+    want = by_definition(codes, scale, z, b, x, group)
+    got = out.cpu()
+    rounded = want.float().to(out.dtype)
+    assert torch.equal(got.isnan(), rounded.isnan())
+    assert torch.equal(got.isinf(), rounded.isinf()) and torch.equal(got[got.isinf()], rounded[rounded.isinf()])
+    at = torch.arange(codes.shape[1]) // (group or codes.shape[1])
+    s = scale.double().t()[:, at]
+    zero = torch.full_like(s, 8.0) if z is None else z.double().t()[:, at]
+    A = (x.double().abs() @ (s.abs() * ((codes.double() - 8).abs() + (zero - 8).abs())).t()) + (0 if b is None else b.double().abs())
+    bound = (codes.shape[1] / 64 + 64) * 2.0 ** -22 * A
+    bound = bound + (want.abs() + bound) * (torch.finfo(out.dtype).eps / 2) + torch.finfo(out.dtype).tiny
+    fin = rounded.isfinite()
+    assert not bool(((got.double() - want).abs() > bound)[fin].any())
+
+
+ROWS_OF_EACH_KERNEL = [(4, torch.bfloat16), (4, torch.float16), (4, torch.float32), (12, torch.bfloat16), (12, torch.float32),
+                       (40, torch.bfloat16), (40, torch.float16), (40, torch.float32), (70, torch.float16)]
+
+
+@pytest.mark.parametrize("M,x_dt", ROWS_OF_EACH_KERNEL)
+@pytest.mark.parametrize("group,zero", [(0, True), (32, True), (64, True), (128, True), (32, False)])
+def test_infinities_meet_zero_points(M, x_dt, group, zero, cuda):
+    """An infinite input: its output is the infinity of (code - zero)'s sign, NaN only where code = zero or where two of them
+    meet with unlike signs; one row of NaN, one with an infinity of each sign."""
+    K, N = 328, 70
+    codes, scale, z, b, x, lin = make(M, N, K, group, x_dt, torch.float32, zero, True, cuda, seed=M + group)
+    if zero:
+        z[:, 5] = 8.0                                  # zero points that are codes: 0 times infinity
+        z[:, 6] = 3.0
+        lin = ops.Int4Linear(lin.tiles, lin.scale, N, K, group, z.to(cuda), lin.bias)
+    x[0, 7] = float("inf")
+    x[1, 40] = -float("inf")
+    x[2, 3], x[2, 100] = float("inf"), -float("inf")
+    x[M - 1, 327] = float("nan")
+    out = torch.empty(M, N, dtype=x_dt, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    check_with_infinities(codes, scale, z, b, x, group, out)
+    assert bool(out[0].isinf().any()) and bool(out[M - 1].isnan().all())
+
+
+@pytest.mark.parametrize("M,x_dt", [m for m in ROWS_OF_EACH_KERNEL if m[1] != torch.float16])
+@pytest.mark.parametrize("group,zero", [(0, True), (32, False), (64, True), (128, False)])
+def test_sums_that_only_pass_the_largest_float_on_their_way(M, x_dt, group, zero, cuda):
+    """Inputs near the largest of their type with scales that bring the terms back: the outputs are the definition's."""
+    K, N = 328, 70
+    codes, scale, z, b, x, lin = make(M, N, K, group, x_dt, torch.float32, zero, True, cuda, seed=M + group + 1)
+    scale = scale * 2.0 ** -10
+    lin = ops.Int4Linear(lin.tiles, scale.to(cuda), N, K, group, lin.zero, lin.bias)
+    x[0] = (x[0].float().clamp(-3, 3) * 1e38).to(x_dt)
+    x[M - 1, 5], x[M - 1, 6] = 3e38, -3e38
+    out = torch.empty(M, N, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    assert bool(by_definition(codes, scale, z, b, x, group).float().isfinite().all())
+    check_with_infinities(codes, scale, z, b, x, group, out)
+
+
+@pytest.mark.parametrize("M", [4, 12, 40])
+def test_scales_and_zero_points_that_are_not_finite_stay_in_their_output(M, cuda):
+    K, N = 200, 40
+    codes, scale, z, b, x, lin = make(M, N, K, 64, torch.bfloat16, torch.float32, True, True, cuda, seed=M + 2)
+    scale[1, 3], scale[2, 5], z[0, 7], z[3, 9] = float("inf"), float("nan"), float("inf"), float("nan")
+    codes[codes == 8] = 9
+    packed = (codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous().to(cuda)
+    lin = ops.Int4Linear.pack(packed, scale.to(cuda), 64, z.to(cuda), b.to(cuda))
+    out = torch.empty(M, N, device=cuda)
+    lin.forward(x.to(cuda), out)
+    ops.context(cuda).wait()
+    want = by_definition(codes, scale, z, b, x, 64).float()
+    assert torch.equal(out.cpu().isnan(), want.isnan()) and torch.equal(out.cpu().isinf(), want.isinf())
+    keep = [n for n in range(N) if n not in (3, 5, 7, 9)]
+    check(codes[keep], scale[:, keep], z[:, keep], b[keep], x, 64, out[:, keep])
