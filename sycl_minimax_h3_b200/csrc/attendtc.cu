@@ -8,8 +8,10 @@
 // page's scale vs enters as an exponent, a = 2^(arg + log2(vs / vref)) = p vs / vref, so P.V accumulates code * a over pages
 // of different scales, and the row's sum takes a's sum over vs / vref. vref is the largest scale that the CTA meets; a
 // page whose scale is under 2^-60 of it counts with that (its values, 127 codes at most, are lost beside vref's).
-// The reference m of a row is moved when a half's largest a would pass 2^14, so that this becomes 2^6: fp16 keeps its 11
-// bits of an a down to 2^-20 of the row's largest, and what it drops is 2^-31 of that.
+// The reference m of a row is a whole number, moved when a half's largest a would pass 2^14, so that this becomes 2^6 to 2^7:
+// fp16 keeps its 11 bits of an a down to 2^-20 of the row's largest, and what it drops is 2^-31 of that. A move by a power
+// of two is exact, in fp16 (weights that are taken already) as in the sums. An a is rounded once, to fp16: the 11 bits of
+// P.V's operands, 2^-11 of it beside the 2^-8 or 2^-11 of the output; the row's sum takes it unrounded.
 // q, and the tail's keys and values, are brought to fp16 by powers of two (per row; per head's tail): exact for 16-bit
 // types except what is some 2^27 times smaller than the row's or the tail's largest.
 //
@@ -70,6 +72,8 @@ __device__ __forceinline__ void codes16(const uint4 u, uint4& lo, uint4& hi) {
 // the exponent e that brings top into [2^13, 2^14) when divided by 2^e, and 2^-e in two normal factors
 __device__ __forceinline__ int exponent_of(float top) { return top > 0.0f ? ilogbf(top) - 13 : 0; }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // |e| <= 126
+// 2^d of a whole d <= 0, 0 below 2^-126
+__device__ __forceinline__ float pow2_down(float d) { return __int_as_float(max(0, 127 + (int) d) << 23); }
 __device__ __forceinline__ uint4 halves8(const float (&x)[8], float m1, float m2) {
     uint32_t h[4];
 #pragma unroll
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
             __syncwarp();
             if (lane == 0) mbar_arrive(hi_free + t);
             const float sm_hi = sage3_bias_max<false>(x, valid_hi) * c_hi + g_hi;
-            if (sm_hi > m_run + 14.0f) m_run = sm_hi - 6.0f;
+            if (sm_hi > m_run + 14.0f) m_run = floorf(sm_hi) - 6.0f;
             const float m_hi = m_run;
             uint32_t p_hi[32];
             take_turn(turns == 0);
@@ -472,9 +476,9 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
             tmem_ld32(t_lane + colS + 32, x[1]);
             tmem_wait_ld();
             const float sm_lo = sage3_bias_max<false>(x, valid_lo) * c_lo + g_lo;
-            if (sm_lo > m_run + 14.0f) m_run = sm_lo - 6.0f;
+            if (sm_lo > m_run + 14.0f) m_run = floorf(sm_lo) - 6.0f;
             if (__any_sync(0xffffffffu, m_run != m_hi)) {
-                const float f = m_run == m_hi ? 1.0f : (m_hi == -INFINITY ? 0.0f : ex2(m_hi - m_run));
+                const float f = m_run == m_hi ? 1.0f : pow2_down(m_hi - m_run);
                 const __half2 f2 = __float2half2_rn(f);
                 sum_hi *= f;
 #pragma unroll
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
             tmem_st16(t_lane + colS, *reinterpret_cast<const uint32_t(*)[16]>(&p_lo[0]));
             tmem_st16(t_lane + colS + 16, *reinterpret_cast<const uint32_t(*)[16]>(&p_lo[16]));
             const bool grow = m_run != m_prev;
-            const float alpha = grow ? (m_prev == -INFINITY ? 0.0f : ex2(m_prev - m_run)) : 1.0f;
+            const float alpha = grow ? pow2_down(m_prev - m_run) : 1.0f;
             l_run = fmaf(l_run, alpha, sum_hi / w_hi + sum_lo / w_lo);
             if (__any_sync(0xffffffffu, grow && i > 0)) {
                 const float al = i > 0 ? alpha : 1.0f;

@@ -619,3 +619,33 @@ def test_attention_of_many_sequences_in_whole_pieces(dtype, seqs, heads, max_len
     starts = _kv.starts_of(news, cuda)
     out = run_attention(cache, q, heads * 2, starts, cuda, max_new=1, max_len=max_len)
     check_attention(cache, q, starts, out, heads * 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("low", [0, 1])
+def test_many_rows_whose_reference_moves_between_halves(dtype, low, cuda):
+    """The second half of a key tile is taken first; keys of the first whose scores are some 2^8.5 to 2^12 times as large move
+    the reference of the weights taken before. Only those have values, so that their roundings alone are seen: one for
+    each weight. ``low``: the same with the move between two key tiles."""
+    n, pages = 4096, 5
+    cache = _kv.random_cache([64 * pages + n], 1, 64, dtype, cuda, seed=52)
+    cache.k.zero_()
+    cache.v.zero_()
+    cache.k_scale.fill_(0.05)
+    cache.v_scale.fill_(2000.0)
+    page = cache.table[0, :pages + n // PAGE].long()
+    for i in range(len(page)):
+        cache.k[page[i], 0, :, :2] = -60
+    first, second = (0, 1) if not low else (2, 1)      # `first` is read after `second` and scores higher
+    cache.k[page[first], 0, :, :2] = 60
+    cache.k[page[second], 0, :, :2] = -5
+    cache.k[page[second], 0, 0, :2] = 0                # the largest of its half, with no value
+    cache.v[page[second], 0, 1:, :] = 100
+    g = torch.Generator().manual_seed(53)
+    q = torch.zeros(n, 64)
+    q[:, 0] = (0.1417 + 0.0583 * torch.rand(n, generator=g)) * 8 / (0.05 * 1.4427)
+    q[:, 1] = 0.05 * torch.rand(n, generator=g)        # scores finer than the first feature's steps
+    q = q.to(dtype).to(cuda)
+    starts = _kv.starts_of([n], cuda)
+    out = run_attention(cache, q, 1, starts, cuda)
+    check_attention(cache, q, starts, out, 1)
