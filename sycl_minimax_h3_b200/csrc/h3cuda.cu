@@ -708,22 +708,20 @@ int h3s_wait(void* ctx) {
     int codes[2] = {0, 0};
     e = cudaMemcpy(codes, c.err, sizeof(codes), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return cuda_fail("h3s_wait", e);
-    const int code = codes[0];
-    if (code || codes[1]) cudaMemset(c.err, 0, sizeof(codes));
-    if (codes[1] && !code) {
-        g_err = std::string("h3s_wait: a call found ") +
-                (codes[1] == kErrPage ? "a page id outside the cache's pool"
-                 : codes[1] == kErrLen ? "lengths or row starts out of range"
-                                       : "a page id outside the cache's pool, and lengths or row starts out of range") +
-                "; what it names was left out";
-        return -1;
-    }
-    if (code) {
-        g_err = "h3s_wait: a wait inside a kernel gave up after " + std::to_string(c.wait_ns / 1000000) +
-                " ms (code " + std::to_string(code) + "); its results are not valid";
-        return -1;
-    }
-    return 0;
+    if (!codes[0] && !codes[1]) return 0;
+    cudaMemset(c.err, 0, sizeof(codes));
+    g_err = "h3s_wait: ";
+    if (codes[0])
+        g_err += "a wait inside a kernel gave up after " + std::to_string(c.wait_ns / 1000000) + " ms (code " +
+                 std::to_string(codes[0]) + "); its results are not valid";
+    if (codes[0] && codes[1]) g_err += "; ";
+    if (codes[1])
+        g_err += std::string("a call found ") +
+                 (codes[1] == kErrPage ? "a page id outside the cache's pool"
+                  : codes[1] == kErrLen ? "lengths or row starts out of range"
+                                        : "a page id outside the cache's pool, and lengths or row starts out of range") +
+                 "; what it names was left out";
+    return -1;
 }
 
 void* h3s_alloc_host(void* ctx, uint64_t bytes) {

@@ -649,3 +649,16 @@ def test_many_rows_whose_reference_moves_between_halves(dtype, low, cuda):
     starts = _kv.starts_of([n], cuda)
     out = run_attention(cache, q, 1, starts, cuda)
     check_attention(cache, q, starts, out, 1)
+
+
+def test_a_wait_that_gave_up_and_a_bad_page_are_both_reported(cuda):
+    cache = _kv.random_cache([200], 1, 64, torch.float16, cuda, seed=54)
+    q = make_rows(1, 64, torch.float16, cuda, 55)
+    starts = _kv.starts_of([1], cuda)
+    cache.table[0, 1] = -1
+    ctx = ops.context(cuda)
+    ops.attention_cached(_kv.rows(q, 1, 64), cache, starts, torch.empty_like(q))
+    ctx.selftest_wait_timeout(2_000_000)               # 2 ms
+    with pytest.raises(native.H3Error, match="gave up.*page id"):
+        ctx.wait()
+    ctx.wait()
