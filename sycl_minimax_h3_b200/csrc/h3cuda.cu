@@ -709,7 +709,7 @@ int h3s_wait(void* ctx) {
     e = cudaMemcpy(codes, c.err, sizeof(codes), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return cuda_fail("h3s_wait", e);
     if (!codes[0] && !codes[1]) return 0;
-    cudaMemset(c.err, 0, sizeof(codes));
+    cudaMemsetAsync(c.err, 0, sizeof(codes), c.st);        // before what this context queues next, which may fail as well
     g_err = "h3s_wait: ";
     if (codes[0])
         g_err += "a wait inside a kernel gave up after " + std::to_string(c.wait_ns / 1000000) + " ms (code " +

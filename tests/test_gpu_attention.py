@@ -279,3 +279,17 @@ def test_output_rows_off_16_bytes(S, min_s, out_dtype, cuda, monkeypatch):
     ops._ctx.clear()
     assert torch.equal(room[1:1 + S * H * D].view(S, H * D), want)
     assert room[0] == 7 and bool((room[1 + S * H * D:] == 7).all())
+
+
+def test_every_failure_is_reported_by_the_wait_behind_it(cuda):
+    """The error word is cleared in the order of the context's stream: a failure queued right after a reported one is not
+    cleared with it. (Waits of a microsecond that run out.)"""
+    ctx = native.Context.open_gpu(0)
+    try:
+        for _ in range(200):
+            ctx.selftest_wait_timeout(1000)
+            with pytest.raises(native.H3Error, match="gave up"):
+                ctx.wait()
+        ctx.wait()
+    finally:
+        ctx.close()
