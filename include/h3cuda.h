@@ -245,8 +245,9 @@ int h3s_kv_append(void* ctx, const h3s_kv_cache* kv, const void* k, const void* 
 
 /* Causal attention with grouped heads over the cache: query row starts[b] + i (i < n; T rows of Hq x dim at stride qs,
  * type dt) is token lens[b] - n + i of sequence b and sees the slots up to its own; query head h reads key/value head
- * h / (Hq / heads), scores q.k / sqrt(dim). out [T, Hq * dim] in dt, rounded once from float; a row that sees nothing
- * (lens[b] < n) is 0, rows behind starts[seqs] are left as they were. accumulate: weight[slot] += the sum of the slot's
+ * h / (Hq / heads), scores q.k / sqrt(dim). out [T, Hq * dim] in dt; a row that sees nothing (lens[b] < n) is 0, rows
+ * behind starts[seqs] are left as they were. An infinite or NaN value in the tail (a page's codes have none) makes its
+ * feature infinite or NaN in every row that sees it, however small its weight. accumulate: weight[slot] += the sum of the slot's
  * softmax weights over the rows and heads that read it (kv->weight needed). max_new, max_len: what the largest n and
  * length are about (0: T, 64 * width), for the division of the work; none is wrong. work: work_bytes of device memory,
  * at least h3s_attention_cached_work(...) of the same arguments, on 16 bytes, this call's own until it has run. */

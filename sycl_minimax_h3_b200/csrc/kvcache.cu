@@ -616,7 +616,7 @@ __device__ __noinline__ void attend_tail(const AttendArgs& a) {
         if (lane == 0) { sm.m[kAttWarps][r] = mx; sm.l[kAttWarps][r] = sum; }
     }
     __syncthreads();
-    // a thread has one feature and TR rows; a value that a row does not see is not multiplied by its p of 0
+    // a thread has one feature and TR rows
     const int d = threadIdx.x % D, rb = threadIdx.x / D * TR;
 #pragma unroll
     for (int r = 0; r < TR; ++r) ot[r] = 0.0f;
@@ -635,14 +635,14 @@ __device__ __noinline__ void attend_tail(const AttendArgs& a) {
             odd = fmaf(x, 0.0f, odd);
         }
     }
-    if (odd != 0.0f && sm.pos[0] < L - 1) {      // some rows see less: theirs again, without what they do not see
+    if (odd != 0.0f) {                           // again, without what a row does not see, and 0 times infinity an infinity
 #pragma unroll
         for (int r = 0; r < TR; ++r) {
             if (rb + r >= nrow) break;
             const int see = min(nkey, sm.pos[rb + r] + 1 - full * kPage);
             ot[r] = 0.0f;
 #pragma unroll 4
-            for (int key = 0; key < see; ++key) ot[r] = fmaf(sm.sc[key][rb + r], ld1<DT>(sm.tail[1], (size_t) key * D + d), ot[r]);
+            for (int key = 0; key < see; ++key) ot[r] = add_weighted(sm.sc[key][rb + r], ld1<DT>(sm.tail[1], (size_t) key * D + d), ot[r]);
         }
     }
     __syncthreads();                                       // the tail has been read, its memory becomes accumulators
@@ -930,10 +930,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
                 const float e = ex2(sm.m[p][r] - mu);
                 const float4 x = *reinterpret_cast<const float4*>(&sm.acc[p][r][d]);
                 sum = fmaf(e, sm.l[p][r], sum);
-                o.x = fmaf(e, x.x, o.x);
-                o.y = fmaf(e, x.y, o.y);
-                o.z = fmaf(e, x.z, o.z);
-                o.w = fmaf(e, x.w, o.w);
+                o.x = add_weighted(e, x.x, o.x);
+                o.y = add_weighted(e, x.y, o.y);
+                o.z = add_weighted(e, x.z, o.z);
+                o.w = add_weighted(e, x.w, o.w);
             }
             const size_t gr = (size_t) sm.row[r];
             if (whole) {
@@ -1009,13 +1009,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
             const float mu = mn == -INFINITY ? 0.0f : mn, al = ex2(m - mu);
             sum *= al;
 #pragma unroll
-            for (int u = 0; u < D / 32; ++u) o[u] *= al;
+            for (int u = 0; u < D / 32; ++u) o[u] = add_weighted(al, o[u], 0.0f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float e = ex2(ml[i].x - mu);
                 sum = fmaf(e, ml[i].y, sum);
 #pragma unroll
-                for (int u = 0; u < D / 32; ++u) o[u] = fmaf(e, x[i][u], o[u]);
+                for (int u = 0; u < D / 32; ++u) o[u] = add_weighted(e, x[i][u], o[u]);
             }
             m = mn;
         }
@@ -1038,7 +1038,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
             const int d = threadIdx.x;
             float y = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) y = fmaf(ex2(sx[w] - mu), so[w][d], y);
+            for (int w = 0; w < kJoinWarps; ++w) y = add_weighted(ex2(sx[w] - mu), so[w][d], y);
             st1<DT>(a.out, gr * D + d, sum == 0.0f ? 0.0f : y / sum);
         }
         if (a.lse && threadIdx.x == 0) a.lse[gr] = sum == 0.0f ? INFINITY : mu + log2f(sum);

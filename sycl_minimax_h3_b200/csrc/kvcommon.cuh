@@ -96,6 +96,8 @@ __device__ __forceinline__ void floats8(const Raw8<DT>& r, float (&x)[8]) {
 }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+// o + e x for a weight e that may have come out 0 for being small: an infinity (or a NaN) in x is one in o all the same
+__device__ __forceinline__ float add_weighted(float e, float x, float o) { return finite(x) ? fmaf(e, x, o) : o + x; }
 
 // The keys that a tile of query rows sees, and how they are divided: np whole pages in pieces of cz pages, and the tail
 // (when seen) as a piece of its own, or with the last piece where no split is left.

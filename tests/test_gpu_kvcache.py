@@ -662,3 +662,44 @@ def test_a_wait_that_gave_up_and_a_bad_page_are_both_reported(cuda):
     with pytest.raises(native.H3Error, match="gave up.*page id"):
         ctx.wait()
     ctx.wait()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("L,n,per", [(100, 1, 1), (100, 3, 4), (4000, 2, 3), (130, 66, 2), (4000, 64, 1), (60, 60, 1)])
+def test_infinite_values_of_small_weights(dtype, dim, L, n, per, cuda):
+    """An infinite value in the tail whose key's score lies so far below the others that its weight is 0 in 32 bits: its
+    feature is infinite in the rows that see it, NaN where both signs meet or a value is NaN, on every path and through
+    every join; the other features stay."""
+    cache = _kv.random_cache([L], 1, dim, dtype, cuda, seed=56)
+    q = make_rows(n, per * dim, dtype, cuda, 57)
+    q[:, ::dim] = 8                                    # feature 0 of every head
+    tail = L % PAGE
+    seen = (max(tail - 3, 0), max(tail - 2, 1))        # two keys that the last rows see
+    cache.tail_k[0, 0, seen[0]:seen[1] + 1] = 0
+    cache.tail_k[0, 0, seen[0]:seen[1] + 1, 0] = -4000.0
+    starts = _kv.starts_of([n], cuda)
+    clean = run_attention(cache, q, per, starts, cuda).view(n, per, dim)
+    check_attention(cache, q, starts, clean.view(n, -1), per)
+    inf = float("inf")
+    cache.tail_v[0, 0, seen[0], 5] = inf
+    cache.tail_v[0, 0, seen[1], 9] = -inf
+    cache.tail_v[0, 0, seen[0], 40], cache.tail_v[0, 0, seen[1], 40] = inf, -inf
+    cache.tail_v[0, 0, seen[1], dim - 1] = float("nan")
+    out = run_attention(cache, q, per, starts, cuda).view(n, per, dim)
+    pos = torch.arange(L - n, L) - (L - tail)
+    sees0, sees1 = pos >= seen[0], pos >= seen[1]
+    assert bool(sees1.any())
+    want = clean.clone()
+    want[sees0.to(cuda), :, 5] = inf
+    want[sees1.to(cuda), :, 9] = -inf
+    want[sees0.to(cuda), :, 40] = inf
+    want[sees1.to(cuda), :, 40] = float("nan")
+    want[sees1.to(cuda), :, dim - 1] = float("nan")
+    odd = ~want.isfinite()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(7.0, 1e4, -1e4)[odd], want.nan_to_num(7.0, 1e4, -1e4)[odd])
+    for t, f in ((seen[0], 5), (seen[1], 9), (seen[0], 40), (seen[1], 40), (seen[1], dim - 1)):
+        cache.tail_v[0, 0, t, f] = 0
+    exact, _, bound = _kv.attention(cache, q, per, starts)
+    off = ((out.double().cpu() - exact.view(n, per, dim)).abs() - bound.view(n, per, dim))[~odd.cpu()]
+    assert float(off.max()) <= 0
