@@ -1459,7 +1459,8 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     const int64_t tiles = T * group / p.rows + seqs;
     if (p.rows == 256) {
         p.grid = (int) tiles;
-        const int64_t units = seqs * heads * std::max<int64_t>(1, (rows + 255) / 256);
+        // (at least the tiles that T rows make: with a hint far below them the splits' partial results would grow with both)
+        const int64_t units = heads * std::max(seqs * std::max<int64_t>(1, (rows + 255) / 256), T * group / 256);
         p.nz = (int) std::max<int64_t>(1, std::min<int64_t>({(pages + kMinPages - 1) / kMinPages, n_sm / units, 512}));
         p.joined = p.nz > 1;
         p.entries = p.joined ? T * heads * group * p.nz : 0;

@@ -703,3 +703,11 @@ def test_infinite_values_of_small_weights(dtype, dim, L, n, per, cuda):
     exact, _, bound = _kv.attention(cache, q, per, starts)
     off = ((out.double().cpu() - exact.view(n, per, dim)).abs() - bound.view(n, per, dim))[~odd.cpu()]
     assert float(off.max()) <= 0
+
+
+@pytest.mark.parametrize("max_new", [12, 64, 1000, None])
+def test_a_hint_below_the_rows_of_a_call_takes_no_more_memory(max_new, cuda):
+    """The partial results of 100,000 rows with a hint of a few: as many as there are without it (30 GB before)."""
+    cache = ops.KVCache.empty(1, 1, 4096, 8, 128, torch.float16, cuda)
+    nbytes = ops.context(cuda).attention_cached_work(cache._ptr, 100000, 32, max_new or 0, 0, 0)
+    assert nbytes <= 2 * 148 * 256 * 130 * 4
