@@ -8,10 +8,12 @@
 // page's scale vs enters as an exponent, a = 2^(arg + log2(vs / vref)) = p vs / vref, so P.V accumulates code * a over pages
 // of different scales, and the row's sum takes a's sum over vs / vref. vref is the largest scale that the CTA meets; a
 // page whose scale is under 2^-60 of it counts with that (its values, 127 codes at most, are lost beside vref's).
-// The reference m of a row is a whole number, moved when a half's largest a would pass 2^14, so that this becomes 2^6 to 2^7:
-// fp16 keeps its 11 bits of an a down to 2^-20 of the row's largest, and what it drops is 2^-31 of that. A move by a power
-// of two is exact, in fp16 (weights that are taken already) as in the sums. An a is rounded once, to fp16: the 11 bits of
-// P.V's operands, 2^-11 of it beside the 2^-8 or 2^-11 of the output; the row's sum takes it unrounded.
+// The reference m of a row is moved when a half's largest a would pass 2^14, so that this becomes 2^6 (to 2^7): fp16 keeps its
+// 11 bits of an a down to 2^-20 of the row's largest, and what it drops is 2^-31 of that. Where the second half moves it
+// while the first one's weights stand in fp16, it moves by a whole number, and these are multiplied by an exact power of
+// two: an a is rounded once, to fp16, which is 2^-11 of it beside the 2^-8 or 2^-11 of the output; the row's sum takes it
+// unrounded. (Whole numbers for every move: 2.94e-4 off the definition instead of 2.76e-4, fp16's own rounding 2.07e-4, at
+// 1,999 tokens behind 15,002, since a weight that sets the reference is 2^6 exactly otherwise.)
 // q, and the tail's keys and values, are brought to fp16 by powers of two (per row; per head's tail): exact for 16-bit
 // types except what is some 2^27 times smaller than the row's or the tail's largest.
 //
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
             __syncwarp();
             if (lane == 0) mbar_arrive(hi_free + t);
             const float sm_hi = sage3_bias_max<false>(x, valid_hi) * c_hi + g_hi;
-            if (sm_hi > m_run + 14.0f) m_run = floorf(sm_hi) - 6.0f;
+            if (sm_hi > m_run + 14.0f) m_run = sm_hi - 6.0f;
             const float m_hi = m_run;
             uint32_t p_hi[32];
             take_turn(turns == 0);
@@ -476,9 +478,13 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
             tmem_ld32(t_lane + colS + 32, x[1]);
             tmem_wait_ld();
             const float sm_lo = sage3_bias_max<false>(x, valid_lo) * c_lo + g_lo;
-            if (sm_lo > m_run + 14.0f) m_run = floorf(sm_lo) - 6.0f;
-            if (__any_sync(0xffffffffu, m_run != m_hi)) {
-                const float f = m_run == m_hi ? 1.0f : pow2_down(m_hi - m_run);
+            float up = 0.0f;                           // how far the reference moves while P_hi stands in fp16: a whole number
+            if (sm_lo > m_run + 14.0f) {
+                up = m_hi == -INFINITY ? INFINITY : floorf(sm_lo - m_hi) - 6.0f;
+                m_run = m_hi == -INFINITY ? sm_lo - 6.0f : m_hi + up;
+            }
+            if (__any_sync(0xffffffffu, up != 0.0f)) {
+                const float f = pow2_down(-up);
                 const __half2 f2 = __float2half2_rn(f);
                 sum_hi *= f;
 #pragma unroll
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
             tmem_st16(t_lane + colS, *reinterpret_cast<const uint32_t(*)[16]>(&p_lo[0]));
             tmem_st16(t_lane + colS + 16, *reinterpret_cast<const uint32_t(*)[16]>(&p_lo[16]));
             const bool grow = m_run != m_prev;
-            const float alpha = grow ? pow2_down(m_prev - m_run) : 1.0f;
+            const float alpha = grow ? (m_prev == -INFINITY ? 0.0f : ex2(m_prev - m_run)) : 1.0f;
             l_run = fmaf(l_run, alpha, sum_hi / w_hi + sum_lo / w_lo);
             if (__any_sync(0xffffffffu, grow && i > 0)) {
                 const float al = i > 0 ? alpha : 1.0f;
