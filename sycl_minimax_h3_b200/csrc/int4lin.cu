@@ -351,7 +351,7 @@ struct RowsSmem {
 };
 
 template <int DT, bool ZERO, bool G32, int MT>
-__global__ void __launch_bounds__(kRowsThreads) int4_rows(const __grid_constant__ Int4Args a, int split) {
+__global__ void __launch_bounds__(kRowsThreads, 1) int4_rows(const __grid_constant__ Int4Args a, int split) {
     constexpr int TERMS = DT == F32 ? 3 : 1;
     constexpr int XT = DT == F16 ? F16 : BF16;
     constexpr int ROWS = 8 * MT, STAGES = RowsSmem<TERMS>::STAGES, AHEAD = 3;
