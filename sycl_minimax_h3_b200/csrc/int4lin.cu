@@ -190,9 +190,11 @@ __device__ __forceinline__ void load_scales(const Int4Args& a, int kt, int n0, i
 // RT strips of 16 outputs per CTA; its 8 warps take the 64-input tiles in turn, each with the loads of the next one under
 // way, and their sums meet in shared memory.
 // One row of 4096 inputs to 12288 outputs in bf16, groups of 128: 11.2 us (25 MB at 2.25 TB/s; the bytes alone 3.9), 28672
-// outputs 22.7 us, 8 rows of 12288 12.0 us. Issue bounds it, not memory (10.4 us with the codes in L2): 27 instructions per
-// word of 8 codes and lane, of which unpacking is 11, and the ends of eight tiles a warp; the schedulers issue 58 % of the
-// time. Codes through a ring of bulk copies, eight tiles ahead, took 14.2 us: more instructions, and no wait less.
+// outputs 22.7 us, 8 rows of 12288 12.0 us; groups of 32 with zero points 17.7 us, float32 22.7 us. Not memory's rate bounds it
+// (10.4 us with the codes in L2) but instructions and the waits between them: 27 per word of 8 codes and lane, of which
+// unpacking is 11, while the schedulers issue 58 % of the time, for a warp has eight tiles, two of them under way, and starts
+// and ends with nothing to do. Codes through a ring of bulk copies, eight tiles ahead, took 14.2 us: more instructions, and
+// no wait less.
 template <int DT, int SDT, bool ZERO, bool G32, int RT>
 __global__ void __launch_bounds__(kI4Warps * 32, DT == F32 ? 2 : 3) int4_few(const __grid_constant__ Int4Args a) {
     constexpr int TERMS = DT == F32 ? 3 : 1, ES = DtInfo<DT>::ES, SES = DtInfo<SDT>::ES, NS = G32 ? 2 : 1;
@@ -335,8 +337,8 @@ __global__ void __launch_bounds__(kI4Warps * 32, DT == F32 ? 2 : 3) int4_few(con
 // 128 outputs x up to 64 rows per CTA: a warp has 16 outputs and every row, so that a tile is unpacked once for all of
 // them; x comes through a ring in shared memory, 128 inputs at a time, of which warps 0-7 take the first 64 and warps
 // 8-15 the others. A cluster of `split` CTAs divides the inputs. The sums meet in shared memory, always in one order.
-// 16 rows of 14336 inputs to 4096 outputs in bf16 23.4 us (29 MB at 1.25 TB/s). A stage's barrier and the unpacking behind it
-// bound it.
+// 16 rows of 14336 inputs to 4096 outputs in bf16 22.0 us (29 MB at 1.33 TB/s), with zero points 26.3; float32 33.8, 48 rows 79.
+// A stage's barrier and the unpacking behind it bound it: the schedulers issue 46 % of the time with 16 warps on an SM.
 constexpr int kRowsN = 128, kRowsM = 64, kRowsThreads = 512;
 
 template <int TERMS>
@@ -605,8 +607,17 @@ cudaError_t tc_nc(const Int4Args& a, int n_sm, cudaStream_t st) {
 template <int DT, int SDT, bool ZERO, bool G32>
 cudaError_t few_s(const Int4Args& a, int n_sm, cudaStream_t st) {
     const int strips = (a.N + 15) / 16;
-    if (strips >= 4 * n_sm) int4_few<DT, SDT, ZERO, G32, 2><<<(unsigned) ((strips + 1) / 2), kI4Warps * 32, 0, st>>>(a);
-    else int4_few<DT, SDT, ZERO, G32, 1><<<(unsigned) strips, kI4Warps * 32, 0, st>>>(a);
+    // Two strips to a CTA share what is done for x, where there are enough of them for every SM: float32, whose x is three
+    // terms, 22.7 us against 29.9 for 12288 outputs of 4096 inputs; 16-bit types 11.3 against 11.8 (28672: 23.0 and 23.6; 9600
+    // 11.0 and 10.5). With zero points or groups of 32 a 16-bit type has not the registers for it: 16.5 against 13.9, and 25.3
+    // against 17.7 with both.
+    if constexpr (DT == F32 || (!ZERO && !G32)) {
+        if (strips >= 4 * n_sm) {
+            int4_few<DT, SDT, ZERO, G32, 2><<<(unsigned) ((strips + 1) / 2), kI4Warps * 32, 0, st>>>(a);
+            return cudaGetLastError();
+        }
+    }
+    int4_few<DT, SDT, ZERO, G32, 1><<<(unsigned) strips, kI4Warps * 32, 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -619,8 +630,10 @@ cudaError_t int4_dt(const Int4Args& a, int n_sm, cudaStream_t st) {
             default: return few_s<DT, F32, ZERO, G32>(a, n_sm, st);
         }
     }
-    // up to 16 rows of a 16-bit type mma.sync is the quicker, its stages being shorter: 4096 outputs of 4096 inputs 9.6 us
-    // against 11.6 (12288 of 4096: 28.4 against 26.2); at 17 rows 11.8 against 11.7, at 32 of 12288 34.6 against 26.6
+    // Up to 16 rows of a 16-bit type mma.sync is the quicker, its stages being shorter. 16 rows in bf16, groups of 128, against
+    // tcgen05, us: 4096 inputs to 4096 outputs 9.0 and 11.4, to 12288 26.9 and 25.7, to 28672 45.5 and 49.7; 14336 to 4096 22.1
+    // and 23.9; with groups of 32 9.7 and 15.2, 28.4 and 45.4, 49.3 and 87.5, 23.6 and 39.4. At 17 rows this kernel's next size,
+    // 32 rows, was 11.8 against 11.7 and 34.6 against 26.6 (12288).
     if (a.M <= 16) return rows_mt<DT, ZERO, G32, 2>(a, n_sm, st);
     if constexpr (DT == F32) {
         if (a.M <= 32) return rows_mt<DT, ZERO, G32, 4>(a, n_sm, st);

@@ -308,3 +308,16 @@ def test_scales_and_zero_points_that_are_not_finite_stay_in_their_output(M, cuda
     assert torch.equal(out.cpu().isnan(), want.isnan()) and torch.equal(out.cpu().isinf(), want.isinf())
     keep = [n for n in range(N) if n not in (3, 5, 7, 9)]
     check(codes[keep], scale[:, keep], z[:, keep], b[keep], x, 64, out[:, keep])
+
+
+@pytest.mark.parametrize("x_dt", TYPES)
+@pytest.mark.parametrize("group,zero", [(0, False), (32, True), (64, True), (128, False), (32, False)])
+@pytest.mark.parametrize("M,N,K", [(1, 9473, 200), (8, 9500, 1030), (3, 12288, 64)])
+def test_few_rows_of_wide_layers(x_dt, group, zero, M, N, K, cuda):
+    """Enough outputs for two strips to a CTA, an odd number of strips among them"""
+    codes, scale, z, b, x, lin = make(M, N, K, group, x_dt, torch.bfloat16, zero, True, cuda, seed=N + K)
+    out = torch.full((M + 1, N), 7.0, dtype=torch.float32, device=cuda)
+    lin.forward(x.to(cuda), out[:M])
+    ops.context(cuda).wait()
+    check(codes, scale, z, b, x, group, out[:M])
+    assert bool((out[M] == 7.0).all())
