@@ -711,3 +711,24 @@ def test_a_hint_below_the_rows_of_a_call_takes_no_more_memory(max_new, cuda):
     cache = ops.KVCache.empty(1, 1, 4096, 8, 128, torch.float16, cuda)
     nbytes = ops.context(cuda).attention_cached_work(cache._ptr, 100000, 32, max_new or 0, 0, 0)
     assert nbytes <= 2 * 148 * 256 * 130 * 4
+
+
+@pytest.mark.parametrize("max_new", [1, 64, 100, 1 << 40])
+def test_append_hints_only_divide_the_work(max_new, cuda):
+    heads, dim, news = 2, 64, [700, 3, 130]
+    k, v = make_rows(sum(news), heads * dim, torch.bfloat16, cuda, 58), make_rows(sum(news), heads * dim, torch.bfloat16, cuda, 59)
+    cache = ops.KVCache.empty(36, 3, 11, heads, dim, torch.bfloat16, cuda)
+    scatter_table(cache, cuda)
+    cache.lens.copy_(torch.tensor(news, dtype=torch.int32))
+    ops.kv_append(cache, _kv.rows(k, heads, dim), _kv.rows(v, heads, dim), _kv.starts_of(news, cuda), max_new=max_new)
+    wait(cuda)
+    at = 0
+    for b, n in enumerate(news):
+        check_written(cache, b, heads, k[at:at + n].view(n, heads, dim), v[at:at + n].view(n, heads, dim))
+        at += n
+
+
+def test_evict_from_more_tokens_than_shared_memory_holds_keys_of(cuda):
+    cache = _kv.random_cache([50001, 300], 1, 64, torch.float16, cuda, seed=60, weights=True, extra=10)
+    cache.weight.mul_(16).floor_()                     # many equal ones
+    check_eviction(cache, 256, 4, 40, cuda)
