@@ -601,22 +601,10 @@ __global__ void __launch_bounds__(TcCfg<HD>::THREADS, 1) attend_tc(const __grid_
     }
 }
 
-template <typename F>
-cudaError_t allow(std::atomic<uint64_t>& ready, F* kernel, int bytes) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
-
 template <int DT, int HD>
 cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = allow(ready, attend_tc<DT, HD>, TcCfg<HD>::SMEM);
+    const cudaError_t e = allow_smem(ready, attend_tc<DT, HD>, TcCfg<HD>::SMEM);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned) (a.kv.heads * a.plan.grid), (unsigned) a.plan.nz);
     attend_tc<DT, HD><<<grid, TcCfg<HD>::THREADS, TcCfg<HD>::SMEM, st>>>(a);

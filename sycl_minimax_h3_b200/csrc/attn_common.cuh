@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -298,6 +299,19 @@ inline std::string make_rows_map(CUtensorMap* m, const void* base, bool int8, in
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return "cuTensorMapEncodeTiled failed (" + std::to_string((int) r) + ")";
     return {};
+}
+
+// A kernel's leave to use this much dynamic shared memory, asked for once per device: `ready` has a bit for each.
+template <typename F>
+cudaError_t allow_smem(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace h3

@@ -537,17 +537,6 @@ __global__ void int4_pack(const uint8_t* __restrict__ codes, long long N, long l
 
 }  // namespace
 
-template <typename F>
-cudaError_t allow(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {   // a bit per device: the attribute belongs to a device
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
-    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
 template <typename... A>
 cudaError_t in_clusters(void (*kernel)(A..., int), int blocks, long long chunks, int split, int threads, size_t smem,
                         cudaStream_t st, const A&... a) {
@@ -569,7 +558,7 @@ template <int DT, bool ZERO, bool G32, int MT>
 cudaError_t rows_mt(const Int4Args& a, int n_sm, cudaStream_t st) {
     constexpr int TERMS = DT == F32 ? 3 : 1;
     static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = allow(ready, int4_rows<DT, ZERO, G32, MT>, sizeof(RowsSmem<TERMS>));
+    const cudaError_t e = allow_smem(ready, int4_rows<DT, ZERO, G32, MT>, sizeof(RowsSmem<TERMS>));
     if (e != cudaSuccess) return e;
     const int blocks = (a.N + kRowsN - 1) / kRowsN, KP = (a.K + 127) / 128;
     const long long chunks = (a.M + 8 * MT - 1) / (8 * MT);
@@ -583,7 +572,7 @@ template <int DT, bool ZERO, int US, int NC>
 cudaError_t tc_nc(const Int4Args& a, int n_sm, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     constexpr size_t bytes = sizeof(TcSmem) + 1024;
-    const cudaError_t e = allow(ready, int4_tc<DT, ZERO, US, NC>, bytes);
+    const cudaError_t e = allow_smem(ready, int4_tc<DT, ZERO, US, NC>, bytes);
     if (e != cudaSuccess) return e;
     const int blocks = (a.N + 127) / 128, KT = (a.K + 63) / 64;
     const long long chunks = (a.M + 32 * NC - 1) / (32 * NC);

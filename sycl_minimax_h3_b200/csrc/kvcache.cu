@@ -1478,18 +1478,6 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
     return p;
 }
 
-template <typename F>
-cudaError_t allow_smem(std::atomic<uint64_t>& ready, F* kernel, size_t bytes) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
-    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
-
 template <int DT, int D, int NB>
 cudaError_t attend_nb(const AttendArgs& a, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};                 // a bit per device: the attribute belongs to a device
