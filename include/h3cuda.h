@@ -247,10 +247,15 @@ int h3s_kv_append(void* ctx, const h3s_kv_cache* kv, const void* k, const void* 
  * type dt) is token lens[b] - n + i of sequence b and sees the slots up to its own; query head h reads key/value head
  * h / (Hq / heads), scores q.k / sqrt(dim). out [T, Hq * dim] in dt; a row that sees nothing (lens[b] < n) is 0, rows
  * behind starts[seqs] are left as they were. An infinite or NaN value in the tail (a page's codes have none) makes its
- * feature infinite or NaN in every row that sees it, however small its weight. accumulate: weight[slot] += the sum of the slot's
- * softmax weights over the rows and heads that read it (kv->weight needed). max_new, max_len: what the largest n and
- * length are about (0: T, 64 * width), for the division of the work; none is wrong. work: work_bytes of device memory,
- * at least h3s_attention_cached_work(...) of the same arguments, on 16 bytes, this call's own until it has run. */
+ * feature infinite or NaN in every row that sees it, however small its weight. Scores, the softmax's maximum and sums and the
+ * sums of weighted values are held in float (these without the division: a value's size times a sequence's tokens stays
+ * below 2^113). What enters the products in fewer bits are the softmax's weights, as fp16 with a power of two per row for a
+ * 16-bit dt (off by up to 2^-11 of each) and as two fp16 terms for float32, and float32 queries, as two fp16 terms (2^-22).
+ * out is rounded once to dt. accumulate: weight[slot] += the sum of the slot's softmax weights over the rows and heads that
+ * read it (kv->weight needed; in any order for a page that sequences share). It scores the keys a second time, in a form
+ * made for single tokens: a long prompt takes several times as long with it. max_new, max_len: what the largest n and length
+ * are about (0: T, 64 * width), for the division of the work; none is wrong. work: work_bytes of device memory, at least
+ * h3s_attention_cached_work(...) of the same arguments, on 16 bytes, this call's own until it has run. */
 int h3s_attention_cached(void* ctx, const h3s_kv_cache* kv, const void* q, int64_t T, int64_t Hq, int64_t qs,
                          const int32_t* starts, int64_t max_new, int64_t max_len, void* out, int accumulate, void* work,
                          uint64_t work_bytes);
@@ -270,12 +275,12 @@ int h3s_kv_evict(void* ctx, const h3s_kv_cache* kv, int32_t* spare, int64_t budg
 /* A linear layer with 4-bit weights for a few rows of x, out = x . W^T + bias:
  *   W[n, k] = scale[k / group, n] * (code[n, k] - zero[k / group, n])      code 0..15, zero NULL: 8
  * x [M, K] in x_dt; scale and zero [ceil(K / group), N] in s_dt; bias float [N] or NULL; out [M, N] in out_dt, rounded
- * once from float. Sums are taken in float as sum x (code - 8) + (8 - zero) sum x and scaled per group; one that is not finite
- * is taken again, term by term in 64 bits, so that infinities and NaN come out as the definition has them and a sum that
- * passes float's largest only on its way comes out as it is. group 32, 64, 128 or 0 (one scale per output). tiles: the codes as h3s_int4_pack lays them out, 16 *
- * ceil(N / 16) * 64 * ceil(K / 64) / 2 bytes on 16 bytes. Any M is right (from some hundred rows on a matrix product on
- * unpacked weights is faster) up to 2,097,120; N up to 2^29 - 128, K up to 2^30; more is refused. M, K or N <= 0: nothing
- * to do, returns 0. */
+ * once from float. Sums are taken in float, as sum x (code - 8) + (8 - zero) sum x, and scaled per group; one that is not
+ * finite is taken again, term by term in 64 bits, so that infinities and NaN come out as the definition has them, and what
+ * passes float's largest only on its way as it is (an output of this kind costs a pass of one thread over its K terms).
+ * group 32, 64, 128 or 0 (one scale per output). tiles: the codes as h3s_int4_pack lays them out, 16 * ceil(N / 16) * 64 *
+ * ceil(K / 64) / 2 bytes on 16 bytes. Any M up to 2,097,120 is right (from some hundred rows on a matrix product on unpacked
+ * weights is faster); N up to 2^29 - 128, K up to 2^30; more is refused. M, K or N <= 0: nothing to do, returns 0. */
 int h3s_int4_linear(void* ctx, const void* x, int x_dt, int64_t M, int64_t K, const void* tiles, int64_t N,
                     const void* scale, const void* zero, int s_dt, int group, const float* bias, void* out, int out_dt);
 /* codes uint8 [N, K / 2] (K even), input 2 i in the low four bits of byte i -> tiles, once per layer. */

@@ -9,10 +9,12 @@
 // A stage's fence stands before the next loads: behind them it waits for their data (x by cp.async and fences: 40 us for
 // 48 rows, 4096 outputs of 14336 inputs; by tensor copies 27).
 // Measured, bf16, groups of 128: 48 x 14336 -> 4096 27 us (29 MB of codes, 209 TFLOP/s; mma.sync 35.5), groups of 64 29, of
-// 32 43; 64 x 14336 -> 16384 81 us (117 MB, 370 TFLOP/s; mma.sync 146). The roles wait for one another: the tensor pipe is
+// 32 43; with zero points 58, 63 and 74; 64 x 14336 -> 16384 81 us (117 MB, 370 TFLOP/s; mma.sync 146); 4096 -> 4096 at 256 rows
+// 30, at 1,024 112 us: the codes are unpacked again for every 64 rows. The roles wait for one another: the tensor pipe is
 // active 13 % and the schedulers issue 35 % of the time; unpacking eight codes is seven logic and four floating-point
 // instructions in eight warps, a wait that suspends resumes some hundred cycles late, and clusters, barriers and the sums at
-// the end are 5 us of every call.
+// the end are 5 us of every call. With zero points three warps take the sums of
+// every stage's rows beside (not profiled).
 #pragma once
 
 constexpr int kTcThreads = 512, kTcStages = 4, kTcBufs = 4, kTcCols = 64;

@@ -74,9 +74,11 @@ __device__ __forceinline__ T block_max(T x, T* red) {     // over 256 threads; e
 // One CTA per (sequence, head), block, and K or V. The CTA of the sequence's first block reads the old tail and, after
 // that, writes the new one: the two share slots.
 // A block's rows are read once, into registers (16 KB a CTA of 256 threads, four to an SM), since the maximum comes before
-// the codes; what bounds a prompt is the issue of the conversions (maximum, product, rounding check, packing), about as much
-// as the loads: three prompts of 700 to 4,133 tokens, 8 heads of 128 in fp16, 58 MB, 27 us (2.2 TB/s; the bytes alone 9). A
-// step of 48 single tokens is 8 us: one launch and three loads that follow from one another (start, length, page).
+// the codes: a CTA's loads, maximum and conversions (product, rounding check, packing) follow one another. Three prompts of
+// 700 to 4,133 tokens, 8 heads of 128 in fp16, 58 MB, are 25 us (2.3 TB/s; the bytes alone 9; float32 28 us): the schedulers
+// issue 64 % of the time with 37 % of an SM's warps, and wait for the loads and the barriers for most of the rest. A step of
+// 48 single tokens is 7 us (float32 5): three loads that follow from one another (start, length, page) in 768 CTAs of 256
+// threads, 1.3 rounds of what is resident, of which 16 threads have a row to move.
 constexpr int kAppThreads = 256;
 
 template <int DT, int D>
@@ -190,9 +192,11 @@ __global__ void __launch_bounds__(kAppThreads, DT == F32 ? 3 : 4) kv_append(cons
 //
 // Four warps per CTA take the pages of a piece in turn, each with a ring of two 8 KB tiles of its own that bulk copies fill:
 // no warp waits for another before the end. What bounds it, by lengths (bf16, 8 heads of 128, 4 queries each): 48 sequences
-// of 2,048 tokens 41 us (4.9 TB/s of codes; the bytes alone 31), of 200 to 8,191 88 us (4.9 TB/s; 66: pieces are whole pages and
-// their ends leave SMs idle), one of 131,037 51 us (5.3 TB/s; 41); one of 64 to 4,096 tokens 6 to 10 us (77: 8.1), which
-// are the loads that follow from one another, start and length, page id, codes and scale, tail, and the joining launch.
+// of 2,048 tokens 41 us (4.9 TB/s of codes; the bytes alone 31; float32 44 us), of 200 to 8,191 94 us (4.6 TB/s; 66: pieces are
+// whole pages and their ends leave SMs idle), one of 131,037 52 us (5.2 TB/s; 41; float32 57); one of 64 to 4,096 tokens 6 to 10
+// us (77: 8.3), which are the loads that follow from one another, start and length, page id, codes and scale, tail, and the
+// joining launch. 32 rows behind 16,384 tokens are 26 us (the bytes alone 5): each tile of 16 rows reads and unpacks the
+// codes for itself.
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -956,7 +960,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, NB == 1 ? 3 : 2) attend(const 
 }
 
 // The splits' partial results of a row as one: a CTA per row, whose warps take the splits in turn and then meet. The
-// partial results lie in L2; a launch that is ready when the pieces end makes it 2 to 3 us.
+// partial results lie in L2; a launch that is ready when the pieces end makes it 2 to 3 us. Not made for many rows: 16,000 of
+// two splits each (500 tokens behind 3,500, 32 heads) are 124 us, most of them a CTA's start and its loads one after another.
 constexpr int kJoinWarps = 8;
 template <int DT, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_constant__ AttendArgs a) {
@@ -1048,7 +1053,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
 // weight[slot] += the sum over the group's query rows of p = 2^(s - lse): the scores once more, against the finished
 // sums. One CTA per (sequence, kv head, piece of the pages), the last piece also the tail; a page's sums stay in one warp.
 // Reading the keys again costs less than keeping every score of the first pass would. 16 sequences of 100 to 4,500 tokens,
-// 2 heads of 64 with 8 queries each in float32: 13 us beside the attention's 14 and 6, all three bound by their first loads.
+// 2 heads of 64 with 8 queries each in float32: 13 us of the call's 23, all of its kernels bound by their first loads (here the
+// schedulers issue 23 % of the time). Not made for prompts: a row's query is laid out again for every page and 8 rows, and
+// 1,999 tokens behind 15,002 (32 heads of 128 over 8, fp16) take 4.24 ms with weights, 0.65 without. Pages that sequences
+// share take their sums in any order.
 template <int DT, int D>
 __global__ void __launch_bounds__(kAttWarps * 32) attend_weights(const __grid_constant__ AttendArgs a, int nzw) {
     constexpr bool TWO = DT == F32;
@@ -1176,7 +1184,7 @@ constexpr int kSelKeys = 48 * 1024;    // keys that fit shared memory; those of 
 // (sequence, head). The weights' keys are read once into shared memory; the key of the last kept one is found by four
 // passes over 8 bits of them each; then every thread counts the kept ones in a run of slots of its own, one scan over
 // the threads gives the places, and the runs are written down. Few CTAs with scans in a row bound it: 18 us for 12 sequences
-// of 3,500 to 8,111 tokens and 8 heads.
+// of 3,500 to 8,111 tokens and 8 heads, 96 CTAs on 148 SMs.
 __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ KvArgs kv, const int* __restrict__ spare,
                                                             int budget, int sinks, int recent, int* __restrict__ kept, int room) {
     extern __shared__ uint32_t keys[];
@@ -1313,9 +1321,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constan
 
 // 64 kept tokens of a (sequence, head) into one spare page, K and V side by side so that their loads are under way
 // together. TAIL: some of them lie in the tail (a sequence's last page or two).
-// A kept token's row is 128 bytes anywhere in the old pages: loads of that size, and the two passes over them in registers
-// (values and maximum, then codes), bound it: 12 sequences cut to 4,096 tokens, 8 heads of 128, 188 MB in 89 us (2.1 TB/s; the
-// bytes alone 29). Both passes take the codes exactly, code x scale in 64 bits where 32 are not sure of the rounding.
+// A kept token's row is 128 bytes anywhere in the old pages. 12 sequences cut to 4,096 tokens, 8 heads of 128, are 188 MB in 89
+// us (2.1 TB/s; the bytes alone 29): a CTA's loads, its pass for the maximum (twice, K and V) and its pass for the codes follow
+// one another with barriers between, and four CTAs are what an SM holds; the schedulers issue 62 % of the time and wait for
+// the barriers and the loads about equally. Both passes take the codes exactly, code x scale in 64 bits where 32 are not
+// sure of the rounding.
 template <int DT, int D, bool TAIL>
 __device__ __forceinline__ void gather_page(const KvArgs& kv, int h, size_t tbase, int page, const int* loc) {
     constexpr int C8 = D / 8, PER = 64 * C8 / 256;
@@ -1447,9 +1457,16 @@ cudaError_t launch_kv_append(const KvArgs& kv, const void* k, const void* v, lon
 }
 
 // Rows of a tile by how many rows a sequence brings (new tokens times the heads of a group): up to 8, 16, and for 16-bit
-// types from kTcRows on 256, on tcgen05. Measured at 32 / 64 rows per kv head, tiles of 16 against tcgen05, us: one
-// sequence of 16,384 tokens 48 / 64 against 44 / 44, four of 2,048 39 / 45 against 29 / 33, sixteen of 300 66 / 108 against
-// 23 / 23, one of 131,072 170 / 302 against 224 / 226; 64-wide heads at 16,384 31 / 38 against 40 / 41.
+// types from kTcRows on 256, on tcgen05. Tiles of 16 against tcgen05, us, 8 kv heads, at 32 / 48 / 64 / 96 / 128 rows of each:
+//   128 wide   1 x 16,384 tokens   26 / 37 / 44 / 61 / 75   against 44 / 47 / 47 / 51 / 54
+//              4 x 2,048           31 / 42 / 46 / 47 / 51           38 / 43 / 46 / 55 / 64
+//              16 x 300            25 / 48 / 50 / 39 / 57           22 / 22 / 23 / 22 / 22
+//   64 wide    1 x 16,384          19 / 25 / 30 / 39 / 49           39 / 39 / 41 / 43 / 43
+//              4 x 2,048           22 / 29 / 32 / 31 / 33           31 / 34 / 37 / 43 / 48
+//              16 x 300            16 / 30 / 31 / 26 / 37           18 / 18 / 18 / 18 / 18
+// and one of 131,072 at 48 / 64 / 128 rows 174 / 213 / 411 against 226 / 226 / 222 (64 wide: 109 / 135 / 259 against 207 / 208 / 204).
+// No one number is right for all: 48 is where many short sequences gain half, which for one long sequence costs a quarter up
+// to 60 rows, and more with 64-wide heads, up to some 100.
 constexpr int64_t kTcRows = 48;
 AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t group, int64_t T, int64_t max_new, int64_t max_len) {
     AttendPlan p{};
@@ -1466,12 +1483,16 @@ AttendPlan attend_plan(int n_sm, int dt, int64_t seqs, int64_t heads, int64_t gr
         p.entries = p.joined ? T * heads * group * p.nz : 0;
         return p;
     }
-    // two or three CTAs are resident on an SM. Units that are many, or as short as a piece may be, stay whole.
+    // two or three CTAs are resident on an SM. Units that are many, or as short as a piece may be, stay whole. Even batches
+    // would rather stay whole from twice the room on (100 sequences of 100 to 1,500 tokens and 8 heads: 49 us whole, 56 cut;
+    // 200 of 500 to 3,000: 140 and 152), but one long sequence among many then holds its few CTAs long after the others have
+    // ended (the 100 with one of 60,000: 427 us whole, 77 cut; 200: 543 and 116).
     const int64_t room = (int64_t) n_sm * (p.rows == 8 ? 3 : 2), units = tiles * heads;
     p.nz = 1;
     p.joined = units <= 8 * room && 2 * (pages + kTailPages) >= 3 * kChunk;
     // five sixths of that: pieces are rounded up to whole ones, and those that then find no room run after all the others
-    // (48 sequences of 200 to 8,191 tokens: 88 us, all of it 94; one of 131,037: 51 and 53)
+    // (48 sequences of 200 to 8,191 tokens: 94 us, all of it 100; one of 131,037: 52.1 and 53.3; 48 of 2,048 40.5 both; 16 of 500
+    // to 20,000: 73.4 and 73.0)
     p.room = p.joined ? (int) (room * 5 / 6) : 0;
     p.grid = (int) (units + p.room);                       // (the caller has seen to it that it is one)
     p.entries = p.joined ? (units + room) * p.rows : 0;

@@ -33,9 +33,9 @@ struct KvArgs {
 // How a call's queries and keys are divided (the same on the host and in every kernel of one call).
 struct AttendPlan {
     int rows;                          // query rows of a tile: 8 or 16, or 256 on tcgen05
-    // 8 or 16 rows: `grid` CTAs take the pieces of all (sequence, tile, head) units one after the other, the pieces of
-    // about as many pages as make `room` of them (0: every unit is one piece). 256: `grid` tiles (of all sequences) x
-    // heads x nz splits of the keys.
+    // 8 or 16 rows: a CTA for each piece that there can be of all (sequence, tile, head) units, units + room of them, whatever
+    // the hints; those without a piece return at once. The pieces have about as many pages as make `room` of them (0: every
+    // unit is one piece). 256: `grid` tiles (of all sequences) x heads x nz splits of the keys, one to a CTA.
     int grid, room, nz;
     bool joined;                       // partial results may be left, which attend_join brings together
     long long entries;                 // of partial rows

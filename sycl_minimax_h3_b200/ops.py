@@ -292,8 +292,9 @@ def attention_cached(q: Rows, cache: KVCache, starts: torch.Tensor, out: torch.T
     """Causal attention with grouped heads over the cache (``h3s_attention_cached``): query rows starts[b] .. starts[b+1] - 1
     are the last tokens of sequence b and see every token up to their own; out [q.tokens, q.heads * dim]. A row that sees
     nothing is 0; rows behind the last sequence are left as they were. ``accumulate`` adds the weight that every token
-    receives to ``cache.weight``. ``max_new`` and ``max_len`` (about the most new tokens, and the longest sequence) only
-    divide the work."""
+    receives to ``cache.weight`` (a second pass over the keys, made for single tokens: dear for a long prompt). Sums are held
+    in float32; the softmax's weights enter the products as fp16, or two fp16 terms for float32 rows. ``max_new`` and
+    ``max_len`` (about the most new tokens, and the longest sequence) only divide the work."""
     heads, dim = cache._sizes[1:3]
     if q.heads == 0 or q.heads % heads != 0:
         raise H3Error(f"attention_cached: {q.heads} query heads over {heads} key/value heads")
@@ -380,7 +381,8 @@ class Int4Linear:
         return self.n
 
     def forward(self, x: torch.Tensor, out: torch.Tensor) -> None:
-        """``out = linear(x)``: x [M, inputs] in a float type, out [M, outputs] in out's type."""
+        """``out = linear(x)``: x [M, inputs] in a float type, out [M, outputs] in out's type. Infinities and NaN come out as the
+        formula has them, also where the float32 sums do not hold them."""
         m = x.numel() // self.k if self.k else 0
         if x.numel() != m * self.k or out.numel() != m * self.n:
             raise H3Error(f"int4_linear: x {list(x.shape)} and out {list(out.shape)} do not fit a [{self.n}, {self.k}] weight")
