@@ -1,4 +1,4 @@
-"""Benchmark of the denoiser self-attention path (BASELINE.json metric: Sage attention ms/call and TOPS at 16.8k / 47k
+"""Benchmark of the denoiser self-attention path (Sage attention ms/call and TOPS at 16.8k / 47k
 tokens, % of the int8 tensor peak, 1/2/4/8 GPUs).
 
 One step = one h3s_attention call of the 47,232-token case (c3: 32 heads x 128, fp16 q/k/v as the strided parts of a

@@ -250,9 +250,10 @@ struct RopeArgs {
 // ---- the Sage pre-pass (kernels/h3sycl.cpp:1733-1761) --------------------------------------------------------------
 // With rope: q and k are normalised and rotated in place by the rms_rope kernel, as two h3s_rms_rope calls would (the
 // same bits): k first, since the K mean needs it, then q on the main stream while the K mean runs beside it (measured
-// at configs[3]: 0.63 against 0.70 ms for the step with both rotations before the fork). (A single pass that normalises q inside its quantiser, saving one read
-// of q, measured slower at configs[3]: its rotation is compute-bound and, running beside the K mean, slows the K mean's
-// chains, the pre-pass's critical path; the quantiser that runs there now is memory-bound.)
+// at 32 heads x 47,232 tokens: 0.63 against 0.70 ms for the step with both rotations before the fork). (A single pass
+// that normalises q inside its quantiser, saving one read of q, measured slower there: its rotation is compute-bound and,
+// running beside the K mean, slows the K mean's chains, the pre-pass's critical path; the quantiser that runs there now is
+// memory-bound.)
 template <int DT>
 int prepass_dt(Ctx& c, const void* q, const void* k, int64_t S, int64_t H, int64_t D, int64_t stride, int8_t* iq, int8_t* ik,
                float* sc, const RopeArgs* rope = nullptr) {

@@ -64,7 +64,7 @@ __device__ __forceinline__ void ld16(const void* p, float* out) {
 // ---- K mean, TMA ring ----------------------------------------------------------------------------------------------
 constexpr int kMeanCh = 64;          // channels per CTA: 128-byte rows of 16-bit k per token, two chain warps
 // The TMA ring of one K-mean CTA: 5 tiles of 32 KB. Beside the q quantiser, whose traffic lengthens the loads' latency,
-// a chain drained 3 tiles before the next arrived: measured at configs[3], the K mean beside the q quantiser took
+// a chain drained 3 tiles before the next arrived: measured at 32 heads x 47,232 tokens, the K mean beside the q quantiser took
 // 214.8 us with 96 KB, 196 us with 160 or 192 KB (167 us alone with any), the pre-pass 331 against 310.5 us.
 constexpr int kMeanRingBytes = 160 * 1024;
 constexpr int kMeanThreads = 32 + kMeanCh;   // warp 0: producer; warps 1-2: one thread per chain

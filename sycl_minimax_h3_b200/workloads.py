@@ -1,4 +1,4 @@
-"""Synthetic inputs of the benchmark configurations (BASELINE.json ``configs``).
+"""Synthetic inputs of the benchmark configurations.
 
 No public dataset is involved: the denoiser's q, k, v are stood in for by seeded normal values with the stated
 distributions. Q, V ~ N(0, 1); K = N(0, 1) + c[h, d], with the per-channel offset c ~ N(0, 4) drawn once per (head,
