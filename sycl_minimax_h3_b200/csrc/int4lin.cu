@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, DT == F32 ? 2 : 3) int4_few(con
         } else {
             s.x[0] = load_raw<DT>(a, row, kt * 64 + 8 * t, false);
             s.x[1] = load_raw<DT>(a, row, kt * 64 + 32 + 8 * t, false);
+            __syncwarp();                                  // the lanes part at the inputs' end, the products are the whole warp's
         }
         xp += kI4Warps * 64 * ES;
     };
@@ -402,6 +403,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows(const __grid_consta
                     terms<DT, TERMS>(load_raw<DT>(a, src[j], k, a.x_vec && k + 8 <= a.K), b);
 #pragma unroll
                     for (int e = 0; e < TERMS; ++e) to[e * kRowsM * 16] = make_uint4(b[e][0], b[e][1], b[e][2], b[e][3]);
+                    __syncwarp();                          // (a warp has whole rows) the lanes part at the inputs' end
                 }
             }
         }
