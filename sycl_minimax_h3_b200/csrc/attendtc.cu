@@ -74,8 +74,8 @@ __device__ __forceinline__ void codes16(const uint4 u, uint4& lo, uint4& hi) {
 // the exponent e that brings top into [2^13, 2^14) when divided by 2^e, and 2^-e in two normal factors
 __device__ __forceinline__ int exponent_of(float top) { return top > 0.0f ? ilogbf(top) - 13 : 0; }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // |e| <= 126
-// 2^d of a whole d <= 0, 0 below 2^-126
-__device__ __forceinline__ float pow2_down(float d) { return __int_as_float(max(0, 127 + (int) d) << 23); }
+// 2^d of a whole d <= 0, 0 below 2^-126 (the conversion saturates: also for -infinity)
+__device__ __forceinline__ float pow2_down(float d) { return __int_as_float(max(0, 127 + __float2int_rz(d)) << 23); }
 __device__ __forceinline__ uint4 halves8(const float (&x)[8], float m1, float m2) {
     uint32_t h[4];
 #pragma unroll
