@@ -1185,8 +1185,8 @@ constexpr int kSelKeys = 48 * 1024;    // keys that fit shared memory; those of 
 // passes over 8 bits of them each; then every thread counts the kept ones in a run of slots of its own, one scan over
 // the threads gives the places, and the runs are written down. Few CTAs with scans in a row bound it: 18 us for 12 sequences
 // of 3,500 to 8,111 tokens and 8 heads, 96 CTAs on 148 SMs.
-__global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ KvArgs kv, const int* __restrict__ spare,
-                                                            int budget, int sinks, int recent, int* __restrict__ kept, int room) {
+__global__ void __launch_bounds__(kSelThreads) evict_select(const __grid_constant__ KvArgs kv, const int* spare,
+                                                            int budget, int sinks, int recent, int* kept, int room) {
     extern __shared__ uint32_t keys[];
     __shared__ int hist[256];
     __shared__ int ssum[32], esum[32];
@@ -1402,28 +1402,28 @@ __device__ __forceinline__ void gather_page(const KvArgs& kv, int h, size_t tbas
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(256, 4) evict_gather(const __grid_constant__ KvArgs kv, const int* __restrict__ spare, int budget,
-                                                       const int* __restrict__ kept) {
+__global__ void __launch_bounds__(256, 4) evict_gather(const __grid_constant__ KvArgs kv, const int* spare, int budget,
+                                                       const int* kept) {
     __shared__ int loc[kPage];
     const int nb = budget / kPage, blk = blockIdx.y;
     const int b = (int) (blockIdx.x / kv.heads), h = (int) (blockIdx.x % kv.heads);
     const int* mine = kept + (size_t) blockIdx.x * budget;
     let_next_launch();
     wait_for_previous();
-    if (mine[0] == kLeftAlone) return;
+    if (fresh(mine) == kLeftAlone) return;
     const int page = spare[(size_t) b * nb + blk];
     int at = 0;
-    if (threadIdx.x < kPage) loc[threadIdx.x] = at = mine[blk * kPage + threadIdx.x];
+    if (threadIdx.x < kPage) loc[threadIdx.x] = at = fresh(mine + blk * kPage + threadIdx.x);
     const size_t tbase = (size_t) blockIdx.x * kPage;
     if (__syncthreads_or(at < 0)) gather_page<DT, D, true>(kv, h, tbase, page, loc);
     else gather_page<DT, D, false>(kv, h, tbase, page, loc);
 }
 
 // the new pages take the old ones' place in the table, which take theirs among the spare ones
-__global__ void __launch_bounds__(256) evict_swap(const KvArgs kv, int* __restrict__ spare, int budget, const int* __restrict__ kept) {
+__global__ void __launch_bounds__(256) evict_swap(const KvArgs kv, int* spare, int budget, const int* kept) {
     const int b = (int) blockIdx.x, nb = budget / kPage;
     wait_for_previous();
-    if (kept[(size_t) b * kv.heads * budget] == kLeftAlone) return;
+    if (fresh(kept + (size_t) b * kv.heads * budget) == kLeftAlone) return;
     for (int i = threadIdx.x; i < nb; i += 256) {
         int* p = kv.table + (size_t) b * kv.width + i;
         int* q = spare + (size_t) b * nb + i;

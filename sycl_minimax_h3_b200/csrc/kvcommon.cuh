@@ -12,6 +12,8 @@ namespace h3 {
 
 // The kernels of one call after its first are launched while the one before still runs (launch_after): they wait here for
 // all of it, and every kernel that one follows lets it be launched from its start on. Between calls nothing changes.
+// What they read of the one before they read through no const __restrict__ pointer: that would promise that nobody writes
+// there while the kernel runs, and lets the compiler load ahead of the wait.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... P, typename... A>
@@ -42,6 +44,12 @@ __device__ __forceinline__ Seq load_seq(const KvArgs& kv, const int* starts, lon
     s.L = kv.lens[b];
     s.ok = s.s0 >= 0 && s1 >= s.s0 && s1 <= T && s.L >= 0 && s.L / kPage <= kv.width;
     return s;
+}
+// A load that stays where it is written, and sees what was written before a wait_for_previous().
+__device__ __forceinline__ int fresh(const int* p) {
+    int x;
+    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(x) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return x;
 }
 __device__ __forceinline__ int quotient(int x, int d, int shift) { return shift >= 0 ? x >> shift : x / d; }   // x >= 0
 __device__ __forceinline__ bool page_ok(const KvArgs& kv, int page) { return page >= 0 && page < kv.pages; }

@@ -732,3 +732,36 @@ def test_evict_from_more_tokens_than_shared_memory_holds_keys_of(cuda):
     cache = _kv.random_cache([50001, 300], 1, 64, torch.float16, cuda, seed=60, weights=True, extra=10)
     cache.weight.mul_(16).floor_()                     # many equal ones
     check_eviction(cache, 256, 4, 40, cuda)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("stale", [-(1 << 31), 0, 77])
+def test_evict_does_not_go_by_what_work_held(dtype, stale, cuda):
+    """The same eviction with a work memory full of each of: what stands for a sequence that is left alone, and places of
+    other tokens. Its kernels are launched while the one before still runs: none may read work before that one has ended."""
+    heads, dim, budget, lens = 2, 64, 2 * PAGE, [129, 3000, 100, 700]
+    cache = _kv.random_cache(lens, heads, dim, dtype, cuda, seed=61, weights=True, extra=8)
+    used = set(cache.table[cache.table >= 0].tolist())
+    spare = torch.tensor([p for p in range(cache.k.shape[0]) if p not in used][:8], dtype=torch.int32, device=cuda).view(4, 2)
+    start = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.weight, cache.table, cache.lens, spare)]
+    work = torch.empty(4 * heads * budget, dtype=torch.int32, device=cuda)
+    plans = [expected_eviction(cache, b, budget, 4, 16) for b in range(4)]
+    before = [_kv.sequence(cache, b, "k") for b in range(4)]
+    weights = [_kv.seq_weights(cache, b) for b in range(4)]
+    for _ in range(40):
+        for t, was in zip((cache.k, cache.v, cache.k_scale, cache.v_scale, cache.weight, cache.table, cache.lens, spare), start):
+            t.copy_(was)
+        work.fill_(stale)
+        ops.context(cuda).kv_evict(cache._ptr, spare.data_ptr(), budget, 4, 16, work.data_ptr(), work.numel() * 4)
+        wait(cuda)
+        assert cache.lens.tolist() == [128, 128, 100, 128]
+        for b, plan in enumerate(plans):
+            if plan is None:
+                continue
+            w = _kv.seq_weights(cache, b)
+            for h in range(heads):
+                assert torch.equal(w[h], weights[b][h, plan[h]])
+                for j in range(2):
+                    page = int(cache.table[b, j])
+                    codes, scale = _kv.quantised(before[b][plan[h][j * PAGE:(j + 1) * PAGE], h])
+                    assert torch.equal(cache.k[page, h].cpu(), codes) and torch.equal(cache.k_scale[page, h].cpu(), scale)
