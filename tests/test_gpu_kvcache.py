@@ -765,3 +765,32 @@ def test_evict_does_not_go_by_what_work_held(dtype, stale, cuda):
                     page = int(cache.table[b, j])
                     codes, scale = _kv.quantised(before[b][plan[h][j * PAGE:(j + 1) * PAGE], h])
                     assert torch.equal(cache.k[page, h].cpu(), codes) and torch.equal(cache.k_scale[page, h].cpu(), scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,per,lens,news", [(8, 4, [9000], [1]), (4, 4, [3000, 70, 900] * 12, [1, 0, 1] * 12), (2, 4, [3000], [100]),
+                                                 (2, 4, [5000, 300], [5, 3])])
+def test_attention_does_not_go_by_what_work_held(dtype, heads, per, lens, news, cuda):
+    """The same bits whatever the work memory holds before the call, and the definition's values: pieces and splits that are
+    joined, and weights, by kernels that are launched while the one before still runs."""
+    cache = _kv.random_cache(lens, heads, 64, dtype, cuda, seed=62, weights=True)
+    q = make_rows(sum(news), heads * per * 64, dtype, cuda, 63)
+    starts = _kv.starts_of(news, cuda)
+    w0, t0 = cache.weight.clone(), cache.tail_weight.clone()
+    ctx, rows, first = ops.context(cuda), _kv.rows(q, heads * per, 64), None
+    nbytes = ctx.attention_cached_work(cache._ptr, sum(news), heads * per, max(news), max(lens), 1)
+    assert nbytes > 16 * sum(news) * heads * per           # there are partial results
+    work = torch.empty((nbytes + 15) // 16 * 4, device=cuda)
+    for held in (float("nan"), 0.0, float("inf"), -3e38, 1.4e-45) * 4:
+        work.fill_(held)
+        cache.weight.copy_(w0)
+        cache.tail_weight.copy_(t0)
+        out = torch.full_like(q, 7.0)
+        ctx.attention_cached(cache._ptr, rows.ptr(), sum(news), heads * per, rows.stride, starts.data_ptr(), max(news), max(lens),
+                             out.data_ptr(), 1, work.data_ptr(), nbytes)
+        wait(cuda)
+        if first is None:
+            check_attention(cache, q, starts, out, heads * per)
+            first = out, cache.weight.clone(), cache.tail_weight.clone()
+        for a, b in zip(first, (out, cache.weight, cache.tail_weight)):
+            assert torch.equal(a, b)
